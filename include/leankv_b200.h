@@ -473,6 +473,11 @@ int leankv_paged_table_step(int t_new, int B, int32_t* seq_len, int32_t* block_t
                             int32_t* kv_indptr, int32_t* kv_page_indices, int32_t* kv_last_page_len,
                             int32_t* start_pos, int32_t* status, void* stream);
 
+/* Cuts every one of B sequences back to at most `keep` tokens: the pages behind go back to the free stack (which holds `stack` entries),
+ * sequence 0's first, and the flat arrays have to be rebuilt (leankv_paged_table_step with t_new = 0). B <= 1024. */
+int leankv_paged_table_crop(int keep, int B, int32_t* seq_len, const int32_t* block_table, int max_pages_per_seq, int32_t* free_stack,
+                            int32_t* free_top, int stack, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

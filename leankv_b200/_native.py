@@ -1,5 +1,5 @@
-"""ctypes bindings of ``libleankv_b200.so`` and ``libleankv_mixers.so`` (the C ABI declared in
-``include/leankv_b200.h`` and ``include/leankv_mixers.h``).
+"""ctypes bindings of ``libleankv_b200.so``, ``libleankv_bytes.so`` and ``libleankv_mixers.so`` (the C ABI declared in
+``include/leankv_b200.h``, ``include/leankv_bytes.h`` and ``include/leankv_mixers.h``).
 
 There is no CPU or PyTorch fallback behind these calls: if the library is missing or a
 kernel reports an error, a ``RuntimeError`` is raised.
@@ -16,6 +16,7 @@ from ctypes import (POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_lon
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG_DIR, "libleankv_b200.so")
 MIXERS_PATH = os.path.join(_PKG_DIR, "libleankv_mixers.so")
+BYTES_PATH = os.path.join(_PKG_DIR, "libleankv_bytes.so")
 
 MAX_SEGMENTS = 4
 TQ_PAGE_TOKENS = 16
@@ -133,6 +134,7 @@ SIGNATURES = {
     "leankv_paged_table_begin": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p]),
     "leankv_paged_table_step": (c_int, [c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                                         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "leankv_paged_table_crop": (c_int, [c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
     "leankv_skinny_gemm_f16": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p]),
     "leankv_skinny_gemm_f16_status": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
     "leankv_silu_mul_f16": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p]),
@@ -270,12 +272,47 @@ MIXER_SIGNATURES = {
     "leankv_causal_step_workspace_bytes": (c_size_t, [POINTER(CausalAttn), c_int]),
     "leankv_causal_step": (c_int, [POINTER(CausalAttn), POINTER(CausalStep), c_void_p]),
 }
-_COMMON = ("leankv_strerror", "leankv_last_cuda_error", "leankv_abi_version")     # capi.cu, in both libraries
+
+
+# ── libleankv_bytes.so ────────────────────────────────────────────────
+
+BYTES_F16, BYTES_BF16, BYTES_F32 = 0, 1, 2
+BYTES_MAX_BATCH, BYTES_MAX_GROUP = 1024, 16
+
+
+class BytePool(Structure):
+    """Mirror of ``leankv_byte_pool_t``."""
+
+    _fields_ = [("dim", c_int), ("kv_heads", c_int), ("n_pages", c_int), ("chunks", c_void_p), ("bounds", c_void_p)]
+
+
+class Vectors(Structure):
+    """Mirror of ``leankv_vectors_t``."""
+
+    _fields_ = [("data", c_void_p), ("seq", c_longlong), ("head", c_longlong), ("token", c_longlong)]
+
+
+BYTE_SIGNATURES = {
+    "leankv_byte_chunk_bytes": (c_size_t, [c_int]),
+    "leankv_byte_bounds_bytes": (c_size_t, [c_int]),
+    "leankv_byte_append": (c_int, [POINTER(BytePool), c_int, POINTER(Vectors), POINTER(Vectors), c_int, c_int, c_void_p, c_void_p,
+                                   c_void_p, c_void_p]),
+    "leankv_byte_unpack": (c_int, [POINTER(BytePool), c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p,
+                                   c_void_p]),
+    "leankv_byte_attn_workspace_bytes": (c_size_t, []),
+    "leankv_byte_attn": (c_int, [POINTER(BytePool), c_int, POINTER(Vectors), POINTER(Vectors), c_int, c_int, c_int, c_float, c_void_p,
+                                 c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    "leankv_byte_select": (c_int, [POINTER(BytePool), c_int, POINTER(Vectors), c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
+                                   c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "leankv_byte_status": (c_int, [c_void_p, POINTER(c_int)]),
+}
+_COMMON = ("leankv_strerror", "leankv_last_cuda_error", "leankv_abi_version")     # capi.cu, in every library
 
 EUNSUPPORTED = -5
 
 _lib = None
 _mixers = None
+_byte_lib = None
 
 
 def _load(path: str, signatures: dict) -> ctypes.CDLL:
@@ -305,6 +342,14 @@ def mixers() -> ctypes.CDLL:
     if _mixers is None:
         _mixers = _load(MIXERS_PATH, {**MIXER_SIGNATURES, **{n: SIGNATURES[n] for n in _COMMON}})
     return _mixers
+
+
+def byte_lib() -> ctypes.CDLL:
+    """The library of the 8-bit paged cache, loaded once."""
+    global _byte_lib
+    if _byte_lib is None:
+        _byte_lib = _load(BYTES_PATH, {**BYTE_SIGNATURES, **{n: SIGNATURES[n] for n in _COMMON}})
+    return _byte_lib
 
 
 def check(code: int, what: str, handle=None) -> None:

@@ -1,7 +1,7 @@
 """Builds the C-ABI libraries in-tree with nvcc for sm_100a.
 
 Usage: ``python -m leankv_b200.build [--force] [--verbose]``. ``libleankv_b200.so`` holds the TEAL and
-TurboQuant kernels, ``libleankv_mixers.so`` the token mixers and dense layers; a model loads (and on
+TurboQuant kernels, ``libleankv_bytes.so`` those of the 8-bit paged cache, ``libleankv_mixers.so`` the token mixers and dense layers; a model loads (and on
 first use builds) the one it needs. The libraries are placed next to this file so that they travel
 with a snapshot of the source tree. nvcc cross-compiles without a GPU present.
 """
@@ -24,12 +24,14 @@ BUILD_DIR = os.path.join(PKG_DIR, "build")
 LIBRARIES = {
     "libleankv_b200.so": ["capi.cu", "teal_gemv.cu", "tq_quantize.cu", "tq_attn.cu", "decoder_ops.cu",
                           "decode_fused.cu", "skinny_gemm.cu"],
+    "libleankv_bytes.so": ["capi.cu", "byte_cache.cu", "byte_attn.cu", "byte_select.cu"],
     "libleankv_mixers.so": ["capi.cu", "dense_gemv.cu", "stream_ops.cu", "window_pool.cu",
                             "window_pool_tile.cu", "window_pool_mma.cu", "time_mix.cu", "mixer_step.cu", "causal_rows.cu", "causal_tile.cu",
                             "causal_step.cu"],
 }
 LIB_PATH = os.path.join(PKG_DIR, "libleankv_b200.so")
 MIXERS_PATH = os.path.join(PKG_DIR, "libleankv_mixers.so")
+BYTES_PATH = os.path.join(PKG_DIR, "libleankv_bytes.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

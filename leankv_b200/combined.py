@@ -13,6 +13,7 @@ from typing import Optional
 import torch
 
 from .teal.patching import apply_teal, remove_teal
+from .turboquant.byte_cache import ByteKVCache
 from .turboquant.cache import TurboQuantCache
 from .turboquant.paged_cache import PagedKVCache
 
@@ -48,15 +49,19 @@ def optimize_model(model, teal_sparsity: Optional[float] = None,
                    teal_thresholds_path: Optional[str] = None,
                    turboquant_bits: Optional[int] = None, use_paged_cache: bool = False,
                    page_size: int = 16, max_pages: int = 2048, use_triton: bool = False,
-                   fused_attention: bool = False, fused_prefill: bool = False):
+                   fused_attention: bool = False, fused_prefill: bool = False, sparse_blocks: Optional[int] = None):
     """Apply TEAL and/or build a TurboQuant cache; returns ``(model, cache)``.
 
     ``use_triton`` (an addition: the reference's ``optimize_model`` cannot select its kernel
     path, ``combined.py:83-87``) forwards to ``apply_teal`` and selects the CUDA sparse GEMV.
     ``fused_attention`` (an addition, paged cache only) registers the HF attention function of
     ``turboquant/hf_attention.py`` so that decode steps of ``model.generate`` run on the packed pages;
-    with ``fused_prefill`` prompt passes do too (causal masks only).
+    with ``fused_prefill`` prompt passes do too (causal masks only). A paged cache of ``turboquant_bits=8`` is a
+    ``ByteKVCache``: codes of 8 bits with a scale for each block of 16 tokens and head; with ``sparse_blocks`` its decode
+    steps read only that many blocks per kv head (needs ``fused_attention``).
     """
+    if sparse_blocks is not None and not (use_paged_cache and turboquant_bits == 8 and fused_attention):
+        raise ValueError("sparse_blocks needs use_paged_cache=True, turboquant_bits=8 and fused_attention=True")
     if teal_sparsity is not None or teal_thresholds_path is not None:
         apply_teal(model, sparsity=teal_sparsity, thresholds_path=teal_thresholds_path,
                    use_triton=use_triton)
@@ -71,16 +76,18 @@ def optimize_model(model, teal_sparsity: Optional[float] = None,
 
     cache = None
     if use_paged_cache:
-        cache = PagedKVCache(num_layers=num_layers, num_kv_heads=num_kv_heads, num_q_heads=num_q_heads,
-                             head_dim=head_dim, page_size=page_size, max_pages=max_pages,
-                             device=model.device, dtype=torch.float16,
-                             bits=turboquant_bits if turboquant_bits is not None else 3)
-        print(f"[LeanKV] PagedKVCache enabled (pages={max_pages}, page_size={page_size}, "
+        kind = ByteKVCache if turboquant_bits == 8 else PagedKVCache
+        held = model.dtype if turboquant_bits == 8 else torch.float16      # of what update() returns
+        cache = kind(num_layers=num_layers, num_kv_heads=num_kv_heads, num_q_heads=num_q_heads,
+                     head_dim=head_dim, page_size=page_size, max_pages=max_pages,
+                     device=model.device, dtype=held,
+                     bits=turboquant_bits if turboquant_bits is not None else 3)
+        print(f"[LeanKV] {kind.__name__} enabled (pages={max_pages}, page_size={page_size}, "
               f"pool={cache.get_total_pool_mb():.0f} MB)")
         if fused_attention:
             from .turboquant.hf_attention import enable_paged_attention
 
-            enable_paged_attention(model, cache, fused_prefill=fused_prefill)
+            enable_paged_attention(model, cache, fused_prefill=fused_prefill, sparse_blocks=sparse_blocks)
             print("[LeanKV] decode attention runs on the packed pages")
     elif turboquant_bits is not None:
         cache = TurboQuantCache(bits=turboquant_bits, head_dim=head_dim, num_layers=num_layers,

@@ -587,6 +587,44 @@ __global__ void __launch_bounds__(kTableThreads) paged_table_step_kernel(
     }
 }
 
+// One CTA. Pages behind the first ceil(keep / 16) of each sequence are pushed, in order, sequence 0 first. A stack that would not hold
+// them (it was not this table's) leaves everything as it is and sets status bit 0.
+__global__ void __launch_bounds__(kTableThreads) paged_table_crop_kernel(int keep, int B, int32_t* seq_len, const int32_t* block_table,
+                                                                         int pps_cap, int32_t* free_stack, int32_t* free_top, int stack,
+                                                                         int32_t* status) {
+    __shared__ int s_have[kTableThreads], s_first[kTableThreads], s_warp[kTableThreads / 32];
+    pdl_begin();
+    const int b = threadIdx.x, warp = b >> 5, lane = b & 31;
+    const int len = b < B ? seq_len[b] : 0, kept = (keep + 15) / 16;
+    const int have = (len + 15) / 16, drop = max(have - kept, 0);
+    int incl = drop;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const int add = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += add;
+    }
+    if (lane == 31) s_warp[warp] = incl;
+    const int top = *free_top;
+    __syncthreads();
+    int before = incl - drop, total = 0;
+    for (int w = 0; w < kTableThreads / 32; ++w) {
+        if (w < warp) before += s_warp[w];
+        total += s_warp[w];
+    }
+    s_have[b] = have;
+    s_first[b] = before;
+    const bool fits = top >= 0 && top + total <= stack;
+    if (b == 0) {
+        if (fits) *free_top = top + total;
+        else atomicOr(status, 1);
+    }
+    __syncthreads();
+    if (!fits) return;
+    if (b < B && len > keep) seq_len[b] = keep;
+    for (int s = warp; s < B; s += kTableThreads / 32)
+        for (int i = kept + lane; i < s_have[s]; i += 32) free_stack[top + s_first[s] + i - kept] = block_table[(size_t)s * pps_cap + i];
+}
+
 }  // namespace
 }  // namespace leankv
 
@@ -610,5 +648,14 @@ extern "C" int leankv_paged_table_step(int t_new, int B, int32_t* seq_len, int32
                                   static_cast<cudaStream_t>(stream), t_new, B, seq_len, block_table, max_pages_per_seq,
                                   free_stack, free_top, kv_indptr, kv_page_indices, kv_last_page_len, start_pos,
                                   status));
+    return LEANKV_OK;
+}
+
+extern "C" int leankv_paged_table_crop(int keep, int B, int32_t* seq_len, const int32_t* block_table, int max_pages_per_seq, int32_t* free_stack,
+                                       int32_t* free_top, int stack, int32_t* status, void* stream) {
+    if (keep < 0 || B <= 0 || max_pages_per_seq <= 0 || stack <= 0 || !seq_len || !block_table || !free_stack || !free_top || !status) return LEANKV_EINVAL;
+    if (B > kTableThreads) return LEANKV_ELIMIT;
+    LEANKV_CUDA_TRY(launch_early(paged_table_crop_kernel, dim3(1), dim3(kTableThreads), 0, static_cast<cudaStream_t>(stream), keep, B, seq_len,
+                                  block_table, max_pages_per_seq, free_stack, free_top, stack, status));
     return LEANKV_OK;
 }

@@ -1,0 +1,296 @@
+"""Paged KV cache in 8 bits, with attention over all of it or over the blocks that score best.
+
+The reference keeps fp16 pages (``leankv/turboquant/paged_cache.py``) or 3-bit codes (``leankv/turboquant/cache.py``); this cache stands
+between the two. A block is the 16 tokens of a page, of one kv head, keys or values: codes ``rint(x * 2^-e)`` in -127 .. 127
+and one scale 2^e, the smallest power of two that holds the block's largest magnitude. No rotation, no calibration; the error of a
+number is at most half a step, 1/254 to 1/127 of the block's largest magnitude. A token that joins a block may raise its scale; the
+codes that are there are then rounded once more. Powers of two make every rounding the same wherever it is done.
+
+The page table, its kernels and the HF surface are those of ``PagedKVCache``. Beside it: head sizes 64 and 128, any group of up to 16 query
+heads a kv head, keys, values and queries in fp16, bf16 or fp32, tensors of any strides of whole 16-byte pieces, ``crop``, and
+``sparse_decode_attention``, which reads the blocks whose upper bound of the query's scores is largest.
+
+    cache = ByteKVCache(num_layers=..., num_kv_heads=8, num_q_heads=32, dtype=torch.bfloat16, device="cuda")
+    cache.append(layer, k, v)                                   # [B, Hkv, T, D]
+    out = cache.prefill_attention(layer, q)                     # [B, Hq, T, D], the T tokens just appended
+    out = cache.decode_attention(layer, q)                      # [B, Hq, D]
+    out = cache.sparse_decode_attention(layer, q, blocks=128)   # the same, 128 blocks per kv head
+
+A cache is used by one stream at a time: its pages, its page table and the workspace of its attention are one set.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from ctypes import byref
+
+import torch
+
+from .. import _native
+from .paged_cache import PAGE, PagedKVCache
+
+_TYPES = {torch.float16: _native.BYTES_F16, torch.bfloat16: _native.BYTES_BF16, torch.float32: _native.BYTES_F32}
+
+
+def _vectors(t: torch.Tensor, token: bool = True) -> tuple:
+    """``[B, H, T, D]`` (or ``[B, H, D]``) as the kernels read it, and the tensor that they read: the one given where its vectors are
+    contiguous and begin at whole 16-byte pieces, else a copy."""
+    size = t.element_size()
+    strides = t.stride()
+    piece = 16 // size
+    if strides[-1] != 1 or t.data_ptr() % 16 or any(s % piece and n > 1 for s, n in zip(strides[:-1], t.shape[:-1])):
+        t = t.clone(memory_format=torch.contiguous_format)
+        strides = t.stride()
+    return _native.Vectors(t.data_ptr(), strides[0], strides[1], strides[2] if token else 0), t
+
+
+class ByteKVCache(PagedKVCache):
+    """Page pool of 8-bit keys and values + attention on it."""
+
+    def __init__(self, num_layers: int = 32, num_kv_heads: int = 8, num_q_heads: int = 32, head_dim: int = 128, page_size: int = 16,
+                 max_pages: int = 2048, dtype: torch.dtype = torch.float16, device=None, bits: int = 8):
+        if head_dim not in (64, 128) or page_size != PAGE or bits != 8:
+            raise RuntimeError("ByteKVCache kernels need head_dim 64 or 128, page_size=16, bits=8")
+        if num_layers < 1 or max_pages < 1 or num_kv_heads < 1 or num_q_heads % num_kv_heads or \
+                not 1 <= num_q_heads // num_kv_heads <= _native.BYTES_MAX_GROUP:
+            raise RuntimeError("ByteKVCache needs layers, pages and 1 to 16 query heads per kv head")
+        if dtype not in _TYPES:
+            raise RuntimeError("ByteKVCache returns float16, bfloat16 or float32")
+        self.num_layers = num_layers
+        self.num_kv_heads = num_kv_heads
+        self.num_q_heads = num_q_heads
+        self.head_dim = head_dim
+        self.page_size = page_size
+        self.max_pages = max_pages
+        self.bits = bits
+        self._dtype = dtype
+        self._device = torch.device(device) if device is not None else torch.device("cuda")
+        self._seen_tokens = 0
+
+        # [layer][page][kv head][keys | values | scales] and [layer][page][kv head][largest | smallest key code | scale]
+        self._chunk, self._bound = 32 * head_dim + 16, 2 * head_dim + 16
+        zeros = lambda n: torch.zeros(num_layers, max_pages, num_kv_heads, n, dtype=torch.uint8, device=self._device)
+        self.kv_data, self.bounds = zeros(self._chunk), zeros(self._bound)
+        self._pools = [_native.BytePool(head_dim, num_kv_heads, max_pages, self.kv_data[i].data_ptr(), self.bounds[i].data_ptr())
+                       for i in range(num_layers)]
+
+        self._seq_lengths: list[int] = []
+        self._batch_size = 0
+        self._free_count = max_pages
+        self.fused_decode = False
+        self.fused_prefill = False
+        self.sparse_blocks = None             # set by hf_attention.enable_paged_attention
+        # not on first use: a call that is being captured would record the clearing instead of doing it
+        size = _native.byte_lib().leankv_byte_attn_workspace_bytes() if self._device.type == "cuda" else 0
+        self._workspace = torch.zeros(size, dtype=torch.uint8, device=self._device)
+        self._scale = 1.0 / math.sqrt(head_dim)
+        self._alloc_tables(0)
+
+    # ── arguments ──────────────────────────────────────────────────────
+
+    def _layer(self, layer_idx: int):
+        if not 0 <= layer_idx < self.num_layers:
+            raise RuntimeError(f"ByteKVCache has layers 0 .. {self.num_layers - 1}, not {layer_idx}")
+        return byref(self._pools[layer_idx])
+
+    def _typed(self, t: torch.Tensor, name: str, *shape) -> torch.Tensor:
+        """``t`` after the checks that every call makes; a type that the kernels do not read becomes the cache's own."""
+        _native.require_cuda(t, name)
+        if t.device.index != (self.kv_data.device.index):
+            raise RuntimeError(f"{name} is on {t.device}, the cache on {self.kv_data.device}")
+        if t.dim() != len(shape) or any(want is not None and n != want for n, want in zip(t.shape, shape)) or t.shape[0] < 1:
+            want = ", ".join("*" if n is None else str(n) for n in shape)
+            raise RuntimeError(f"{name} must be [{want}], not {list(t.shape)}")
+        if t.shape[0] > _native.BYTES_MAX_BATCH:
+            raise RuntimeError(f"{name}: the page table holds up to {_native.BYTES_MAX_BATCH} sequences")
+        return t if t.dtype in _TYPES else t.to(self._dtype)
+
+    def check_blocks(self, blocks: int, sinks: int = 1, recent: int = 2) -> None:
+        if sinks < 0 or recent < 1 or blocks < sinks + recent:
+            raise RuntimeError("sparse attention needs recent >= 1, sinks >= 0 and blocks >= sinks + recent")
+
+    def _most_pages(self, batch: int) -> int:
+        return -(-max(self._seq_lengths[:batch]) // PAGE)
+
+    # ── appends ────────────────────────────────────────────────────────
+
+    def append(self, layer_idx: int, key_states: torch.Tensor, value_states: torch.Tensor):
+        """Codes of ``[B, Hkv, T_new, D]`` K/V of one layer go into the pages of the first B sequences. Layer 0 advances the page table
+        that all layers share; the other layers' tokens of the same step follow it."""
+        k = self._typed(key_states, "key_states", None, self.num_kv_heads, None, self.head_dim)
+        v = self._typed(value_states, "value_states", k.shape[0], self.num_kv_heads, k.shape[2], self.head_dim)
+        pool, lib = self._layer(layer_idx), _native.byte_lib()
+        batch, _, t_new, _ = k.shape
+        if k.dtype != v.dtype:
+            v = v.to(k.dtype)
+        if t_new == 0:
+            return
+        if layer_idx == 0:
+            known = self._seq_lengths
+            lengths = known[:batch] + [0] * (batch - len(known))
+            need = sum(-(-(n + t_new) // PAGE) - -(-n // PAGE) for n in lengths)
+            if need > self._free_count:
+                raise RuntimeError(f"ByteKVCache: out of pages ({self.max_pages} used). "
+                                   f"Increase max_pages or reduce batch/sequence length.")
+            self._ensure_batch_size(batch)
+            self._table_step(t_new, batch)
+            self._seen_tokens += t_new
+            self._free_count -= need
+            for b in range(batch):
+                known[b] += t_new
+        elif len(self._seq_lengths) < batch or min(self._seq_lengths[:batch]) < t_new:
+            raise RuntimeError("ByteKVCache: layer 0 has not appended these tokens yet")
+        indptr, flat, last = self._device_meta(batch)
+        (kd, k), (vd, v) = _vectors(k), _vectors(v)
+        with _native.on_device(self._device):
+            rc = lib.leankv_byte_append(pool, _TYPES[k.dtype], byref(kd), byref(vd), batch, t_new, indptr.data_ptr(), flat.data_ptr(),
+                                        last.data_ptr(), _native.current_stream())
+        _native.check(rc, "leankv_byte_append", lib)
+
+    def _gather_kv(self, layer_idx: int, batch_size: int):
+        """Dense ``[B, Hkv, max_seq, D]`` K and V in the cache's type (zeros behind a sequence's last token)."""
+        pool, lib = self._layer(layer_idx), _native.byte_lib()
+        max_seq = max(self._seq_lengths[:batch_size], default=0)
+        shape = (batch_size, self.num_kv_heads, max_seq, self.head_dim)
+        keys, values = (torch.empty(shape, dtype=self._dtype, device=self._device) for _ in range(2))
+        if batch_size and max_seq:
+            indptr, flat, last = self._device_meta(batch_size)
+            with _native.on_device(self._device):
+                rc = lib.leankv_byte_unpack(pool, _TYPES[self._dtype], keys.data_ptr(), values.data_ptr(), batch_size, max_seq,
+                                            indptr.data_ptr(), flat.data_ptr(), last.data_ptr(), _native.current_stream())
+            _native.check(rc, "leankv_byte_unpack", lib)
+        return keys, values
+
+    def unpack_sequence(self, layer_idx: int, batch_idx: int, which: int):
+        """Codes (int8 ``[Hkv, T, D]``) and scales (fp32 ``[Hkv, blocks]``) of one sequence's keys (0) or values (1)."""
+        self._layer(layer_idx)
+        t, d, h = self._seq_lengths[batch_idx], self.head_dim, self.num_kv_heads
+        n = -(-t // PAGE)
+        c = self.kv_data[layer_idx][self._block_table[batch_idx, :n].long()].transpose(0, 1).reshape(h, n, -1)
+        scales = c[..., 32 * d:32 * d + 8].contiguous().view(torch.float32)[..., which]
+        c = c[..., 16 * d * which:16 * d * (which + 1)]
+        if which == 0:
+            c = c.reshape(h, n, d // 64, PAGE, 64).permute(0, 1, 3, 2, 4).reshape(h, n * PAGE, d)
+        else:      # [part][g][t][word][token of four]: channel 32 part + 8 word + g, token 2 t + {0, 1, 8, 9}
+            c = c.reshape(h, n, d // 32, 8, 4, 4, 2, 2).permute(0, 1, 6, 4, 7, 2, 5, 3).reshape(h, n * PAGE, d)
+        return (c[:, :t].to(torch.int16) - 128).to(torch.int8), scales
+
+    # ── attention ──────────────────────────────────────────────────────
+
+    def _attend(self, layer_idx: int, q: torch.Tensor, out: torch.Tensor, tokens: int, lists=None, n_lists: int = 0) -> None:
+        """``q`` and ``out`` [B, Hq, (T,) D]: the last ``tokens`` tokens of each sequence over the pages."""
+        pool, lib, batch = self._layer(layer_idx), _native.byte_lib(), q.shape[0]
+        indptr, flat, last = self._device_meta(batch)
+        (qd, q), (od, _) = _vectors(q, q.dim() == 4), _vectors(out, q.dim() == 4)
+        with _native.on_device(self._device):
+            rc = lib.leankv_byte_attn(pool, _TYPES[q.dtype], byref(qd), byref(od), batch, self.num_q_heads, tokens, self._scale,
+                                      indptr.data_ptr(), flat.data_ptr(), last.data_ptr(), self._most_pages(batch), lists, n_lists,
+                                      self._workspace.data_ptr(), self._workspace.numel(), _native.current_stream())
+        _native.check(rc, "leankv_byte_attn", lib)
+
+    def decode_attention(self, layer_idx: int, query: torch.Tensor) -> torch.Tensor:
+        """``softmax(q K^T / sqrt(d)) V`` over every stored token of each sequence; query/out ``[B, Hq, D]``."""
+        q = self._typed(query, "query", None, self.num_q_heads, self.head_dim)
+        self._ensure_batch_size(q.shape[0])
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        self._attend(layer_idx, q, out, 1)
+        return out if out.dtype == query.dtype else out.to(query.dtype)
+
+    def sparse_decode_attention(self, layer_idx: int, query: torch.Tensor, blocks: int, sinks: int = 1, recent: int = 2,
+                                return_blocks: bool = False):
+        """``decode_attention`` that reads at most ``blocks`` blocks (of 16 tokens) per sequence and kv head: the first ``sinks``, the last
+        ``recent``, and those with the largest upper bound of the group's summed scores (from the largest and smallest key code of
+        each channel; ties to the earlier block). With ``return_blocks`` also their numbers, ascending and then -1, int32
+        ``[B, Hkv, blocks]``. A sequence of no more than ``blocks`` blocks is read whole."""
+        q = self._typed(query, "query", None, self.num_q_heads, self.head_dim)
+        self.check_blocks(blocks, sinks, recent)
+        batch = q.shape[0]
+        self._ensure_batch_size(batch)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        pages = self._most_pages(batch)
+        if pages <= blocks and not return_blocks:
+            self._attend(layer_idx, q, out, 1)
+        else:
+            pool, lib = self._layer(layer_idx), _native.byte_lib()
+            indptr, flat, _ = self._device_meta(batch)
+            chosen, ids = torch.empty(2, batch, self.num_kv_heads, blocks, dtype=torch.int32, device=q.device)
+            scores = torch.empty(batch * self.num_kv_heads * max(pages, 1), dtype=torch.float32, device=q.device)
+            qd, q = _vectors(q, False)
+            with _native.on_device(self._device):
+                rc = lib.leankv_byte_select(pool, _TYPES[q.dtype], byref(qd), batch, self.num_q_heads, indptr.data_ptr(),
+                                            flat.data_ptr(), pages, blocks, sinks, recent, chosen.data_ptr(), ids.data_ptr(),
+                                            scores.data_ptr(), _native.current_stream())
+            _native.check(rc, "leankv_byte_select", lib)
+            self._attend(layer_idx, q, out, 1, ids.data_ptr(), blocks)
+        out = out if out.dtype == query.dtype else out.to(query.dtype)
+        return (out, chosen) if return_blocks else out
+
+    def prefill_attention(self, layer_idx: int, query: torch.Tensor) -> torch.Tensor:
+        """Causal attention of the last T tokens of every sequence (the chunk that ``append`` has just added) over everything up to
+        each: query/out ``[B, Hq, T, D]``."""
+        q = self._typed(query, "query", None, self.num_q_heads, None, self.head_dim)
+        batch, _, t_new, _ = q.shape
+        if len(self._seq_lengths) < batch or min(self._seq_lengths[:batch]) < t_new:
+            raise RuntimeError("prefill_attention: the chunk has not been appended to this sequence")
+        out = torch.empty(batch, t_new, self.num_q_heads, self.head_dim, dtype=q.dtype, device=q.device).transpose(1, 2)
+        if t_new:
+            self._attend(layer_idx, q, out, t_new)
+        return out if out.dtype == query.dtype else out.to(query.dtype)
+
+    def kernel_status(self) -> int:
+        """Status word of the attention's bounded waits and page checks (0 = clean, bit 0: a wait ran out, bit 1: a page id outside
+        the pool)."""
+        val = ctypes.c_int(0)
+        if self._workspace.is_cuda:
+            with _native.on_device(self._device):
+                _native.check(_native.byte_lib().leankv_byte_status(self._workspace.data_ptr(), byref(val)), "leankv_byte_status",
+                              _native.byte_lib())
+        return val.value
+
+    # ── page table ─────────────────────────────────────────────────────
+
+    def crop(self, max_length: int):
+        """Cut every sequence back to at most ``max_length`` tokens (below zero: that many tokens fewer than the longest has), as after
+        drafted tokens that were not accepted. The scale of a block that keeps some tokens stays as it is."""
+        if max_length < 0:
+            max_length = max(self.get_seq_length() + max_length, 0)
+        batch = len(self._seq_lengths)
+        if not batch or max(self._seq_lengths) <= max_length:
+            return
+        with _native.on_device(self._device):
+            rc = _native.lib().leankv_paged_table_crop(max_length, batch, self._seq_len_dev.data_ptr(), self._block_table.data_ptr(),
+                                                       self._pps_cap, self._free_stack.data_ptr(), self._free_top.data_ptr(),
+                                                       self.max_pages, self._status.data_ptr(), _native.current_stream())
+        _native.check(rc, "leankv_paged_table_crop")
+        kept = -(-max_length // PAGE)
+        for b, n in enumerate(self._seq_lengths):
+            if n > max_length:
+                self._free_count += -(-n // PAGE) - kept
+                self._seq_lengths[b] = max_length
+        self._meta_batch = -1
+
+    def reset(self):
+        """Forget every sequence. Pages need no clearing: only positions that have been written are read."""
+        if self._device.type != "cuda":
+            return super().reset()
+        with _native.on_device(self._device):
+            # the status word, the free stack and its height lie one behind the other
+            words = 4 + -(-self.max_pages // 4) * 4
+            rc = _native.lib().leankv_paged_table_begin(self._status.data_ptr(), 4, self.max_pages, words, _native.current_stream())
+        _native.check(rc, "leankv_paged_table_begin")
+        self._seq_len_dev.zero_()
+        self._seq_lengths = []
+        self._batch_size = 0
+        self._seen_tokens = 0
+        self._free_count = self.max_pages
+        self._meta_batch = -1
+
+    # ── diagnostics ────────────────────────────────────────────────────
+
+    def bytes_per_page(self) -> int:
+        """Bytes one page occupies in one layer (K and V, all kv heads, with the blocks' bounds)."""
+        return self.num_kv_heads * (self._chunk + self._bound)
+
+    def get_total_pool_mb(self) -> float:
+        return (self.kv_data.numel() + self.bounds.numel()) / 1e6

@@ -18,6 +18,8 @@ Prompt passes (more than one query token) take the dense route through SDPA unle
 
 from __future__ import annotations
 
+from typing import Optional
+
 import torch
 
 ATTN_NAME = "leankv_paged"
@@ -46,7 +48,11 @@ def paged_attention_forward(module, query, key, value, attention_mask, dropout: 
                 "the paged decode kernel cannot apply an attention mask that hides cached positions "
                 "(padded batches of unequal prompt length, sliding-window attention): run such inputs "
                 "with disable_paged_attention(model), which takes the dense SDPA route")
-        out = cache.decode_attention(module.layer_idx, query[:, :, 0, :])        # [B, Hq, D]
+        few = getattr(cache, "sparse_blocks", None)
+        if few:
+            out = cache.sparse_decode_attention(module.layer_idx, query[:, :, 0, :], few)
+        else:
+            out = cache.decode_attention(module.layer_idx, query[:, :, 0, :])    # [B, Hq, D]
         return out.unsqueeze(1), None
     if cache is not None and query.shape[2] > 1 and getattr(cache, "fused_decode", False) and \
             getattr(cache, "fused_prefill", False):
@@ -95,9 +101,16 @@ def _attention_modules(model):
     return [layer.self_attn for layer in inner.layers]
 
 
-def enable_paged_attention(model, cache, fused_prefill: bool = False) -> None:
+def enable_paged_attention(model, cache, fused_prefill: bool = False, sparse_blocks: Optional[int] = None) -> None:
     """Route ``model``'s decode-step attention through ``cache.decode_attention`` and, with
-    ``fused_prefill``, its prompt passes through ``cache.prefill_attention`` (causal masks only)."""
+    ``fused_prefill``, its prompt passes through ``cache.prefill_attention`` (causal masks only). With ``sparse_blocks`` (a
+    ``ByteKVCache``) decode steps read that many 16-token blocks per kv head, those that score best
+    (``cache.sparse_decode_attention``)."""
+    if sparse_blocks is not None:
+        if not hasattr(cache, "sparse_decode_attention"):
+            raise RuntimeError("sparse_blocks needs a cache that selects blocks: ByteKVCache")
+        cache.check_blocks(sparse_blocks)
+        cache.sparse_blocks = sparse_blocks
     register()
     for attn in _attention_modules(model):
         attn._leankv_paged_cache = cache
@@ -113,6 +126,8 @@ def disable_paged_attention(model) -> None:
         if cache is not None:
             cache.fused_decode = False
             cache.fused_prefill = False
+            if getattr(cache, "sparse_blocks", None) is not None:
+                cache.sparse_blocks = None
             del attn._leankv_paged_cache
     prev = getattr(model, "_leankv_prev_attn", None)
     if prev is not None:

@@ -1,0 +1,521 @@
+"""The 8-bit paged cache on the GPU against its definition in 64 bits (``oracle/bytes.py``).
+
+Codes, scales, bounds and chosen blocks have to be equal: every rounding in them is of an exact number. Attention: the kernels
+form scores, weights and sums in 32 bits from exact codes and a query of 22 bits or more, weights enter as two 11-bit parts. A score is a sum of
+``dim`` products in fp32 (tensor-core sums drop bits of 2^-22 of the largest term at worst), |s| up to some 20 in these tests, so a weight is off by at most
+2^-22 * 20 * 2 ~ 1e-5 of itself, and so is an output relative to its row; then one rounding to the output type, eps / 2 at most. Bound: relative 2-norm
+over a row ``eps / 2 + 2e-5``.
+"""
+
+import math
+
+import pytest
+import torch
+
+from leankv_b200 import _native
+from leankv_b200.turboquant.byte_cache import ByteKVCache
+from oracle import bytes as obytes
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+def vectors(gen, batch, heads, tokens, dim, dtype, large=True):
+    x = torch.randn(batch, heads, tokens, dim, generator=gen)
+    if large:
+        x[..., ::dim // 4] *= 8
+    return x.to(dtype)
+
+
+def row_errors(got, want):
+    """Relative 2-norm of each row's error; rows that should be zero have to be."""
+    got, want = got.double().cpu().flatten(0, -2), want.flatten(0, -2)
+    size = want.norm(dim=-1)
+    assert bool((got[size == 0] == 0).all())
+    return ((got - want).norm(dim=-1) / size.clamp_min(1e-300))[size > 0]
+
+
+def close(got, want, dtype):
+    err = row_errors(got, want)
+    assert got.dtype == dtype
+    bound = torch.finfo(dtype).eps / 2 + 2e-5
+    assert len(err) == 0 or float(err.max()) <= bound, (float(err.max()), bound)
+
+
+class Pair:
+    """A cache on the GPU and its definition, given the same tokens."""
+
+    def __init__(self, batch, heads, group, dim, dtype, pages=64, layers=1, seed=0):
+        self.gen = torch.Generator().manual_seed(seed)
+        self.batch, self.heads, self.group, self.dim, self.dtype = batch, heads, group, dim, dtype
+        self.cache = ByteKVCache(num_layers=layers, num_kv_heads=heads, num_q_heads=heads * group, head_dim=dim, max_pages=pages, dtype=dtype, device=DEV)
+        self.plain = obytes.Cache(batch, heads, dim)
+
+    def append(self, tokens, batch=None, scale=1.0, layer=0):
+        k, v = ((vectors(self.gen, batch or self.batch, self.heads, tokens, self.dim, torch.float32) * scale).to(self.dtype) for _ in range(2))
+        self.cache.append(layer, k.to(DEV), v.to(DEV))
+        self.plain.append(k, v)
+
+    def queries(self, tokens=None):
+        shape = (self.batch, self.heads * self.group) + (() if tokens is None else (tokens,)) + (self.dim,)
+        return torch.randn(shape, generator=self.gen).to(self.dtype)
+
+    def check_pages(self, layer=0):
+        for b in range(self.batch):
+            if self.plain.n[b] == 0:
+                continue
+            for which in range(2):
+                codes, scales = self.cache.unpack_sequence(layer, b, which)
+                assert torch.equal(codes.cpu().double(), self.plain.codes(b, which))
+                assert torch.equal(scales.cpu().double().nan_to_num(-1.0), self.plain.scales(b, which).nan_to_num(-1.0))
+            ids = self.cache._block_table[b, :-(-self.plain.n[b] // 16)].long()
+            rec = self.cache.bounds[layer][ids].cpu()
+            for h in range(self.heads):
+                for j, block in enumerate(self.plain.blocks[0][b][h]):
+                    got = rec[j, h, :2 * self.dim].contiguous().view(torch.int8).double()
+                    assert torch.equal(got[:self.dim], block.codes.amax(0)) and torch.equal(got[self.dim:], block.codes.amin(0))
+
+    def check_decode(self):
+        q = self.queries()
+        got = self.cache.decode_attention(0, q.to(DEV))
+        want = torch.stack([self.plain.attend(b, q[b, :, None])[:, 0] for b in range(self.batch)])
+        close(got, want, self.dtype)
+        assert self.cache.kernel_status() == 0
+
+    def check_prompt(self, tokens):
+        q = self.queries(tokens)
+        got = self.cache.prefill_attention(0, q.to(DEV))
+        want = torch.stack([self.plain.attend(b, q[b]) for b in range(self.batch)])
+        close(got, want, self.dtype)
+        assert self.cache.kernel_status() == 0
+
+    def check_sparse(self, blocks, sinks=1, recent=2):
+        q = self.queries()
+        got, chosen = self.cache.sparse_decode_attention(0, q.to(DEV), blocks, sinks, recent, return_blocks=True)
+        for b in range(self.batch):
+            want = self.plain.choose(b, q[b], blocks, sinks, recent)
+            assert torch.equal(chosen[b].cpu(), want), (b, chosen[b].cpu(), want)
+            close(got[b], self.plain.attend(b, q[b, :, None], want)[:, 0], self.dtype)
+        again = self.cache.sparse_decode_attention(0, q.to(DEV), blocks, sinks, recent)
+        assert torch.equal(again, got) and self.cache.kernel_status() == 0
+        return chosen
+
+
+# ── pages ────────────────────────────────────────────────────────────────────────────────────────────────────
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("chunks", [(1,), (16,), (17, 1, 1, 13), (5, 40, 3), (1, 2, 1, 33, 1, 1)])
+def test_codes_scales_and_bounds_are_those_of_the_definition(dtype, dim, chunks):
+    p = Pair(3, 2, 2, dim, dtype, seed=sum(chunks) + dim)
+    for i, n in enumerate(chunks):
+        p.append(n, scale=[1.0, 3.0, 1e-3, 40.0][i % 4])
+        p.check_pages()
+    keys, values = p.cache[0]
+    for b in range(3):
+        for got, which in ((keys, 0), (values, 1)):
+            assert got.dtype == dtype and torch.equal(got[b].cpu(), p.plain.values(b, which).to(dtype))
+
+
+def test_ragged_sequences_keep_their_own_scales():
+    p = Pair(4, 3, 1, 64, BF16)
+    p.append(21)
+    p.append(9, batch=2, scale=7.0)
+    p.append(1, batch=3, scale=0.1)
+    p.append(2, scale=30.0)
+    p.check_pages()
+    keys, _ = p.cache[0]
+    assert keys.shape == (4, 3, 33, 64)
+    assert bool((keys[3, :, 23:] == 0).all()) and bool((keys[2, :, 24:] == 0).all())
+    p.check_decode()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_smallest_and_largest_magnitudes(dtype):
+    p = Pair(1, 2, 1, 64, dtype)
+    for scale in (0.0, 1e-40, 1e-30, 1e30):
+        p.append(16, scale=scale)
+    p.append(3, scale=0.0)
+    p.append(2, scale=1e-20)
+    p.check_pages()
+
+
+def test_an_fp16_block_whose_largest_code_stands_for_more_than_fp16_holds():
+    p = Pair(1, 1, 1, 64, F16)
+    k = torch.full((1, 1, 4, 64), 65504.0, dtype=F16)
+    p.cache.append(0, k.to(DEV), (-k).to(DEV))
+    p.plain.append(k, -k)
+    p.check_pages()
+    keys, values = p.cache[0]
+    assert bool((keys == 65504).all()) and bool((values == -65504).all())
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("which", [0, 1])
+def test_a_block_that_holds_no_number_answers_nobody_who_sees_it(bad, which):
+    p = Pair(2, 2, 2, 64, BF16)
+    p.append(32)
+    k, v = (vectors(p.gen, 2, 2, 20, 64, BF16) for _ in range(2))
+    (k, v)[which][0, 1, 2, 5] = bad                    # position 34 of sequence 0, head 1: block 2
+    p.cache.append(0, k.to(DEV), v.to(DEV))
+    p.plain.append(k, v)
+    p.check_pages()
+    q = p.queries()
+    got = p.cache.decode_attention(0, q.to(DEV)).cpu()
+    assert bool(got[0, 2:].isnan().all())
+    q20 = p.queries(20)
+    prompt = p.cache.prefill_attention(0, q20.to(DEV)).cpu()
+    assert bool(prompt[0, 2:].isnan().all())           # every token of the chunk shares the block or comes behind it
+    q40 = p.queries(40)                                # positions 12 .. 51; those before 32 do not see block 2
+    wide = p.cache.prefill_attention(0, q40.to(DEV))
+    assert bool(wide[0, 2:, 20:].isnan().all())
+    want = [p.plain.attend(b, q40[b]) for b in range(2)]
+    close(wide[0, :2], want[0][:2], BF16)
+    close(wide[1], want[1], BF16)
+    cut = obytes.Cache(2, 2, 64)
+    cut.blocks = [[[row[:2] for row in seq] for seq in side] for side in p.plain.blocks]
+    cut.n = [32, 32]
+    close(wide[0, 2:, :20], cut.attend(0, q40[0, :, :20])[2:], BF16)
+    # the block counts as the best one of all
+    sparse, chosen = p.cache.sparse_decode_attention(0, q.to(DEV), 3, 0, 1, return_blocks=True)
+    if which == 0:
+        assert 2 in chosen[0, 1].tolist() and bool(sparse[0, 2:].isnan().all())
+    p.append(30)                                       # the block is full by now and stays as it is
+    p.check_pages()
+    assert p.cache.kernel_status() == 0
+
+
+def test_crop_gives_pages_back_and_the_next_tokens_join_what_is_left():
+    p = Pair(3, 2, 1, 128, F16, pages=24)
+    p.append(50)
+    p.append(20, batch=1)
+    used = p.cache.get_pages_used()
+    for keep, then in ((64, 3), (41, 9), (32, 1), (17, 2), (0, 33)):
+        p.cache.crop(keep)
+        p.plain.crop(keep)
+        assert p.cache._seq_lengths == p.plain.n
+        assert p.cache.get_pages_used() == sum(-(-n // 16) for n in p.plain.n) <= used
+        if keep:
+            p.check_decode()
+        p.append(then, scale=2.0)
+        p.check_pages()
+        p.check_decode()
+    p.cache.crop(-3)
+    assert p.cache.get_seq_length() == max(p.plain.n) - 3 and p.cache.page_table_status() == 0
+    free = p.cache._free_stack[:p.cache._free_count].tolist()
+    held = [i for b, n in enumerate(p.cache._seq_lengths) for i in p.cache._block_table[b, :-(-n // 16)].tolist()]
+    assert sorted(free + held) == list(range(24)) and int(p.cache._free_top) == len(free)
+
+
+def test_a_full_pool_is_refused_and_leaves_the_cache_as_it_was():
+    p = Pair(2, 1, 1, 64, F16, pages=6)
+    p.append(40)
+    with pytest.raises(RuntimeError, match="out of pages"):
+        p.append(20)
+    assert p.cache._seq_lengths == [40, 40] and p.cache.get_pages_used() == 6
+    p.plain.n = [40, 40]
+    p.check_pages()
+    p.check_decode()
+    p.cache.reset()
+    assert p.cache.get_pages_used() == 0 and p.cache.get_seq_length() == 0
+    p.plain = obytes.Cache(2, 1, 64)
+    p.append(48)
+    p.check_pages()
+
+
+def test_arguments_that_do_not_fit_are_refused():
+    p = Pair(2, 2, 3, 64, F16, layers=2)
+    k = torch.zeros(2, 2, 4, 64, dtype=F16, device=DEV)
+    for bad in (k[:, :1], k[..., :32], k[0], torch.zeros(1025, 2, 1, 64, dtype=F16, device=DEV), k[:0]):
+        with pytest.raises(RuntimeError):
+            p.cache.append(0, bad, bad)
+    with pytest.raises(RuntimeError):
+        p.cache.append(0, k, k[:, :, :3])
+    with pytest.raises(RuntimeError, match="layers"):
+        p.cache.append(2, k, k)
+    with pytest.raises(RuntimeError, match="layer 0"):
+        p.cache.append(1, k, k)
+    assert p.cache._seq_lengths in ([], [0, 0])
+    p.cache.append(0, k, k)
+    with pytest.raises(RuntimeError, match="appended"):
+        p.cache.prefill_attention(0, torch.zeros(2, 6, 5, 64, dtype=F16, device=DEV))
+    for bad in (torch.zeros(2, 5, 64, dtype=F16, device=DEV), torch.zeros(2, 6, 32, dtype=F16, device=DEV), torch.zeros(6, 64, dtype=F16, device=DEV)):
+        with pytest.raises(RuntimeError):
+            p.cache.decode_attention(0, bad)
+
+
+# ── attention ────────────────────────────────────────────────────────────────────────────────────────────────
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("group", [1, 4, 7, 8, 9, 16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_decode_attention_for_every_group_and_type(dtype, group, dim):
+    p = Pair(3, 2, group, dim, dtype, seed=group)
+    p.append(37)
+    p.append(70, batch=2)
+    p.append(1, batch=1)
+    p.check_decode()
+
+
+@pytest.mark.parametrize("tokens", [1, 2, 15, 16, 17, 31, 64, 127, 129, 500, 1025])
+def test_decode_attention_for_lengths_around_blocks_and_shares(tokens):
+    p = Pair(2, 1, 4, 128, F16, pages=200, seed=tokens)
+    p.append(tokens)
+    p.check_decode()
+
+
+def test_sequences_without_tokens_get_zeros():
+    p = Pair(5, 2, 3, 64, BF16)
+    p.append(20, batch=2)
+    p.check_decode()                                   # sequences 2 .. 4 are empty
+    p.cache.crop(0)
+    p.plain.crop(0)
+    p.check_decode()
+
+
+@pytest.mark.parametrize("batch, heads, tokens", [(1, 1, 9000), (1, 8, 3000), (7, 3, 1111), (70, 2, 90)])
+def test_shares_of_many_thread_blocks_add_up(batch, heads, tokens):
+    p = Pair(batch, heads, 4, 128, F16, pages=batch * (tokens // 16 + 6) + 8, seed=batch)
+    p.append(tokens)
+    p.append(73, batch=(batch + 1) // 2)
+    p.check_decode()
+    q = p.queries().to(DEV)
+    first = p.cache.decode_attention(0, q)
+    assert all(torch.equal(p.cache.decode_attention(0, q), first) for _ in range(5))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("dim, group, heads", [(64, 3, 2), (128, 4, 1), (128, 7, 2), (64, 16, 1)])
+@pytest.mark.parametrize("past, tokens", [(0, 2), (0, 33), (5, 12), (70, 31), (250, 5)])
+def test_prompt_attention_is_causal(dtype, dim, group, heads, past, tokens):
+    p = Pair(2, heads, group, dim, dtype, seed=past + tokens)
+    if past:
+        p.append(past)
+    p.append(tokens)
+    p.check_prompt(tokens)
+
+
+def test_prompt_attention_of_sequences_of_different_lengths():
+    p = Pair(3, 2, 4, 128, F16)
+    p.append(30, batch=1)
+    p.append(17, batch=2)
+    p.append(40)
+    p.check_prompt(40)
+    p.check_prompt(3)                                  # any number of last tokens, not only the last chunk's
+
+
+def test_weights_far_apart_and_rows_that_grow():
+    """Scores that rise block by block, and one token that outweighs all others."""
+    p = Pair(1, 1, 4, 64, F32, pages=80)
+    k = torch.randn(1, 1, 1000, 64, generator=p.gen) * (1 + torch.arange(1000) / 100.0)[None, None, :, None]
+    k[0, 0, 700] *= 30
+    v = torch.randn(1, 1, 1000, 64, generator=p.gen) * torch.logspace(-6, 6, 1000)[None, None, torch.randperm(1000, generator=p.gen), None]
+    p.cache.append(0, k.to(DEV), v.to(DEV))
+    p.plain.append(k, v)
+    q = p.queries() * 0.05
+    got = p.cache.decode_attention(0, q.to(DEV))
+    want = p.plain.attend(0, q[0, :, None])[:, 0][None]
+    # |s| reaches some 60 here, and the values' magnitudes differ by 2^40: what counts is the error relative to the weighted magnitudes
+    size = p.plain.values(0, 1).abs()[0]
+    w = torch.softmax(p.plain.values(0, 0)[0] @ q[0].double().T / 8, 0).T
+    assert bool(((got.cpu().double() - want).abs()[0] <= 1e-4 * (w @ size)).all())
+
+
+def test_queries_of_any_scale():
+    for dtype, scale in ((BF16, 1e-30), (BF16, 1e4), (F32, 1e-35), (F32, 1e-3), (F16, 1e-4)):
+        p = Pair(1, 2, 3, 64, dtype)
+        p.append(50, scale=0.1 if scale > 1 else 1.0)
+        q = (p.queries().float() * scale).to(dtype)
+        if scale > 1:
+            q = (q.float() * 1e-3).to(dtype)
+        got = p.cache.decode_attention(0, q.to(DEV))
+        close(got, p.plain.attend(0, q[0, :, None])[:, 0][None], dtype)
+    p = Pair(1, 1, 2, 64, F32)
+    p.append(50)
+    zero = p.cache.decode_attention(0, torch.zeros(1, 2, 64, device=DEV))
+    close(zero, p.plain.attend(0, torch.zeros(2, 1, 64))[:, 0][None], F32)
+
+
+def test_other_strides_other_types_and_views():
+    p = Pair(2, 2, 3, 64, BF16)
+    k = vectors(p.gen, 2, 40, 2, 64, BF16).transpose(1, 2)          # [B, T, H, D] as a projection leaves it
+    v = vectors(p.gen, 2, 2, 40, 2 * 64, BF16)[..., 64:]
+    p.cache.append(0, k.to(DEV).transpose(1, 2).contiguous().transpose(1, 2), v.to(DEV))
+    p.plain.append(k, v)
+    p.check_pages()
+    q = torch.randn(2, 40, 6, 64, generator=p.gen).to(BF16)
+    on = q.to(DEV)
+    whole = p.cache.prefill_attention(0, on.transpose(1, 2))
+    close(whole, torch.stack([p.plain.attend(b, q[b].transpose(0, 1)) for b in range(2)]), BF16)
+    one = p.cache.decode_attention(0, on.transpose(1, 2)[:, :, 7])
+    assert torch.equal(one, p.cache.decode_attention(0, on[:, 7].contiguous()))
+    odd = torch.zeros(2, 6, 68, dtype=BF16, device=DEV)
+    odd[..., 3:67] = on[:, 7]
+    assert torch.equal(p.cache.decode_attention(0, odd[..., 3:67]), one)
+    double = p.cache.decode_attention(0, on[:, 7].double())          # a type that no kernel reads goes through the cache's own
+    assert double.dtype == torch.float64 and torch.equal(double.to(BF16), one)
+    mixed = p.cache.decode_attention(0, on[:, 7].float())            # queries need not be of the cache's type
+    close(mixed, torch.stack([p.plain.attend(b, q[b, 7, :, None])[:, 0] for b in range(2)]), F32)
+
+
+# ── blocks by score ──────────────────────────────────────────────────────────────────────────────────────────
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("dim, group", [(64, 1), (64, 16), (128, 4), (128, 5)])
+@pytest.mark.parametrize("blocks, sinks, recent", [(4, 1, 2), (7, 0, 1), (9, 3, 5), (40, 1, 2)])
+def test_chosen_blocks_are_the_best_ones(dtype, dim, group, blocks, sinks, recent):
+    p = Pair(3, 2, group, dim, dtype, pages=100, seed=blocks)
+    p.append(150)
+    p.append(203, batch=2)
+    p.append(60, batch=1)
+    p.check_sparse(blocks, sinks, recent)
+
+
+@pytest.mark.parametrize("tokens", [1, 16, 48, 63, 64, 65, 80, 81])
+def test_short_sequences_are_read_whole(tokens):
+    p = Pair(2, 1, 2, 64, F16, seed=tokens)
+    p.append(tokens)
+    chosen = p.check_sparse(4)
+    assert chosen.shape == (2, 1, 4)
+    q = p.queries().to(DEV)
+    if tokens <= 64:
+        assert torch.equal(p.cache.sparse_decode_attention(0, q, 4), p.cache.decode_attention(0, q))
+
+
+def test_equal_scores_go_to_the_earlier_block():
+    p = Pair(1, 2, 2, 64, F16, pages=64)
+    k = vectors(p.gen, 1, 2, 16, 64, F16).repeat(1, 1, 50, 1)       # every block is the same
+    p.cache.append(0, k.to(DEV), k.to(DEV))
+    p.plain.append(k, k)
+    assert p.check_sparse(9, 1, 2)[0, 0].tolist() == [0, 1, 2, 3, 4, 5, 6, 48, 49]
+    p.cache.reset()
+    p.plain = obytes.Cache(1, 2, 64)
+    zeros = torch.zeros(1, 2, 700, 64, dtype=F16)
+    p.cache.append(0, zeros.to(DEV), k[:, :, :700].to(DEV))
+    p.plain.append(zeros, k[:, :, :700])
+    assert p.check_sparse(6, 0, 1)[0, 1].tolist() == [0, 1, 2, 3, 4, 43]
+
+
+@pytest.mark.parametrize("tokens, blocks", [(70000, 300), (16 * 4097, 33), (270000, 17)])
+def test_choice_among_many_blocks(tokens, blocks):
+    """More blocks than a small CTA, and than any CTA, keeps in registers; scores against the definition, vectorised."""
+    gen = torch.Generator(device=DEV).manual_seed(tokens)
+    cache = ByteKVCache(num_layers=1, num_kv_heads=1, num_q_heads=2, head_dim=64, max_pages=tokens // 16 + 1, dtype=F16, device=DEV)
+    k = torch.randn(1, 1, tokens, 64, generator=gen, device=DEV).to(F16)
+    cache.append(0, k, k)
+    q = torch.randn(1, 2, 64, generator=gen, device=DEV).to(F16)
+    out, chosen = cache.sparse_decode_attention(0, q, blocks, return_blocks=True)
+    codes, scales = cache.unpack_sequence(0, 0, 0)
+    n = scales.shape[1]
+    c = codes[0].double()[:16 * (tokens // 16)].view(-1, 16, 64)
+    e = obytes.least_exponent(float(q.abs().max()), 2047)
+    i = torch.round(q[0].double() * 2.0 ** -e)
+    u = c.amax(1) @ i.clamp(min=0).sum(0) + c.amin(1) @ i.clamp(max=0).sum(0)
+    score = u.float() * scales[0, :len(u)]
+    score[0] = math.inf
+    score = torch.cat([score, score.new_full((n - len(score),), 0.0)])
+    score[n - 2:] = math.inf
+    want = torch.sort(score, descending=True, stable=True).indices[:blocks].sort().values
+    assert torch.equal(chosen[0, 0].long(), want)
+    kk = (codes[0].double() * scales[0].double().repeat_interleave(16)[:tokens, None])
+    at = (want[:, None] * 16 + torch.arange(16, device=DEV)).flatten()
+    at = at[at < tokens]
+    w = torch.softmax(q[0].double() @ kk[at].T / 8, -1)
+    vc, vs = cache.unpack_sequence(0, 0, 1)
+    close(out[0], (w @ (vc[0].double() * vs[0].double().repeat_interleave(16)[:tokens, None])[at]).cpu(), F16)
+
+
+# ── as they are used ─────────────────────────────────────────────────────────────────────────────────────────
+
+def test_a_prompt_in_chunks_then_single_tokens_on_several_layers():
+    p = Pair(2, 2, 4, 128, BF16, layers=3, pages=40)
+    plains = [p.plain] + [obytes.Cache(2, 2, 128) for _ in range(2)]
+    for tokens in (33, 16, 1, 1, 7, 1):
+        for layer in range(3):
+            p.plain = plains[layer]
+            p.append(tokens, layer=layer)
+            q = p.queries(tokens)
+            got = p.cache.prefill_attention(layer, q.to(DEV)) if tokens > 1 else p.cache.decode_attention(layer, q[:, :, 0].to(DEV))[:, :, None]
+            close(got, torch.stack([p.plain.attend(b, q[b]) for b in range(2)]), BF16)
+    for layer in range(3):
+        p.plain = plains[layer]
+        p.check_pages(layer)
+    assert p.cache.seen_tokens == 59 and p.cache.get_seq_length() == 59
+
+
+def test_update_returns_the_dense_cache():
+    p = Pair(2, 2, 1, 64, F16)
+    for tokens in (20, 1):
+        k, v = (vectors(p.gen, 2, 2, tokens, 64, F16) for _ in range(2))
+        dense = p.cache.update(k.to(DEV), v.to(DEV), 0)
+        p.plain.append(k, v)
+        for which in range(2):
+            assert torch.equal(dense[which].cpu(), torch.stack([p.plain.values(b, which) for b in range(2)]).to(F16))
+
+
+def test_captured_calls_on_another_stream_replay_on_new_inputs():
+    p = Pair(2, 2, 4, 128, F16, pages=80)
+    p.append(450)
+    q = p.queries().to(DEV)
+    p.cache.decode_attention(0, q)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dense = p.cache.decode_attention(0, q)
+        few, chosen = p.cache.sparse_decode_attention(0, q, 8, return_blocks=True)
+        prompt = p.cache.prefill_attention(0, q[:, :, None].expand(-1, -1, 3, -1))
+    for _ in range(3):
+        new = p.queries()
+        q.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        close(dense, torch.stack([p.plain.attend(b, new[b, :, None])[:, 0] for b in range(2)]), F16)
+        for b in range(2):
+            want = p.plain.choose(b, new[b], 8, 1, 2)
+            assert torch.equal(chosen[b].cpu(), want)
+            close(few[b], p.plain.attend(b, new[b, :, None], want)[:, 0], F16)
+        close(prompt, torch.stack([p.plain.attend(b, new[b, :, None].expand(-1, 3, -1)) for b in range(2)]), F16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = p.cache.decode_attention(0, q)
+    side.synchronize()
+    assert torch.equal(again, dense) and p.cache.kernel_status() == 0
+
+
+def test_pages_beyond_four_gigabytes():
+    """The free stack hands out the last pages first: offsets of 6 GB and of 3 GB into the pool."""
+    p = Pair(2, 8, 2, 128, F16, pages=200_000)
+    assert p.cache.kv_data.numel() > 6 * 2 ** 30
+    p.append(40)
+    assert int(p.cache._block_table[0, 0]) > 199_000
+    p.check_pages()
+    p.check_decode()
+    p.check_prompt(5)
+    p.append(200)
+    p.check_sparse(6)
+
+
+def test_page_ids_outside_the_pool_are_reported_and_left_alone():
+    """The kernels check every id against the pool: nothing is read or written there, the other sequences are answered."""
+    p = Pair(3, 2, 2, 64, F16)
+    p.append(40)
+    before = p.cache.kv_data.clone()
+    p.cache._device_meta(3)
+    flat = p.cache._kv_page_indices
+    good = flat.clone()
+    for bad in (64, 1 << 30, -1, -(1 << 31)):
+        flat[4] = bad                                  # sequence 1's second page
+        q = p.queries()
+        got = p.cache.decode_attention(0, q.to(DEV))
+        for b in (0, 2):
+            close(got[b], p.plain.attend(b, q[b, :, None])[:, 0], F16)
+        p.cache.sparse_decode_attention(0, q.to(DEV), 2, 0, 1)
+        p.cache.prefill_attention(0, q[:, :, None].expand(-1, -1, 9, -1).to(DEV))
+        assert p.cache.kernel_status() == 2
+        p.cache._workspace[:4].zero_()
+        assert p.cache[0][0].shape == (3, 2, 40, 64)
+        assert torch.equal(p.cache.kv_data, before)
+    flat.copy_(good)
+    p.check_decode()
