@@ -62,16 +62,23 @@ int leankv_byte_unpack(const leankv_byte_pool_t* pool /* host */, int dtype, voi
 /* Attention of the last `tokens` tokens of each of B sequences over the cache, causal among themselves: q_heads / kv_heads (up to
  * LEANKV_BYTES_MAX_GROUP) query heads share a kv head; q and out of `dtype`. Softmax statistics and sums are fp32. A sequence
  * without tokens, and a query before the first token, gets zeros.
- * max_pages_seq: an upper bound of any sequence's pages, for the launch's size.
+ * max_pages_seq, total_pages: upper bounds of any sequence's pages and of all sequences' together, for the launch's shape.
  * blocks = NULL: every page. Else (tokens = 1) the pages of sequence b and kv head h are block_pages[(b * kv_heads + h) * n_blocks ..], as
  * many as there are blocks or n_blocks, the last of them the sequence's last page (leankv_byte_select writes such lists).
  * The workspace is zero-filled once; its first word is a status (0 = clean; leankv_byte_status): bit 0 a bounded wait ran out, bit 1 a page
- * id outside the pool. The launches of two streams need a workspace each. */
+ * id outside the pool, bit 2 more pages than total_pages (nothing was written). The launches of two streams need a workspace each. */
 size_t leankv_byte_attn_workspace_bytes(void);       /* the same for all shapes */
 int leankv_byte_attn(const leankv_byte_pool_t* pool /* host */, int dtype, const leankv_vectors_t* q /* host */,
                      const leankv_vectors_t* out /* host */, int B, int q_heads, int tokens, float scale, const int32_t* kv_indptr,
-                     const int32_t* kv_page_indices, const int32_t* kv_last_page_len, int max_pages_seq,
+                     const int32_t* kv_page_indices, const int32_t* kv_last_page_len, int max_pages_seq, long long total_pages,
                      const int32_t* block_pages, int n_blocks, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The same for longer chunks of prompts, on tcgen05 (256 (token, head) rows against 128 keys at a time); q and out fp16 or bf16 (fp32:
+ * LEANKV_EUNSUPPORTED), scale > 0. Weights enter the value product as fp16. The workspace is the one above. */
+int leankv_byte_prompt_attn(const leankv_byte_pool_t* pool /* host */, int dtype, const leankv_vectors_t* q /* host */,
+                            const leankv_vectors_t* out /* host */, int B, int q_heads, int tokens, float scale,
+                            const int32_t* kv_indptr, const int32_t* kv_page_indices, const int32_t* kv_last_page_len,
+                            int max_pages_seq, void* workspace, size_t workspace_bytes, void* stream);
 
 /* The blocks that one query token of each sequence reads, for each kv head: all of them where there are no more than n_blocks; else the
  * first `sinks`, the last `recent` (>= 1; sinks + recent <= n_blocks) and those with the largest score, ties to the lower block.

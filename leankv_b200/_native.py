@@ -301,7 +301,9 @@ BYTE_SIGNATURES = {
                                    c_void_p]),
     "leankv_byte_attn_workspace_bytes": (c_size_t, []),
     "leankv_byte_attn": (c_int, [POINTER(BytePool), c_int, POINTER(Vectors), POINTER(Vectors), c_int, c_int, c_int, c_float, c_void_p,
-                                 c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+                                 c_void_p, c_void_p, c_int, c_longlong, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    "leankv_byte_prompt_attn": (c_int, [POINTER(BytePool), c_int, POINTER(Vectors), POINTER(Vectors), c_int, c_int, c_int, c_float,
+                                        c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
     "leankv_byte_select": (c_int, [POINTER(BytePool), c_int, POINTER(Vectors), c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
                                    c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
     "leankv_byte_status": (c_int, [c_void_p, POINTER(c_int)]),

@@ -15,15 +15,17 @@
 // Bound: a chunk's 2 * 16 * dim + 16 bytes come once from memory. They come by one bulk copy into a ring of a warp's own (4 to 8 chunks ahead), 190 KB in
 // flight on an SM; the tensor cores and some 300 issue slots a page and warp run under that.
 //
-// Split: all pages of all (sequence, kv head, row tile) triples are one flat list, the grid one wave of CTAs with equal shares. A share is cut at
-// the triples' borders; a triple that several CTAs share leaves partial sums in the workspace, and the last CTA to arrive adds
-// them up in the CTAs' order, so that results do not depend on timing.
+// Split. A cluster of CTAs has one (sequence, kv head, row tile) triple or, where there are fewer triples than the device has room for clusters, an equal part of
+// its pages; the CTAs share those pages and add their sums up through distributed shared memory, each a slice of the rows. Parts of one triple meet in the workspace:
+// the last CTA to arrive adds them in order. Nothing depends on timing. (16 sequences around 4096 tokens, 8 kv heads: one flat list of pages cut into equal shares, joined
+// in the workspace, took 36.8 us: shares that crossed a border ran twice through the start, and every join cost some 4 us.)
 
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
 
 #include "byte_layout.cuh"
+#include "byte_workspace.cuh"
 #include "umma.cuh"
 
 namespace leankv {
@@ -32,23 +34,20 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kCtasPerSm = 3;
-constexpr int kMinPages = 8;                       // of a CTA
+constexpr int kCtasPerSm = 4;
+constexpr int kMaxCluster = 8;
+constexpr int kFewPages = 4;                       // of a CTA: below, a smaller cluster
+constexpr int kPartPages = 32;                     // of a CTA: below, a triple is not cut into parts (joining them costs 2 - 3 us)
+constexpr int kWavePages = 64;                     // of a CTA where there is more than one wave of them
 // A row's reference lies kLift below the largest score seen when it last moved, and moves when a score exceeds it by more than kReach: weights are at most
 // 2^15 in fp16, and one of 2^-24 of the largest is still a normal number there. Moving costs the rescaling of all sums.
 constexpr float kLift = 10.f, kReach = 15.f;
 constexpr float kNoRef = -1.0e30f;                 // a maximum before any score: finite, so that masked scores give weight 0
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kCounters = 4096;
-constexpr int kStatusWords = 64;
-constexpr int kMaxCtas = 1024;
-constexpr int kTimedOut = 1, kBadPage = 2;
-
-__host__ __device__ constexpr int stages(int dim) { return dim == 128 ? 4 : 8; }
+constexpr int kJoin = 32;                          // parts of a triple that are joined at a time
+__host__ __device__ constexpr int stages(int dim) { return dim == 128 ? 3 : 6; }
 __host__ __device__ constexpr int row_floats(int dim) { return dim + 4; }               // a row of the warps' sums in shared memory: no bank is met twice
 __host__ __device__ constexpr size_t ring_bytes(int dim) { return (size_t)kWarps * stages(dim) * chunk_bytes(dim); }
-__host__ __device__ constexpr size_t partial_floats(int dim, int rows) { return (size_t)rows * (dim + 2); }
-constexpr size_t kWorkspaceBytes = 4 * (size_t)kStatusWords + 4 * (size_t)kCounters + 2 * (size_t)kMaxCtas * partial_floats(128, 16) * 4;
 
 struct AttnParams {
     const uint8_t* chunks;
@@ -60,6 +59,7 @@ struct AttnParams {
     const int32_t* last;
     const int32_t* lists;                          // [B][H][n_lists] page ids, or null: every page
     int n_lists;
+    int part_pages;                                // a triple of more pages is cut into parts; 0: none is
     int* status;
     unsigned* counters;
     float* partials;
@@ -100,6 +100,26 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
 }
 __device__ __forceinline__ float2 unpack_f16(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
 
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Numbers at a shared address of this CTA's, as the CTA `rank` of the cluster has them there.
+__device__ __forceinline__ uint32_t peer(uint32_t at, int rank) {
+    uint32_t there;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
+    return there;
+}
+__device__ __forceinline__ float2 peer_f32x2(uint32_t at, int rank) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(peer(at, rank)));
+    return v;
+}
+__device__ __forceinline__ float4 peer_f32x4(uint32_t at, int rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(peer(at, rank)));
+    return v;
+}
+
 template <typename T>
 __device__ __forceinline__ void store4_as(T* to, float4 v) {
     if constexpr (std::is_same<T, float>::value) *reinterpret_cast<float4*>(to) = v;
@@ -118,11 +138,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_kernel(const AttnPa
     constexpr int kPitch = row_floats(D);
     extern __shared__ __align__(128) uint8_t s_ring[];
     __shared__ __align__(8) uint64_t s_bar[kWarps][kStages];
-    __shared__ int s_first[LEANKV_BYTES_MAX_BATCH + 1];              // pages of the sequences before b
+    __shared__ int s_first[LEANKV_BYTES_MAX_BATCH + 1];              // parts of the sequences before b, for each (head, row tile)
     __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
+    __shared__ float2 s_ml[kRows];                                   // of the CTA
     __shared__ int s_sum[kWarps];
     __shared__ int s_last;
-    static_assert((size_t)kWarps * kRows * kPitch * 4 <= ring_bytes(D), "the warps' sums lie over the ring");
+    static_assert((size_t)(kWarps + 1) * kRows * kPitch * 4 <= ring_bytes(D) && (3 * kJoin * kRows + kThreads) * 4 <= ring_bytes(D), "sums lie over the ring");
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     if (lane == 0) {
@@ -133,14 +154,25 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_kernel(const AttnPa
     __syncwarp();
     pdl_begin();
 
-    // ---- pages of each sequence, added up ----
-    const int ip0 = p.indptr[0];
-    if (p.lists == nullptr) {
-        for (int i = tid; i <= p.B; i += kThreads) s_first[i] = p.indptr[i] - ip0;
+    unsigned rank, ctas;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
+    const int unit = blockIdx.x / ctas, HR = p.H * p.row_tiles, rows_all = p.tokens * p.G;
+
+    // ---- the cluster's triple, and its part of the pages ----
+    auto held = [&](int b) {                           // pages that sequence b's triples read
+        const int n = p.indptr[b + 1] - p.indptr[b];
+        return p.lists == nullptr ? n : min(n, p.n_lists);
+    };
+    int b, hr, part = 0, parts = 1;
+    if (p.part_pages == 0) {
+        b = unit / HR;
+        hr = unit - b * HR;
     } else {
         const int per = (p.B + kThreads - 1) / kThreads, from = min(tid * per, p.B), to = min(from + per, p.B);
+        auto parts_of = [&](int i) { return max(1, (held(i) + p.part_pages - 1) / p.part_pages); };
         int sum = 0;
-        for (int i = from; i < to; ++i) sum += min(p.indptr[i + 1] - p.indptr[i], p.n_lists);
+        for (int i = from; i < to; ++i) sum += parts_of(i);
         int incl = sum;
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) {
@@ -153,329 +185,406 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_kernel(const AttnPa
         for (int w = 0; w < warp; ++w) run += s_sum[w];
         for (int i = from; i < to; ++i) {
             s_first[i] = run;
-            run += min(p.indptr[i + 1] - p.indptr[i], p.n_lists);
+            run += parts_of(i);
         }
         if (to == p.B) s_first[p.B] = run;             // every thread with to = B has the same sum
+        __syncthreads();
+        if (s_first[p.B] * HR > (int)(gridDim.x / ctas)) {                 // more pages than the caller's bound: parts would be missing
+            if (unit == 0 && rank == 0 && tid == 0) atomicOr(p.status, kTooMany);
+            return;
+        }
+        if (unit >= s_first[p.B] * HR) return;         // the whole cluster: the grid was sized for the bound
+        b = 0;
+        for (int step = 512; step > 0; step >>= 1)
+            if (b + step < p.B && s_first[b + step] * HR <= unit) b += step;
+        parts = s_first[b + 1] - s_first[b];
+        part = unit - s_first[b] * HR;
+        hr = part / parts;
+        part -= hr * parts;
     }
-    __syncthreads();
-
-    const int HR = p.H * p.row_tiles, rows_all = p.tokens * p.G;
-    auto out_row = [&](int b, int hr, int r) -> T* {       // row r of a tile; null where there is none
-        const int h = hr / p.row_tiles, row = (hr - h * p.row_tiles) * kRows + r;
+    const int ip = p.indptr[b], all_pages = p.indptr[b + 1] - ip, length = (all_pages - 1) * kPage + p.last[b];
+    const int have = p.lists == nullptr ? all_pages : min(all_pages, p.n_lists);
+    const int h = hr / p.row_tiles, row0 = (hr - h * p.row_tiles) * kRows;
+    const int32_t* ids = p.lists == nullptr ? p.indices + ip : p.lists + ((long long)b * p.H + h) * p.n_lists;
+    auto share = [](int n, int i, int of) { return i * (n / of) + min(i, n % of); };       // the first of n things that the i-th has
+    const int part0 = share(have, part, parts), part_n = share(have, part + 1, parts) - part0;
+    const int i0 = part0 + share(part_n, (int)rank, (int)ctas), n = part0 + share(part_n, (int)rank + 1, (int)ctas) - i0;
+    auto out_row = [&](int r) -> T* {                  // row r of the tile; null where there is none
+        const int row = row0 + r;
         if (row >= rows_all) return nullptr;
         const int tok = row / p.G;
         return static_cast<T*>(p.out.data) + b * p.out.seq + (long long)(h * p.G + row - tok * p.G) * p.out.head + tok * p.out.token;
     };
     const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
-        if (s_first[b + 1] > s_first[b]) continue;
-        for (int i = tid; i < HR * kRows * (D / 4); i += kThreads) {
-            T* to = out_row(b, i / (kRows * (D / 4)), i / (D / 4) % kRows);
-            if (to != nullptr) store4_as(to + 4 * (i % (D / 4)), none);
-        }
-    }
-
-    // ---- this CTA's share of the flat list ----
-    const long long F = (long long)s_first[p.B] * HR, triples = (long long)p.B * HR;
-    long long C = min((long long)gridDim.x, (F + kMinPages - 1) / kMinPages);
-    if (C >= 3 * triples) C -= C % triples;            // equal sequences are cut at their borders
-    if ((long long)blockIdx.x >= C) return;
-    const long long f_lo = blockIdx.x * F / C, f_hi = (blockIdx.x + 1ll) * F / C;
-    auto cta_of = [&](long long f) { return (int)(((f + 1) * C + F - 1) / F) - 1; };
 
     const uint32_t bar0 = umma::smem_addr(&s_bar[warp][0]);
     uint8_t* ring = s_ring + (size_t)warp * kStages * kChunk;
     const uint32_t ring0 = umma::smem_addr(ring);
-    unsigned taken = 0;                                // chunks of this warp so far
     bool ok = true;
+    const int mine = warp < n ? (n - warp + kWarps - 1) / kWarps : 0;       // pages i0 + warp, + kWarps, ..
+    auto page_id = [&](int j) -> int { return j < mine ? ids[i0 + warp + kWarps * j] : 0; };
+    int id_now = page_id(lane), id_next = page_id(lane + 32);
+    auto copy = [&](int j, int id) {                   // chunk j of the warp
+        const unsigned s = (unsigned)j % kStages;
+        if (lane == 0) {
+            expect_bytes(bar0 + 8 * s, kChunk);
+            bulk_copy(ring0 + s * kChunk, p.chunks + ((size_t)((unsigned)id < (unsigned)p.n_pages ? id : 0) * p.H + h) * kChunk, kChunk, bar0 + 8 * s);
+        }
+    };
+    for (int j = 0; j < min(mine, kStages); ++j) copy(j, __shfl_sync(0xffffffffu, id_now, j));
 
-    for (long long f = f_lo; f < f_hi;) {
-        int b = 0;
-        for (int step = 512; step > 0; step >>= 1)
-            if (b + step < p.B && (long long)s_first[b + step] * HR <= f) b += step;
-        // sequences without pages share their first page's number with the next one: the search ends on the last of them, which has pages
-        const int have = s_first[b + 1] - s_first[b];
-        const long long in_seq = f - (long long)s_first[b] * HR;
-        const int hr = (int)(in_seq / have), i0 = (int)(in_seq - (long long)hr * have);
-        const int n = (int)min((long long)(have - i0), f_hi - f);
-        const long long triple = f - i0;
-        const int h = hr / p.row_tiles, row0 = (hr - h * p.row_tiles) * kRows;
-        f += n;
-
-        const int ip = p.indptr[b], all_pages = p.indptr[b + 1] - ip, length = (all_pages - 1) * kPage + p.last[b];
-        const int32_t* ids = p.lists == nullptr ? p.indices + ip : p.lists + ((long long)b * p.H + h) * p.n_lists;
-        const int mine = ok && warp < n ? (n - warp + kWarps - 1) / kWarps : 0;       // pages i0 + warp, + kWarps, ..
-        auto page_id = [&](int j) -> int { return j < mine ? ids[i0 + warp + kWarps * j] : 0; };
-        int id_now = page_id(lane), id_next = page_id(lane + 32);
-        auto copy = [&](int j, int id) {               // chunk j of the segment
-            const unsigned s = (taken + j) % kStages;
-            if (lane == 0) {
-                expect_bytes(bar0 + 8 * s, kChunk);
-                bulk_copy(ring0 + s * kChunk, p.chunks + ((size_t)((unsigned)id < (unsigned)p.n_pages ? id : 0) * p.H + h) * kChunk, kChunk, bar0 + 8 * s);
-            }
-        };
-        for (int j = 0; j < min(mine, kStages); ++j) copy(j, __shfl_sync(0xffffffffu, id_now, j));
-
-        // ---- queries: B operands, and what the rows' scores are multiplied with ----
-        uint32_t qf[kTiles][kQParts][kSteps][2];
-        float factor[kTiles][2];
-        int limit[kTiles][2];                          // the last position that rows 2t, 2t + 1 see
+    // ---- queries: B operands, and what the rows' scores are multiplied with ----
+    uint32_t qf[kTiles][kQParts][kSteps][2];
+    float factor[kTiles][2];
+    int limit[kTiles][2];                          // the last position that rows 2t, 2t + 1 see
 #pragma unroll
-        for (int n8 = 0; n8 < kTiles; ++n8) {
-            const int row = row0 + 8 * n8 + g, tok = row / p.G;
-            Eight<T> x[D / 64][2];
-            const T* src = static_cast<const T*>(p.q.data) + b * p.q.seq + (long long)(h * p.G + row - tok * p.G) * p.q.head + tok * p.q.token + 16 * t;
-            uint32_t amax = 0;
+    for (int n8 = 0; n8 < kTiles; ++n8) {
+        const int row = row0 + 8 * n8 + g, tok = row / p.G;
+        Eight<T> x[D / 64][2];
+        const T* src = static_cast<const T*>(p.q.data) + b * p.q.seq + (long long)(h * p.G + row - tok * p.G) * p.q.head + tok * p.q.token + 16 * t;
+        uint32_t amax = 0;
 #pragma unroll
-            for (int hh = 0; hh < D / 64; ++hh)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    if (row < rows_all) x[hh][e].load(src + 64 * hh + 8 * e);
-                    else x[hh][e].zero();
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) amax = max(amax, __float_as_uint(x[hh][e].get(k)) & 0x7fffffffu);
-                }
-            amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            // the largest magnitude is brought to 2^14 .. 2^15; numbers below 2^-38 of it lose places
-            const int e2 = std::is_same<T, __half>::value ? 0 : max((int)(amax >> 23) - 127 - 14, -126);
-            const float down = power_of_two(-e2);
-#pragma unroll
-            for (int hh = 0; hh < D / 64; ++hh)
-#pragma unroll
-                for (int s = 0; s < 4; ++s)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float a = x[hh][s >> 1].get(4 * (s & 1) + 2 * e) * down, c = x[hh][s >> 1].get(4 * (s & 1) + 2 * e + 1) * down;
-                        const uint32_t hi = pack_f16(a, c);
-                        qf[n8][0][4 * hh + s][e] = hi;
-                        if constexpr (kQParts == 2) {
-                            const float2 got = unpack_f16(hi);
-                            qf[n8][kQParts - 1][4 * hh + s][e] = pack_f16(a - got.x, c - got.y);
-                        }
-                    }
-            const float mult = power_of_two(e2) * p.scale;
-            const int lim = length - p.tokens + tok;
+        for (int hh = 0; hh < D / 64; ++hh)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                factor[n8][e] = __shfl_sync(0xffffffffu, mult, 8 * t + 4 * e);
-                limit[n8][e] = __shfl_sync(0xffffffffu, lim, 8 * t + 4 * e);
+                if (row < rows_all) x[hh][e].load(src + 64 * hh + 8 * e);
+                else x[hh][e].zero();
+#pragma unroll
+                for (int k = 0; k < 8; ++k) amax = max(amax, __float_as_uint(x[hh][e].get(k)) & 0x7fffffffu);
             }
-        }
-        // positions at and below this one are seen by all rows of the tile (rows beyond the last one may see more)
-        const int seen_by_all = length - p.tokens + row0 / p.G;
-
-        float o[kTiles][kSteps][4];
-        float m[kTiles][2], l[kTiles][2];
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        // the largest magnitude is brought to 2^14 .. 2^15; numbers below 2^-38 of it lose places
+        const int e2 = std::is_same<T, __half>::value ? 0 : max((int)(amax >> 23) - 127 - 14, -126);
+        const float down = power_of_two(-e2);
 #pragma unroll
-        for (int n8 = 0; n8 < kTiles; ++n8) {
+        for (int hh = 0; hh < D / 64; ++hh)
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[n8][i][e] = 0.f;
-            m[n8][0] = m[n8][1] = kNoRef;
-            l[n8][0] = l[n8][1] = 0.f;
-        }
-
-        for (int j = 0; j < mine; ++j) {
-            if (j > 0 && (j & 31) == 0) {
-                id_now = id_next;
-                id_next = page_id(j + 32 + lane);
-            }
-            const unsigned s = (taken + j) % kStages;
-            ok = __all_sync(0xffffffffu, umma::bar_wait(bar0 + 8 * s, (taken + j) / kStages & 1));
-            if (!ok) {                                 // those behind it are given the same time, then the rows get NaN
-                for (int x = j + 1; x < min(mine, j + kStages); ++x) umma::bar_wait(bar0 + 8 * ((taken + x) % kStages), (taken + x) / kStages & 1);
-                if (lane == 0) atomicOr(p.status, kTimedOut);
-                break;
-            }
-            const bool bad = (unsigned)__shfl_sync(0xffffffffu, id_now, j & 31) >= (unsigned)p.n_pages;
-            const uint8_t* chunk = ring + (size_t)s * kChunk;
-            const float2 scales = *reinterpret_cast<const float2*>(chunk + 2 * half_bytes(D));
-
-            float sc[kTiles][4];
-#pragma unroll
-            for (int n8 = 0; n8 < kTiles; ++n8)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sc[n8][e] = 0.f;
-#pragma unroll
-            for (int hh = 0; hh < D / 64; ++hh) {
-                const uint4 ka = *reinterpret_cast<const uint4*>(chunk + hh * 1024 + g * 64 + t * 16);
-                const uint4 kb = *reinterpret_cast<const uint4*>(chunk + hh * 1024 + (g + 8) * 64 + t * 16);
-                const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint32_t a[4] = {codes_f16<0>(wa[k]), codes_f16<0>(wb[k]), codes_f16<1>(wa[k]), codes_f16<1>(wb[k])};
-#pragma unroll
-                    for (int n8 = 0; n8 < kTiles; ++n8)
-#pragma unroll
-                        for (int part = 0; part < kQParts; ++part) mma_f16(sc[n8], a, qf[n8][part][4 * hh + k][0], qf[n8][part][4 * hh + k][1]);
-                }
-            }
-            // a block with a scale that is no number answers nobody who sees it; its codes are zeros
-            const float ks = isnan(scales.y) ? scales.y : scales.x, vs = isnan(scales.y) ? 0.f : scales.y;
-            const int i = i0 + warp + kWarps * j;      // of the triple's pages
-            // only the last page of a list is cut
-            const int first = p.lists == nullptr ? i * kPage : i == have - 1 ? (all_pages - 1) * kPage : 0;
-            const bool cut = bad || first + kPage - 1 > seen_by_all;
-            uint32_t ph[kTiles][2], pl[kTiles][2];
-            bool raise = false;
-#pragma unroll
-            for (int n8 = 0; n8 < kTiles; ++n8) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {          // token g + 8 (e >> 1), row 2t + (e & 1)
-                    sc[n8][e] *= ks * factor[n8][e & 1];
-                    if (cut && (bad || first + g + 8 * (e >> 1) > limit[n8][e & 1])) sc[n8][e] = -INFINITY;
-                    raise |= sc[n8][e] > m[n8][e & 1] + kReach;
-                }
-            }
-            if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-                for (int n8 = 0; n8 < kTiles; ++n8)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float best = fmaxf(sc[n8][e], sc[n8][e + 2]);
-#pragma unroll
-                        for (int x = 4; x < 32; x *= 2) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, x));
-                        if (best - kLift > m[n8][e]) {
-                            const float down = ex2(m[n8][e] - (best - kLift));
-                            m[n8][e] = best - kLift;
-                            l[n8][e] *= down;
-#pragma unroll
-                            for (int k = 0; k < kSteps; ++k) {
-                                o[n8][k][e] *= down;
-                                o[n8][k][e + 2] *= down;
-                            }
-                        }
-                    }
-            }
-#pragma unroll
-            for (int n8 = 0; n8 < kTiles; ++n8) {
-                float w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    w[e] = ex2(sc[n8][e] - m[n8][e & 1]);
-                    l[n8][e & 1] += w[e];
-                }
+            for (int s = 0; s < 4; ++s)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const uint32_t hi = pack_f16(w[2 * e], w[2 * e + 1]);
-                    const float2 got = unpack_f16(hi);
-                    ph[n8][e] = transpose8(hi);
-                    pl[n8][e] = transpose8(pack_f16(w[2 * e] - got.x, w[2 * e + 1] - got.y));
-                }
-            }
-            const uint8_t* values = chunk + half_bytes(D) + lane * 16;
-#pragma unroll
-            for (int part = 0; part < D / 32; ++part) {
-                const uint4 v = *reinterpret_cast<const uint4*>(values + part * 512);
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const uint32_t a[4] = {codes_f16<0>(w[2 * k]), codes_f16<0>(w[2 * k + 1]), codes_f16<1>(w[2 * k]), codes_f16<1>(w[2 * k + 1])};
-#pragma unroll
-                    for (int n8 = 0; n8 < kTiles; ++n8) {
-                        float d[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma_f16(d, a, pl[n8][0], pl[n8][1]);
-                        mma_f16(d, a, ph[n8][0], ph[n8][1]);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[n8][2 * part + k][e] = fmaf(d[e], vs, o[n8][2 * part + k][e]);
+                    const float a = x[hh][s >> 1].get(4 * (s & 1) + 2 * e) * down, c = x[hh][s >> 1].get(4 * (s & 1) + 2 * e + 1) * down;
+                    const uint32_t hi = pack_f16(a, c);
+                    qf[n8][0][4 * hh + s][e] = hi;
+                    if constexpr (kQParts == 2) {
+                        const float2 got = unpack_f16(hi);
+                        qf[n8][kQParts - 1][4 * hh + s][e] = pack_f16(a - got.x, c - got.y);
                     }
                 }
-            }
-            __syncwarp();
-            if (j + kStages < mine) copy(j + kStages, __shfl_sync(0xffffffffu, ((j + kStages) ^ j) & 32 ? id_next : id_now, (j + kStages) & 31));
-            if (bad && lane == 0) atomicOr(p.status, kBadPage);
+        const float mult = power_of_two(e2) * p.scale;
+        const int lim = length - p.tokens + tok;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            factor[n8][e] = __shfl_sync(0xffffffffu, mult, 8 * t + 4 * e);
+            limit[n8][e] = __shfl_sync(0xffffffffu, lim, 8 * t + 4 * e);
         }
-        taken += mine;
+    }
+    // positions at and below this one are seen by all rows of the tile (rows beyond the last one may see more)
+    const int seen_by_all = length - p.tokens + row0 / p.G;
 
-        // ---- the warps' sums, over the ring ----
-        __syncthreads();                               // every warp has read its last chunk
-        float* sums = reinterpret_cast<float*>(s_ring);
+    float o[kTiles][kSteps][4];
+    float m[kTiles][2], l[kTiles][2];
+#pragma unroll
+    for (int n8 = 0; n8 < kTiles; ++n8) {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n8][i][e] = 0.f;
+        m[n8][0] = m[n8][1] = kNoRef;
+        l[n8][0] = l[n8][1] = 0.f;
+    }
+
+    for (int j = 0; j < mine; ++j) {
+        if (j > 0 && (j & 31) == 0) {
+            id_now = id_next;
+            id_next = page_id(j + 32 + lane);
+        }
+        const unsigned s = (unsigned)j % kStages;
+        ok = __all_sync(0xffffffffu, umma::bar_wait(bar0 + 8 * s, (unsigned)j / kStages & 1));
+        if (!ok) {                                 // those behind it are given the same time, then the rows get NaN
+            for (int x = j + 1; x < min(mine, j + kStages); ++x) umma::bar_wait(bar0 + 8 * ((unsigned)x % kStages), (unsigned)x / kStages & 1);
+            if (lane == 0) atomicOr(p.status, kTimedOut);
+            break;
+        }
+        const bool bad = (unsigned)__shfl_sync(0xffffffffu, id_now, j & 31) >= (unsigned)p.n_pages;
+        const uint8_t* chunk = ring + (size_t)s * kChunk;
+        const float2 scales = *reinterpret_cast<const float2*>(chunk + 2 * half_bytes(D));
+
+        float sc[kTiles][4];
 #pragma unroll
         for (int n8 = 0; n8 < kTiles; ++n8)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
+            for (int e = 0; e < 4; ++e) sc[n8][e] = 0.f;
 #pragma unroll
-                for (int x = 4; x < 32; x *= 2) l[n8][e] += __shfl_xor_sync(0xffffffffu, l[n8][e], x);
-                const int r = 8 * n8 + 2 * t + e;
-                if (g == 0) {
-                    s_m[warp][r] = m[n8][e];
-                    s_l[warp][r] = ok ? l[n8][e] : NAN;
+        for (int hh = 0; hh < D / 64; ++hh) {
+            const uint4 ka = *reinterpret_cast<const uint4*>(chunk + hh * 1024 + g * 64 + t * 16);
+            const uint4 kb = *reinterpret_cast<const uint4*>(chunk + hh * 1024 + (g + 8) * 64 + t * 16);
+            const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t a[4] = {codes_f16<0>(wa[k]), codes_f16<0>(wb[k]), codes_f16<1>(wa[k]), codes_f16<1>(wb[k])};
+#pragma unroll
+                for (int n8 = 0; n8 < kTiles; ++n8)
+#pragma unroll
+                    for (int part = 0; part < kQParts; ++part) mma_f16(sc[n8], a, qf[n8][part][4 * hh + k][0], qf[n8][part][4 * hh + k][1]);
+            }
+        }
+        // a block with a scale that is no number answers nobody who sees it; its codes are zeros
+        const float ks = isnan(scales.y) ? scales.y : scales.x, vs = isnan(scales.y) ? 0.f : scales.y;
+        const int i = i0 + warp + kWarps * j;      // of the triple's pages
+        // only the last page of a list is cut
+        const int first = p.lists == nullptr ? i * kPage : i == have - 1 ? (all_pages - 1) * kPage : 0;
+        const bool cut = bad || first + kPage - 1 > seen_by_all;
+        uint32_t ph[kTiles][2], pl[kTiles][2];
+        bool raise = false;
+#pragma unroll
+        for (int n8 = 0; n8 < kTiles; ++n8) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {          // token g + 8 (e >> 1), row 2t + (e & 1)
+                sc[n8][e] *= ks * factor[n8][e & 1];
+                if (cut && (bad || first + g + 8 * (e >> 1) > limit[n8][e & 1])) sc[n8][e] = -INFINITY;
+                raise |= sc[n8][e] > m[n8][e & 1] + kReach;
+            }
+        }
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+            for (int n8 = 0; n8 < kTiles; ++n8)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float best = fmaxf(sc[n8][e], sc[n8][e + 2]);
+#pragma unroll
+                    for (int x = 4; x < 32; x *= 2) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, x));
+                    if (best - kLift > m[n8][e]) {
+                        const float down = ex2(m[n8][e] - (best - kLift));
+                        m[n8][e] = best - kLift;
+                        l[n8][e] *= down;
+#pragma unroll
+                        for (int k = 0; k < kSteps; ++k) {
+                            o[n8][k][e] *= down;
+                            o[n8][k][e + 2] *= down;
+                        }
+                    }
                 }
-                float* to = sums + ((size_t)warp * kRows + r) * kPitch + g;
+        }
 #pragma unroll
-                for (int k = 0; k < kSteps; ++k) {
-                    to[16 * k] = o[n8][k][e];
-                    to[16 * k + 8] = o[n8][k][e + 2];
+        for (int n8 = 0; n8 < kTiles; ++n8) {
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                w[e] = ex2(sc[n8][e] - m[n8][e & 1]);
+                l[n8][e & 1] += w[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint32_t hi = pack_f16(w[2 * e], w[2 * e + 1]);
+                const float2 got = unpack_f16(hi);
+                ph[n8][e] = transpose8(hi);
+                pl[n8][e] = transpose8(pack_f16(w[2 * e] - got.x, w[2 * e + 1] - got.y));
+            }
+        }
+        const uint8_t* values = chunk + half_bytes(D) + lane * 16;
+#pragma unroll
+        for (int part = 0; part < D / 32; ++part) {
+            const uint4 v = *reinterpret_cast<const uint4*>(values + part * 512);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint32_t a[4] = {codes_f16<0>(w[2 * k]), codes_f16<0>(w[2 * k + 1]), codes_f16<1>(w[2 * k]), codes_f16<1>(w[2 * k + 1])};
+#pragma unroll
+                for (int n8 = 0; n8 < kTiles; ++n8) {
+                    float d[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma_f16(d, a, pl[n8][0], pl[n8][1]);
+                    mma_f16(d, a, ph[n8][0], ph[n8][1]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[n8][2 * part + k][e] = fmaf(d[e], vs, o[n8][2 * part + k][e]);
                 }
             }
-        __syncthreads();
-        const bool whole = n == have;
-        float* part = p.partials + (2 * (size_t)blockIdx.x + (i0 > 0 ? 0 : 1)) * partial_floats(D, kRows);
-        for (int i = tid; i < kRows * (D / 4); i += kThreads) {
-            const int r = i / (D / 4), d4 = i % (D / 4);
-            float top = s_m[0][r], sum = 0.f;
+        }
+        __syncwarp();
+        if (j + kStages < mine) copy(j + kStages, __shfl_sync(0xffffffffu, ((j + kStages) ^ j) & 32 ? id_next : id_now, (j + kStages) & 31));
+        if (bad && lane == 0) atomicOr(p.status, kBadPage);
+    }
+
+    // ---- the warps' sums, over the ring: first of the CTA, then of the cluster ----
+    __syncthreads();                                   // every warp has read its last chunk
+    float* sums = reinterpret_cast<float*>(s_ring);
 #pragma unroll
-            for (int w = 1; w < kWarps; ++w) top = fmaxf(top, s_m[w][r]);
+    for (int n8 = 0; n8 < kTiles; ++n8)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int x = 4; x < 32; x *= 2) l[n8][e] += __shfl_xor_sync(0xffffffffu, l[n8][e], x);
+            const int r = 8 * n8 + 2 * t + e;
+            if (g == 0) {
+                s_m[warp][r] = m[n8][e];
+                s_l[warp][r] = ok ? l[n8][e] : NAN;
+            }
+            float* to = sums + ((size_t)warp * kRows + r) * kPitch + g;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                to[16 * k] = o[n8][k][e];
+                to[16 * k + 8] = o[n8][k][e + 2];
+            }
+        }
+    __syncthreads();
+    constexpr int kAll = kRows * (D / 4), kItems = kAll / kThreads;       // four numbers of a row each
+    float* shared = sums + (size_t)kWarps * kRows * kPitch;               // the CTA's, for its neighbours
+    float* partial = p.partials + (size_t)unit * partial_floats(D, kRows);
+    auto finish = [&](int i, float4 v, float top, float sum) {
+        const int r = i / (D / 4), d4 = i % (D / 4);
+        if (parts > 1) {
+            *reinterpret_cast<float4*>(partial + 4 * i) = v;
+            if (d4 == 0) *reinterpret_cast<float2*>(partial + (size_t)kRows * D + 2 * r) = make_float2(top, sum);
+            return;
+        }
+        T* to = out_row(r);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        if (to != nullptr) store4_as(to + 4 * d4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+    };
+#pragma unroll
+    for (int x = 0; x < kItems; ++x) {
+        const int i = tid + x * kThreads, r = i / (D / 4), d4 = i % (D / 4);
+        float top = s_m[0][r], sum = 0.f;
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, s_m[w][r]);
+        float4 v = none;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float f = ex2(s_m[w][r] - top);
+            const float4 y = *reinterpret_cast<const float4*>(sums + ((size_t)w * kRows + r) * kPitch + 4 * d4);
+            sum = fmaf(s_l[w][r], f, sum);
+            v.x = fmaf(y.x, f, v.x), v.y = fmaf(y.y, f, v.y), v.z = fmaf(y.z, f, v.z), v.w = fmaf(y.w, f, v.w);
+        }
+        if (ctas == 1) {
+            finish(i, v, top, sum);
+        } else {
+            *reinterpret_cast<float4*>(shared + 4 * i) = v;
+            if (d4 == 0) s_ml[r] = make_float2(top, sum);
+        }
+    }
+    if (ctas > 1) {
+        cluster_sync();
+        const uint32_t mine_at = umma::smem_addr(shared), ml_at = umma::smem_addr(s_ml);
+        for (int i = tid * (int)ctas + (int)rank; i < kAll; i += kThreads * (int)ctas) {
+            const int r = i / (D / 4);
+            float2 ml[kMaxCluster];
+            float4 y[kMaxCluster];
+            float top = kNoRef, sum = 0.f;
+#pragma unroll
+            for (int c = 0; c < kMaxCluster; ++c) {
+                if (c >= (int)ctas) continue;
+                ml[c] = peer_f32x2(ml_at + 8 * r, c);
+                y[c] = peer_f32x4(mine_at + 16 * i, c);
+                top = fmaxf(top, ml[c].x);
+            }
             float4 v = none;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float x = ex2(s_m[w][r] - top);
-                const float4 y = *reinterpret_cast<const float4*>(sums + ((size_t)w * kRows + r) * kPitch + 4 * d4);
-                sum = fmaf(s_l[w][r], x, sum);
-                v.x = fmaf(y.x, x, v.x), v.y = fmaf(y.y, x, v.y), v.z = fmaf(y.z, x, v.z), v.w = fmaf(y.w, x, v.w);
+            for (int c = 0; c < kMaxCluster; ++c) {
+                if (c >= (int)ctas) continue;
+                const float f = ex2(ml[c].x - top);
+                sum = fmaf(ml[c].y, f, sum);
+                v.x = fmaf(y[c].x, f, v.x), v.y = fmaf(y[c].y, f, v.y), v.z = fmaf(y[c].z, f, v.z), v.w = fmaf(y[c].w, f, v.w);
             }
-            if (whole) {
-                T* to = out_row(b, hr, r);
-                const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                if (to != nullptr) store4_as(to + 4 * d4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-            } else {
-                *reinterpret_cast<float4*>(part + (size_t)r * D + 4 * d4) = v;
-                if (d4 == 0) *reinterpret_cast<float2*>(part + (size_t)kRows * D + 2 * r) = make_float2(top, sum);
-            }
+            finish(i, v, top, sum);
         }
-        // generic writes to the ring come before the next copies into it
-        umma::fence_operands();
-        __syncthreads();
-        if (whole) continue;
+        cluster_sync();                                // nobody leaves while its sums are read
+    }
+    if (parts == 1) return;
 
-        // ---- a triple that several CTAs share: the last one adds the shares up ----
-        const int c0 = cta_of(triple), c1 = cta_of(triple + have - 1);
-        if (tid == 0) {
-            const bool is_last = arrive(p.counters + c0) == (unsigned)(c1 - c0);
-            if (is_last) p.counters[c0] = 0;
-            s_last = is_last;
+    // ---- parts of a triple: the last CTA adds them up ----
+    __syncthreads();
+    const int unit0 = unit - part;
+    if (tid == 0) {
+        const bool is_last = arrive(p.counters + unit0) == (unsigned)(parts * (int)ctas - 1);
+        if (is_last) p.counters[unit0] = 0;
+        s_last = is_last;
+    }
+    __syncthreads();
+    if (!s_last) return;
+    // kJoin parts at a time: what each counts (a thread a row and part), and their sums; 16 loads of a thread are in flight
+    constexpr int kGroups = kThreads / kRows, kEach = kJoin / kGroups, kBatch = 16 / kItems;
+    float* s_w = sums;                                 // [kJoin][kRows]: factors, and factors times sums
+    float* s_wl = s_w + kJoin * kRows;
+    float* s_top = s_wl + kJoin * kRows;               // [kGroups][kRows]
+    const int mr = tid % kRows, mg = tid / kRows;
+    float4 v[kItems];
+    float sum[kItems], top = kNoRef;
+#pragma unroll
+    for (int x = 0; x < kItems; ++x) v[x] = none, sum[x] = 0.f;
+    for (int from = 0; from < parts; from += kJoin) {
+        const int here = min(kJoin, parts - from);
+        const float* first = p.partials + (size_t)(unit0 + from) * partial_floats(D, kRows);
+        auto piece = [&](int c, int x) { return __ldcg(reinterpret_cast<const float4*>(first + (size_t)c * partial_floats(D, kRows)) + tid + x * kThreads); };
+        float2 ml[kEach];
+        float now = top;
+#pragma unroll
+        for (int x = 0; x < kEach; ++x) {
+            const int c = mg + x * kGroups;
+            ml[x] = c < here ? __ldcg(reinterpret_cast<const float2*>(first + (size_t)c * partial_floats(D, kRows) + (size_t)kRows * D) + mr) : make_float2(kNoRef, 0.f);
+        }
+        float4 y[kBatch][kItems];
+#pragma unroll
+        for (int c = 0; c < kBatch; ++c)
+#pragma unroll
+            for (int x = 0; x < kItems; ++x)
+                if (c < here) y[c][x] = piece(c, x);
+#pragma unroll
+        for (int x = 0; x < kEach; ++x) now = fmaxf(now, ml[x].x);
+        s_top[mg * kRows + mr] = now;
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < kGroups; ++x) now = fmaxf(now, s_top[x * kRows + mr]);
+#pragma unroll
+        for (int x = 0; x < kEach; ++x) {
+            const float f = ex2(ml[x].x - now);
+            s_w[(mg + x * kGroups) * kRows + mr] = f;
+            s_wl[(mg + x * kGroups) * kRows + mr] = f * ml[x].y;
         }
         __syncthreads();
-        if (s_last) {
-            auto slot = [&](int c) { return p.partials + (2 * (size_t)c + (triple < c * F / C ? 0 : 1)) * partial_floats(D, kRows); };
-            for (int i = tid; i < kRows * (D / 4); i += kThreads) {
-                const int r = i / (D / 4), d4 = i % (D / 4);
-                float top = kNoRef, sum = 0.f;
-                float4 v = none;
-#pragma unroll 4
-                for (int c = c0; c <= c1; ++c) {
-                    const float* from = slot(c);
-                    const float pm = ld_cg_f32(from + (size_t)kRows * D + 2 * r), pl = ld_cg_f32(from + (size_t)kRows * D + 2 * r + 1);
-                    const float4 y = ld_cg_f32x4(from + (size_t)r * D + 4 * d4);
-                    const float now = fmaxf(top, pm), keep = ex2(top - now), x = ex2(pm - now);
-                    top = now;
-                    sum = fmaf(pl, x, sum * keep);
-                    v.x = fmaf(y.x, x, v.x * keep), v.y = fmaf(y.y, x, v.y * keep);
-                    v.z = fmaf(y.z, x, v.z * keep), v.w = fmaf(y.w, x, v.w * keep);
-                }
-                T* to = out_row(b, hr, r);
-                const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                if (to != nullptr) store4_as(to + 4 * d4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-            }
+        if (mg == 0) s_top[mr] = ex2(top - now);       // of the parts before
+        top = now;
+        __syncthreads();
+        auto add = [&](int c, int x, float4 a) {
+            const int r = (tid + x * kThreads) / (D / 4);
+            const float w = s_w[c * kRows + r];
+            sum[x] += s_wl[c * kRows + r];
+            v[x].x = fmaf(a.x, w, v[x].x), v[x].y = fmaf(a.y, w, v[x].y), v[x].z = fmaf(a.z, w, v[x].z), v[x].w = fmaf(a.w, w, v[x].w);
+        };
+#pragma unroll
+        for (int x = 0; x < kItems; ++x) {
+            const float keep = s_top[(tid + x * kThreads) / (D / 4)];
+            sum[x] *= keep, v[x].x *= keep, v[x].y *= keep, v[x].z *= keep, v[x].w *= keep;
         }
-        __syncthreads();                               // s_last is read
+#pragma unroll
+        for (int c = 0; c < kBatch; ++c)
+#pragma unroll
+            for (int x = 0; x < kItems; ++x)
+                if (c < here) add(c, x, y[c][x]);
+        for (int from_c = kBatch; from_c < here; from_c += kBatch) {
+#pragma unroll
+            for (int c = 0; c < kBatch; ++c)
+#pragma unroll
+                for (int x = 0; x < kItems; ++x)
+                    if (from_c + c < here) y[c][x] = piece(from_c + c, x);
+#pragma unroll
+            for (int c = 0; c < kBatch; ++c)
+#pragma unroll
+                for (int x = 0; x < kItems; ++x)
+                    if (from_c + c < here) add(from_c + c, x, y[c][x]);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int x = 0; x < kItems; ++x) {
+        const int i = tid + x * kThreads;
+        T* to = out_row(i / (D / 4));
+        const float inv = sum[x] == 0.f ? 0.f : 1.f / sum[x];
+        if (to != nullptr) store4_as(to + 4 * (i % (D / 4)), make_float4(v[x].x * inv, v[x].y * inv, v[x].z * inv, v[x].w * inv));
     }
 }
 
 template <typename T, int D, int kTiles>
-int launch(const AttnParams& p, int max_pages_seq, cudaStream_t st) {
+int launch(const AttnParams& p, int max_pages_seq, long long total_pages, cudaStream_t st) {
     static std::atomic<unsigned long long> ready{0};             // a bit for each device
     int dev = 0;
     LEANKV_CUDA_TRY(cudaGetDevice(&dev));
@@ -485,16 +594,35 @@ int launch(const AttnParams& p, int max_pages_seq, cudaStream_t st) {
         LEANKV_CUDA_TRY(cudaFuncSetAttribute(attn_kernel<T, D, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         ready.fetch_or(1ull << dev, std::memory_order_release);
     }
-    const long long pages = (long long)p.B * p.H * p.row_tiles * (p.lists == nullptr ? max_pages_seq : std::min(max_pages_seq, p.n_lists));
-    const long long grid = std::min<long long>(std::min(kCtasPerSm * sm_count(), kMaxCtas), (pages + kMinPages - 1) / kMinPages);
-    LEANKV_CUDA_TRY(launch_early(attn_kernel<T, D, kTiles>, dim3((unsigned)std::max(grid, 1ll)), dim3(kThreads), smem, st, p));
+    // Clusters: as many CTAs of a triple as the device holds at once, up to eight and no fewer pages each than kFewPages; beyond one wave kWavePages each. Parts:
+    // where whole clusters fit more than once, but not below kPartPages a CTA; bounded by the workspace.
+    const long long room = (long long)kCtasPerSm * sm_count(), triples = (long long)p.B * p.H * p.row_tiles;
+    const long long longest = p.lists == nullptr ? max_pages_seq : std::min(max_pages_seq, p.n_lists);
+    const long long total = (p.lists == nullptr ? std::min(total_pages, (long long)p.B * longest) : (long long)p.B * longest) * p.H * p.row_tiles;
+    const bool waves = triples > room;
+    int ctas = 1;
+    while (ctas < kMaxCluster && (waves ? longest > (long long)ctas * kWavePages : 2 * ctas * triples <= room && longest > (long long)ctas * kFewPages)) ctas *= 2;
+    const long long clusters = room / ctas;
+    long long part_pages = waves ? (long long)ctas * kWavePages
+                                 : std::min((longest + clusters / triples - 1) / (clusters / triples),
+                                            clusters > triples ? (total + clusters - triples - 1) / (clusters - triples) : longest);
+    part_pages = std::max({part_pages, (long long)ctas * kPartPages, 1ll});
+    if (total / part_pages + triples > kMaxParts) part_pages = triples >= kMaxParts ? longest : std::max(part_pages, total / (kMaxParts - triples) + 1);
+    AttnParams q = p;
+    q.part_pages = longest <= part_pages ? 0 : (int)part_pages;
+    const long long units = q.part_pages == 0 ? triples : total / part_pages + triples;
+    if (units * ctas > 0x7fffffffll) return LEANKV_ELIMIT;
+    if (ctas == 1)
+        LEANKV_CUDA_TRY(launch_early(attn_kernel<T, D, kTiles>, dim3((unsigned)units), dim3(kThreads), smem, st, q));
+    else
+        LEANKV_CUDA_TRY(launch_cluster_kernel_ex(true, dim3(ctas), attn_kernel<T, D, kTiles>, dim3((unsigned)(units * ctas)), dim3(kThreads), smem, st, q));
     return LEANKV_OK;
 }
 
 template <typename T>
-int launch(const AttnParams& p, int dim, int rows, int max_pages_seq, cudaStream_t st) {
-    if (dim == 128) return rows == 8 ? launch<T, 128, 1>(p, max_pages_seq, st) : launch<T, 128, 2>(p, max_pages_seq, st);
-    return rows == 8 ? launch<T, 64, 1>(p, max_pages_seq, st) : launch<T, 64, 2>(p, max_pages_seq, st);
+int launch(const AttnParams& p, int dim, int rows, int max_pages_seq, long long total_pages, cudaStream_t st) {
+    if (dim == 128) return rows == 8 ? launch<T, 128, 1>(p, max_pages_seq, total_pages, st) : launch<T, 128, 2>(p, max_pages_seq, total_pages, st);
+    return rows == 8 ? launch<T, 64, 1>(p, max_pages_seq, total_pages, st) : launch<T, 64, 2>(p, max_pages_seq, total_pages, st);
 }
 
 }  // namespace
@@ -507,11 +635,11 @@ extern "C" size_t leankv_byte_attn_workspace_bytes(void) { return bytes::kWorksp
 
 extern "C" int leankv_byte_attn(const leankv_byte_pool_t* pool, int dtype, const leankv_vectors_t* q, const leankv_vectors_t* out, int B,
                                 int q_heads, int tokens, float scale, const int32_t* kv_indptr, const int32_t* kv_page_indices,
-                                const int32_t* kv_last_page_len, int max_pages_seq, const int32_t* block_pages, int n_blocks, void* workspace,
-                                size_t workspace_bytes, void* stream) {
+                                const int32_t* kv_last_page_len, int max_pages_seq, long long total_pages, const int32_t* block_pages, int n_blocks,
+                                void* workspace, size_t workspace_bytes, void* stream) {
     if (!bytes::good_pool(pool) || !bytes::good_type(dtype) || !q || !out || !q->data || !out->data || B <= 0 || tokens <= 0 || q_heads <= 0 ||
         q_heads % pool->kv_heads != 0 || !kv_indptr || !kv_page_indices || !kv_last_page_len || max_pages_seq < 0 ||
-        (block_pages != nullptr && (tokens != 1 || n_blocks <= 0)))
+        total_pages < 0 || (block_pages != nullptr && (tokens != 1 || n_blocks <= 0)))
         return LEANKV_EINVAL;
     if (B > LEANKV_BYTES_MAX_BATCH || q_heads / pool->kv_heads > LEANKV_BYTES_MAX_GROUP) return LEANKV_ELIMIT;
     if (!bytes::aligned_pool(pool) || !bytes::aligned_vectors(q, dtype, B, q_heads, tokens) ||
@@ -533,9 +661,9 @@ extern "C" int leankv_byte_attn(const leankv_byte_pool_t* pool, int dtype, const
     p.counters = reinterpret_cast<unsigned*>(p.status + bytes::kStatusWords);
     p.partials = reinterpret_cast<float*>(p.counters + bytes::kCounters);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return dtype == LEANKV_BYTES_F16 ? bytes::launch<__half>(p, pool->dim, rows, max_pages_seq, st)
-         : dtype == LEANKV_BYTES_BF16 ? bytes::launch<bf16>(p, pool->dim, rows, max_pages_seq, st)
-                                      : bytes::launch<float>(p, pool->dim, rows, max_pages_seq, st);
+    return dtype == LEANKV_BYTES_F16 ? bytes::launch<__half>(p, pool->dim, rows, max_pages_seq, total_pages, st)
+         : dtype == LEANKV_BYTES_BF16 ? bytes::launch<bf16>(p, pool->dim, rows, max_pages_seq, total_pages, st)
+                                      : bytes::launch<float>(p, pool->dim, rows, max_pages_seq, total_pages, st);
 }
 
 extern "C" int leankv_byte_status(const void* workspace, int* status) {

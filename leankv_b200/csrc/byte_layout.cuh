@@ -10,6 +10,8 @@
 // Both are read straight into registers; nothing is transposed or shuffled on the way to the tensor cores.
 #pragma once
 
+#include <type_traits>
+
 #include "leankv_bytes.h"
 #include "typed.cuh"
 
@@ -154,6 +156,17 @@ template <> struct Eight<float> {
         return (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
     }
 };
+
+// Two numbers in a 16-bit type.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_as(float a, float b) {
+    if constexpr (std::is_same<T, bf16>::value) {
+        return pack_bf16(a, b);
+    } else {
+        const __half2 v = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+}
 
 }  // namespace bytes
 }  // namespace leankv

@@ -1,0 +1,502 @@
+// Causal attention of a prompt chunk over the 8-bit pages, on tcgen05.
+//
+// A CTA takes 256 rows of a kv head, two tiles of 128 (query token, query head) pairs, against 128 keys (eight pages) at a time. Both row tiles use the same
+// keys and values, so that the codes are turned into fp16 operands once for 256 rows, inside this kernel:
+//   warps 8, 9   pages from memory into registers a whole key tile ahead; code + 128 behind the byte 0x64 is the fp16 number 1152 + code, one
+//                subtraction (keys) or fused multiply-add (values) makes it exact; 16-byte (8-byte) stores fill core matrices in order
+//   warp 10      S_r = Q_r K^T and O_r += P_r V of both row tiles, one thread issues
+//   warps 0 - 7  a thread a row: scores from tensor memory, maximum, weights back over the scores as fp16
+// The row tiles alternate: the products of one run under the exponentials of the other. Tensor memory: S of both (128 columns each), O of both (dim each).
+//
+// Exactness. Keys enter as their codes (the scale, one number for 16 keys, is multiplied to the scores in fp32), queries in fp16 with a power of two taken out
+// of each row. Values enter as code * 2^(e - r), r the largest exponent among the CTA's pages: exact down to 2^-24, and a page whose numbers are 2^-25 of
+// the largest page's is lost against it. Weights are fp16 (2^-11), the reference of a row kLift below its maximum so that 2^-21 of the
+// largest weight still has all its places; their sum is fp32 before that rounding.
+//
+// Bound: a key tile is 4 x 512 tensor cycles (dim 128) and 2 x 1024 cycles of ex2; operand reads (192 KB) and the converted tiles (64 KB written) take the
+// same time of shared memory's 128 bytes a cycle.
+
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
+#include "byte_layout.cuh"
+#include "byte_workspace.cuh"
+#include "tile_softmax.cuh"
+
+namespace leankv {
+namespace bytes {
+namespace {
+
+constexpr int kRowsTile = 128, kTiles = 2;
+constexpr int kKeysTile = 128, kPagesTile = kKeysTile / kPage;
+constexpr int kConvWarps = 2, kMmaWarp = 8 + kConvWarps;
+constexpr int kThreads = 32 * (kMmaWarp + 1);
+constexpr int kPagesWarp = kPagesTile / kConvWarps;
+constexpr float kNoRef = -1.0e30f;
+constexpr float kLift = 7.f, kReach = 15.f;           // the reference of a row is its maximum - kLift when it moves, and moves beyond kReach above it
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kScaleSlots = 4;
+
+__host__ __device__ constexpr uint32_t q_bytes(int dim) { return kRowsTile * dim * 2; }
+__host__ __device__ constexpr uint32_t k_bytes(int dim) { return kKeysTile * dim * 2; }
+constexpr size_t smem_bytes(int dim) { return kTiles * q_bytes(dim) + 4 * k_bytes(dim) + 1024; }
+
+struct PromptParams {
+    const uint8_t* chunks;
+    int n_pages, H, B, G, tokens, tile_tokens;        // tokens of a row tile
+    leankv_vectors_t q, out;
+    float scale;                                      // softmax scale * log2(e)
+    const int32_t* indptr;
+    const int32_t* indices;
+    const int32_t* last;
+    int n_splits;
+    float* o_part;                                    // [split][B][tokens][heads][dim], each divided by its own sum
+    float2* ml_part;                                  // [split][B][tokens][heads]: reference and sum
+    int* status;
+};
+
+enum { kQFull, kKFull, kVFull = kKFull + 2, kKFree = kVFull + 2, kVFree = kKFree + 2, kSFull = kVFree + 2, kPFull = kSFull + 2, kPvDone = kPFull + 2, kBars = kPvDone + 2 };
+
+// Codes of a word's bytes 0, 1 / 2, 3 times s: (1024 + byte) s - 1152 s in one rounding of an exact number.
+__device__ __forceinline__ uint32_t codes_times(uint32_t w, uint32_t sel, __half2 s, __half2 off) {
+    const uint32_t x = __byte_perm(w, 0x64646464u, sel);
+    const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&x), s, off);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+// Position c of a page's 16 in the operands: the values' words hold tokens 2t, 2t + 1, 2t + 8, 2t + 9, and keys follow the same order.
+__host__ __device__ constexpr int token_at(int c) { return 2 * (c >> 2) + (c & 1) + 8 * ((c >> 1) & 1); }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams p) {
+    extern __shared__ __align__(16) uint8_t s_raw[];
+    __shared__ __align__(8) uint64_t s_bar[kBars];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_top[kConvWarps];
+    __shared__ __align__(16) float s_ks[kScaleSlots][kPagesTile];
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    uint8_t* base = s_raw + ((1024u - (umma::smem_addr(s_raw) & 1023u)) & 1023u);
+    uint8_t* s_q = base;                              // two row tiles
+    uint8_t* s_k = s_q + kTiles * q_bytes(D);         // two key tiles
+    uint8_t* s_v = s_k + 2 * k_bytes(D);              // two value tiles
+    auto bar = [&](int b) { return umma::smem_addr(&s_bar[b]); };
+    auto wait2 = [&](int b, int j) { return umma::bar_wait(bar(b + (j & 1)), (uint32_t)((j >> 1) & 1)); };      // pairs by key tile
+    auto wait1 = [&](int b, int j) { return umma::bar_wait(bar(b), (uint32_t)(j & 1)); };                       // one for every key tile
+    auto all = [&](bool done) { return __all_sync(0xffffffffu, done) != 0; };
+
+    if (warp == kMmaWarp) umma::tmem_alloc_n(umma::smem_addr(&s_tmem), 512);
+    if (tid == 0) {
+        for (int b = 0; b < kBars; ++b) {
+            const int count = b >= kKFull && b < kKFree ? 32 * kConvWarps : b >= kPFull && b < kPvDone ? kRowsTile : 1;
+            umma::bar_init_n(bar(b), count);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+
+    const int kvh = blockIdx.x % p.H, b = blockIdx.x / p.H, split = blockIdx.z;
+    const int ip = p.indptr[b], pages = p.indptr[b + 1] - ip;
+    const int start = pages > 0 ? (pages - 1) * kPage + p.last[b] - p.tokens : -p.tokens;      // position of the chunk's first token
+    const int block = (int)gridDim.y - 1 - (int)blockIdx.y;                                    // the longest first
+    const int tok0 = block * kTiles * p.tile_tokens, last_tok = min(tok0 + kTiles * p.tile_tokens, p.tokens) - 1;
+    const int n_all = start + last_tok < 0 ? 0 : (start + last_tok) / kKeysTile + 1;
+    const int t0 = (int)((long long)n_all * split / p.n_splits), n = (int)((long long)n_all * (split + 1) / p.n_splits) - t0;
+    const int page0 = t0 * kPagesTile;
+
+    bool ok = true;
+    const int tile = warp >> 2, row = tid & (kRowsTile - 1);             // of the row threads
+    const int tok = tok0 + tile * p.tile_tokens + row / p.G;
+    const bool real = warp < 8 && row < p.tile_tokens * p.G && tok < p.tokens;
+    const int head = kvh * p.G + row % p.G;
+    float factor = 0.f;
+    if (warp < 8) {
+        // ---- queries: a thread a row, fp16 with the row's power of two taken out ----
+        uint8_t* to = s_q + tile * q_bytes(D);
+        Eight<T> x[D / 8];
+        uint32_t amax = 0;
+        const T* src = static_cast<const T*>(p.q.data) + b * p.q.seq + (long long)head * p.q.head + (long long)tok * p.q.token;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+            if (real) x[c].load(src + 8 * c);
+            else x[c].zero();
+        }
+        int e2 = 0;
+        if constexpr (std::is_same<T, bf16>::value) {
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(x[c].get(e)) & 0x7fffffffu);
+            e2 = max((int)(amax >> 23) - 127 - 14, -126);
+        }
+        const float down = power_of_two(-e2);
+        factor = power_of_two(e2) * p.scale;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+            uint32_t w[4];
+            if constexpr (std::is_same<T, bf16>::value) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const __half2 v = __floats2half2_rn(x[c].get(2 * e) * down, x[c].get(2 * e + 1) * down);
+                    w[e] = *reinterpret_cast<const uint32_t*>(&v);
+                }
+            } else {
+                w[0] = x[c].a.x, w[1] = x[c].a.y, w[2] = x[c].a.z, w[3] = x[c].a.w;
+            }
+            *reinterpret_cast<uint4*>(to + umma::offset_k(row, c, D / 8)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        umma::fence_operands();
+    } else if (warp < kMmaWarp) {
+        // ---- the largest exponent of the values that this CTA will see ----
+        int top = 0;
+        const int from = page0, to = min(page0 + n * kPagesTile, pages);
+        for (int i = from + tid - 256; i < to; i += 32 * kConvWarps) {
+            const int id = p.indices[ip + i];
+            if ((unsigned)id >= (unsigned)p.n_pages) continue;
+            const uint32_t s = *reinterpret_cast<const uint32_t*>(p.chunks + ((size_t)id * p.H + kvh) * chunk_bytes(D) + 2 * half_bytes(D) + 4);
+            if (s < 0x7f800000u) top = max(top, (int)(s >> 23));
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (lane == 0) s_top[warp - 8] = top;
+    }
+    umma::fence_before_sync();
+    __syncthreads();
+    umma::fence_after_sync();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
+    const uint32_t tm_s = tmem, tm_o = tmem + 2 * kKeysTile;
+    const int top = max(max(s_top[0], s_top[1]), 1);  // biased exponent
+    float m = kNoRef, l = 0.f;
+
+    if (warp >= 8 && warp < kMmaWarp) {
+        // ---- codes to operands: a warp has pages kPagesWarp w .. of every key tile ----
+        const int first = (warp - 8) * kPagesWarp;
+        const int g = lane >> 2, t = lane & 3;
+        constexpr int kLoads = D / 32;                // 16-byte pieces of a lane, of keys and of values
+        uint4 kr[kPagesWarp][kLoads], vr[kPagesWarp][kLoads];
+        float2 sc[kPagesWarp];
+        auto page_of = [&](int j) -> int {            // lane i < kPagesWarp: page id of key tile j, or -1
+            const int i = page0 + j * kPagesTile + first + lane;
+            if (lane >= kPagesWarp || j >= n || i >= pages) return -1;
+            const int id = p.indices[ip + i];
+            if ((unsigned)id >= (unsigned)p.n_pages) {
+                atomicOr(p.status, kBadPage);
+                return -1;
+            }
+            return id;
+        };
+        auto chunk_of = [&](int ids, int i) -> const uint8_t* {
+            const int id = __shfl_sync(0xffffffffu, ids, i);
+            return id < 0 ? nullptr : p.chunks + ((size_t)id * p.H + kvh) * chunk_bytes(D);
+        };
+        const uint4 none = make_uint4(kZeroCodes, kZeroCodes, kZeroCodes, kZeroCodes);
+        // keys: lane (position of eight, 16 bytes): positions 8 (x & 1) .., channels 64 (x >> 1) + 16 (lane / 8) ..; eight lanes fill a core matrix
+        auto load_keys = [&](const uint8_t* chunk, int i) {
+#pragma unroll
+            for (int x = 0; x < kLoads; ++x)
+                kr[i][x] = chunk == nullptr ? none : __ldg(reinterpret_cast<const uint4*>(chunk + (x >> 1) * 1024 + token_at(8 * (x & 1) + (lane & 7)) * 64 + (lane >> 3) * 16));
+            sc[i] = chunk == nullptr ? make_float2(0.f, 0.f) : __ldg(reinterpret_cast<const float2*>(chunk + 2 * half_bytes(D)));
+        };
+        auto load_values = [&](const uint8_t* chunk, int i) {
+#pragma unroll
+            for (int x = 0; x < kLoads; ++x)
+                vr[i][x] = chunk == nullptr ? none : __ldg(reinterpret_cast<const uint4*>(chunk + half_bytes(D)) + x * 32 + lane);
+        };
+        int ids = page_of(0), ids_next = page_of(1);
+#pragma unroll
+        for (int i = 0; i < kPagesWarp; ++i) {
+            const uint8_t* chunk = chunk_of(ids, i);
+            load_keys(chunk, i);
+            load_values(chunk, i);
+        }
+        const __half2 one = __half2half2(__ushort_as_half(0x3c00)), minus = __half2half2(__ushort_as_half(0xe480));      // 1, -1152
+        for (int j = 0; j < n && ok; ++j) {
+            if (j >= 2) ok = all(wait2(kKFree, j - 2));
+            if (!ok) break;
+            ids = ids_next;
+            ids_next = page_of(j + 2);
+            uint8_t* k_to = s_k + (j & 1) * k_bytes(D);
+            float vs[kPagesWarp];
+#pragma unroll
+            for (int i = 0; i < kPagesWarp; ++i) {
+#pragma unroll
+                for (int x = 0; x < kLoads; ++x) {
+                    const uint32_t w[4] = {kr[i][x].x, kr[i][x].y, kr[i][x].z, kr[i][x].w};
+                    const int at = 16 * (first + i) + 8 * (x & 1) + (lane & 7);
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const uint32_t a = w[2 * half], c = w[2 * half + 1];
+                        *reinterpret_cast<uint4*>(k_to + umma::offset_k(at, 8 * (x >> 1) + 2 * (lane >> 3) + half, D / 8)) =
+                            make_uint4(codes_times(a, 0x4140, one, minus), codes_times(a, 0x4342, one, minus), codes_times(c, 0x4140, one, minus), codes_times(c, 0x4342, one, minus));
+                    }
+                }
+                vs[i] = sc[i].y;
+                if (lane == 0) s_ks[j & (kScaleSlots - 1)][first + i] = isnan(sc[i].y) ? sc[i].y : sc[i].x;
+                load_keys(chunk_of(ids, i), i);
+            }
+            umma::fence_operands();
+            umma::bar_arrive(bar(kKFull + (j & 1)));
+            if (j >= 2) ok = all(wait2(kVFree, j - 2));
+            if (!ok) break;
+            uint8_t* v_to = s_v + (j & 1) * k_bytes(D);
+#pragma unroll
+            for (int i = 0; i < kPagesWarp; ++i) {
+                // 2^(e - r) in fp16: 0 below 2^-24, and for a scale that is no number (its codes are zeros)
+                const int e = (int)(__float_as_uint(vs[i]) >> 23) - top;
+                const uint32_t bits = e > 0 || e < -24 ? 0u : e >= -14 ? (uint32_t)(e + 15) << 10 : 1u << (e + 24);
+                const __half2 s = __half2half2(__ushort_as_half((unsigned short)bits));
+                const __half2 off = __hmul2(s, minus);
+#pragma unroll
+                for (int x = 0; x < kLoads; ++x) {
+                    const uint32_t w[4] = {vr[i][x].x, vr[i][x].y, vr[i][x].z, vr[i][x].w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        *reinterpret_cast<uint2*>(v_to + umma::offset_k(8 * (4 * x + k) + g, 2 * (first + i) + (t >> 1), kKeysTile / 8) + 8 * (t & 1)) =
+                            make_uint2(codes_times(w[k], 0x4140, s, off), codes_times(w[k], 0x4342, s, off));
+                }
+                load_values(chunk_of(ids, i), i);
+            }
+            umma::fence_operands();
+            umma::bar_arrive(bar(kVFull + (j & 1)));
+        }
+    } else if (warp == kMmaWarp) {
+        // ---- products ----
+        auto scores = [&](int r, int j) {
+            if (umma::elect()) {
+                const uint64_t a = umma::desc_k(umma::smem_addr(s_q + r * q_bytes(D)), D / 8), c = umma::desc_k(umma::smem_addr(s_k + (j & 1) * k_bytes(D)), D / 8);
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks)
+                    umma::mma_f16_n(tm_s + r * kKeysTile, a + (uint64_t)ks * (2 * umma::kLbo >> 4), c + (uint64_t)ks * (2 * umma::kLbo >> 4), umma::idesc_n(kKeysTile), ks > 0);
+                umma::commit(bar(kSFull + r));
+                if (r == kTiles - 1 && j + 2 < n) umma::commit(bar(kKFree + (j & 1)));
+            }
+            __syncwarp();
+        };
+        if (n > 0) ok = all(wait2(kKFull, 0));
+        if (n > 0 && ok) {
+            umma::fence_after_sync();
+            for (int r = 0; r < kTiles; ++r) scores(r, 0);
+        }
+        for (int j = 0; j < n && ok; ++j) {
+            ok = all(wait2(kVFull, j));
+            for (int r = 0; r < kTiles && ok; ++r) {
+                ok = all(wait1(kPFull + r, j));
+                if (!ok) break;
+                umma::fence_after_sync();
+                if (umma::elect()) {
+                    const uint64_t c = umma::desc_k(umma::smem_addr(s_v + (j & 1) * k_bytes(D)), kKeysTile / 8);
+#pragma unroll
+                    for (int ks = 0; ks < kKeysTile / 16; ++ks)
+                        umma::mma_f16_ts(tm_o + r * D, tm_s + r * kKeysTile + 8 * ks, c + (uint64_t)ks * (2 * umma::kLbo >> 4), umma::idesc_n(D), j > 0 || ks > 0);
+                    umma::commit(bar(kPvDone + r));
+                    if (r == kTiles - 1 && j + 2 < n) umma::commit(bar(kVFree + (j & 1)));
+                }
+                __syncwarp();
+                if (j + 1 < n) {                       // its scores go over these weights
+                    if (r == 0) ok = all(wait2(kKFull, j + 1));
+                    ok = ok && all(wait1(kPvDone + r, j));
+                    if (ok) {
+                        umma::fence_after_sync();
+                        scores(r, j + 1);
+                    }
+                }
+            }
+        }
+    } else {
+        // ---- rows ----
+        const int lane0 = 32 * (warp & 3);
+        const int qpos = start + (real ? tok : last_tok);       // rows that are none see what the last token sees; nothing of theirs is kept
+        const uint32_t tm = tm_s + tile * kKeysTile, to = tm_o + tile * D;
+        for (int j = 0; j < n; ++j) {
+            ok = all(wait2(kVFull, j) && wait1(kSFull + tile, j));       // the first for the scales; its next phase needs these rows' weights
+            if (!ok) break;
+            umma::fence_after_sync();
+            uint32_t s[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) umma::ld32_async(s[c], tm, lane0, 32 * c);
+            float ks[kPagesTile];
+            const float4* scales = reinterpret_cast<const float4*>(s_ks[j & (kScaleSlots - 1)]);
+#pragma unroll
+            for (int i = 0; i < kPagesTile / 4; ++i) {
+                const float4 v = scales[i];
+                ks[4 * i] = v.x * factor, ks[4 * i + 1] = v.y * factor, ks[4 * i + 2] = v.z * factor, ks[4 * i + 3] = v.w * factor;
+            }
+            umma::settle(s[0]);
+            umma::settled(s[1]);
+            umma::settled(s[2]);
+            umma::settled(s[3]);
+            const int k1 = qpos - (t0 + j) * kKeysTile;                  // the row's last key of the tile
+            const bool cut = __any_sync(0xffffffffu, k1 < kKeysTile - 1);
+            if (cut) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int x = 0; x < 32; ++x)
+                        if (32 * c + (x & 16) + token_at(x & 15) > k1) s[c][x] = 0xff800000u;
+            }
+            float best = kNoRef;
+#pragma unroll
+            for (int i = 0; i < kPagesTile; ++i) {
+                float top4[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) top4[x] = __uint_as_float(s[i >> 1][16 * (i & 1) + x]);
+#pragma unroll
+                for (int x = 4; x < 16; ++x) top4[x & 3] = fmaxf(top4[x & 3], __uint_as_float(s[i >> 1][16 * (i & 1) + x]));
+                best = fmaxf(best, fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * ks[i]);
+            }
+            const bool raise = best > m + kReach;
+            if (__any_sync(0xffffffffu, raise)) {
+                // nothing is being added to these outputs: the scores were asked for behind the last value product
+                const float now = raise ? best - kLift : m, f = ex2(m - now);
+                m = now;
+                l *= f;
+                if (j > 0) scale_outputs(to, lane0, D, f);
+            }
+            Two sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t w16[16];
+#pragma unroll
+                for (int x = 0; x < 32; x += 2) {
+                    const float k = ks[2 * c + (x >> 4)];
+                    Two w = fma2({__uint_as_float(s[c][x]), __uint_as_float(s[c][x + 1])}, {k, k}, {-m, -m});
+                    w.x = ex2(w.x);
+                    w.y = ex2(w.y);
+                    if (cut) {                         // a scale that is no number does not reach a row that does not see its block
+                        if (32 * c + (x & 16) + token_at(x & 15) > k1) w.x = 0.f;
+                        if (32 * c + (x & 16) + token_at((x + 1) & 15) > k1) w.y = 0.f;
+                    }
+                    sum[(x >> 1) & 1] = add2(sum[(x >> 1) & 1], w);
+                    const __half2 h = __floats2half2_rn(w.x, w.y);
+                    w16[x / 2] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+                umma::st16_async(w16, tm, lane0, 16 * c);
+            }
+            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+            umma::stored();
+            umma::fence_before_sync();
+            umma::bar_arrive(bar(kPFull + tile));
+        }
+        if (ok && n > 0) ok = all(wait1(kPvDone + tile, n - 1));
+        umma::fence_after_sync();
+        if (!ok && lane == 0) atomicOr(p.status, kTimedOut);
+
+        // ---- out ----
+        const float inv = !ok ? NAN : l == 0.f ? 0.f : 1.f / l;
+        const float back = __uint_as_float((uint32_t)top << 23);
+        const long long vec = ((long long)b * p.tokens + tok) * (p.H * p.G) + head;
+        T* dst = static_cast<T*>(p.out.data) + b * p.out.seq + (long long)head * p.out.head + (long long)tok * p.out.token;
+        float* part = p.o_part + ((long long)split * p.B * p.tokens * (p.H * p.G) + vec) * D;
+#pragma unroll
+        for (int c0 = 0; c0 < D; c0 += 32) {
+            uint32_t o[32];
+            __syncwarp();
+            if (n > 0) umma::ld32(o, to, lane0, c0);
+            if (!real) continue;
+#pragma unroll
+            for (int x = 0; x < 32; x += 8) {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = n > 0 ? __uint_as_float(o[x + e]) * inv * back : 0.f;
+                if (p.n_splits > 1) {
+                    reinterpret_cast<float4*>(part + c0 + x)[0] = make_float4(v[0], v[1], v[2], v[3]);
+                    reinterpret_cast<float4*>(part + c0 + x)[1] = make_float4(v[4], v[5], v[6], v[7]);
+                } else {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = pack_as<T>(v[2 * e], v[2 * e + 1]);
+                    *reinterpret_cast<uint4*>(dst + c0 + x) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+        }
+        if (real && p.n_splits > 1) p.ml_part[(long long)split * p.B * p.tokens * (p.H * p.G) + vec] = make_float2(m, ok ? l : NAN);
+    }
+    if (warp >= 8 && !ok && lane == 0) atomicOr(p.status, kTimedOut);
+    umma::fence_before_sync();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        umma::fence_after_sync();
+        umma::tmem_free_n(tmem, 512);
+    }
+}
+
+// The shares of a row's keys, in order; a thread has four numbers.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) join_kernel(const PromptParams p) {
+    pdl_begin();
+    const long long n_vec = (long long)p.B * p.tokens * (p.H * p.G);
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, vec = i / (D / 4);
+    const int d4 = (int)(i % (D / 4));
+    if (vec >= n_vec) return;
+    float top = kNoRef;
+    for (int s = 0; s < p.n_splits; ++s) top = fmaxf(top, p.ml_part[s * n_vec + vec].x);
+    float sum = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < p.n_splits; ++s) {
+        const float2 ml = p.ml_part[s * n_vec + vec];
+        const float w = ml.y * ex2(ml.x - top);
+        const float4 o = *reinterpret_cast<const float4*>(p.o_part + (s * n_vec + vec) * D + 4 * d4);
+        sum += w;
+        v.x = fmaf(o.x, w, v.x), v.y = fmaf(o.y, w, v.y), v.z = fmaf(o.z, w, v.z), v.w = fmaf(o.w, w, v.w);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int heads = p.H * p.G, head = (int)(vec % heads);
+    const long long tok = vec / heads % p.tokens, b = vec / heads / p.tokens;
+    T* dst = static_cast<T*>(p.out.data) + b * p.out.seq + head * p.out.head + tok * p.out.token + 4 * d4;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_as<T>(v.x * inv, v.y * inv), pack_as<T>(v.z * inv, v.w * inv));
+}
+
+template <typename T, int D>
+int launch(const PromptParams& p, int blocks, cudaStream_t st) {
+    static std::atomic<unsigned long long> ready{0};             // a bit for each device
+    int dev = 0;
+    LEANKV_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) return LEANKV_ELIMIT;
+    if (((ready.load(std::memory_order_acquire) >> dev) & 1ull) == 0) {
+        LEANKV_CUDA_TRY(cudaFuncSetAttribute(prompt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(D)));
+        ready.fetch_or(1ull << dev, std::memory_order_release);
+    }
+    LEANKV_CUDA_TRY(launch_plain(prompt_kernel<T, D>, dim3((unsigned)(p.H * p.B), (unsigned)blocks, (unsigned)p.n_splits), dim3(kThreads), smem_bytes(D), st, p));
+    if (p.n_splits > 1) {
+        const long long work = (long long)p.B * p.tokens * p.H * p.G * (D / 4);
+        LEANKV_CUDA_TRY(launch_early(join_kernel<T, D>, dim3((unsigned)((work + 255) / 256)), dim3(256), 0, st, p));
+    }
+    return LEANKV_OK;
+}
+
+}  // namespace
+}  // namespace bytes
+}  // namespace leankv
+
+using namespace leankv;
+
+extern "C" int leankv_byte_prompt_attn(const leankv_byte_pool_t* pool, int dtype, const leankv_vectors_t* q, const leankv_vectors_t* out, int B,
+                                       int q_heads, int tokens, float scale, const int32_t* kv_indptr, const int32_t* kv_page_indices,
+                                       const int32_t* kv_last_page_len, int max_pages_seq, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!bytes::good_pool(pool) || !bytes::good_type(dtype) || !q || !out || !q->data || !out->data || B <= 0 || tokens <= 0 || q_heads <= 0 ||
+        q_heads % pool->kv_heads != 0 || !kv_indptr || !kv_page_indices || !kv_last_page_len || max_pages_seq < 0 || !(scale > 0.f))
+        return LEANKV_EINVAL;
+    if (dtype == LEANKV_BYTES_F32) return LEANKV_EUNSUPPORTED;
+    if (B > LEANKV_BYTES_MAX_BATCH || q_heads / pool->kv_heads > LEANKV_BYTES_MAX_GROUP) return LEANKV_ELIMIT;
+    if (!bytes::aligned_pool(pool) || !bytes::aligned_vectors(q, dtype, B, q_heads, tokens) ||
+        !bytes::aligned_vectors(out, dtype, B, q_heads, tokens) || !aligned16(workspace))
+        return LEANKV_EALIGN;
+    if (!workspace || workspace_bytes < bytes::kWorkspaceBytes) return LEANKV_EWORKSPACE;
+    bytes::PromptParams p = {};
+    p.chunks = static_cast<const uint8_t*>(pool->chunks);
+    p.n_pages = pool->n_pages, p.H = pool->kv_heads, p.B = B, p.G = q_heads / pool->kv_heads, p.tokens = tokens;
+    p.tile_tokens = bytes::kRowsTile / p.G;
+    p.q = *q, p.out = *out;
+    p.scale = scale * bytes::kLog2e;
+    p.indptr = kv_indptr, p.indices = kv_page_indices, p.last = kv_last_page_len;
+    p.status = static_cast<int*>(workspace);
+    const long long blocks = ((long long)tokens + bytes::kTiles * p.tile_tokens - 1) / (bytes::kTiles * p.tile_tokens);
+    const long long ctas = blocks * p.H * B;
+    if (blocks > 65535 || (long long)p.H * B > 0x7fffffffll) return LEANKV_ELIMIT;
+    // fewer CTAs than SMs share the keys, four key tiles each at least; the partial sums of so many CTAs fit the workspace
+    const long long key_tiles = ((long long)max_pages_seq + bytes::kPagesTile - 1) / bytes::kPagesTile;
+    const long long room = std::min(sm_count(), bytes::kPromptCtas) / ctas;
+    p.n_splits = (int)std::max(1ll, std::min({room, key_tiles / 4, 16ll}));
+    p.ml_part = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + bytes::kPartialsAt);
+    p.o_part = reinterpret_cast<float*>(p.ml_part + (size_t)bytes::kPromptCtas * bytes::kPromptRows);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (pool->dim == 128) return dtype == LEANKV_BYTES_F16 ? bytes::launch<__half, 128>(p, (int)blocks, st) : bytes::launch<bf16, 128>(p, (int)blocks, st);
+    return dtype == LEANKV_BYTES_F16 ? bytes::launch<__half, 64>(p, (int)blocks, st) : bytes::launch<bf16, 64>(p, (int)blocks, st);
+}

@@ -85,6 +85,7 @@ class ByteKVCache(PagedKVCache):
         size = _native.byte_lib().leankv_byte_attn_workspace_bytes() if self._device.type == "cuda" else 0
         self._workspace = torch.zeros(size, dtype=torch.uint8, device=self._device)
         self._scale = 1.0 / math.sqrt(head_dim)
+        self._prompt_rows = 128               # (token, query head) rows of a kv head from which a chunk goes to the prompt kernel
         self._alloc_tables(0)
 
     # ── arguments ──────────────────────────────────────────────────────
@@ -178,15 +179,19 @@ class ByteKVCache(PagedKVCache):
 
     # ── attention ──────────────────────────────────────────────────────
 
-    def _attend(self, layer_idx: int, q: torch.Tensor, out: torch.Tensor, tokens: int, lists=None, n_lists: int = 0) -> None:
+    def _attend(self, layer_idx: int, q: torch.Tensor, out: torch.Tensor, tokens: int, lists=None, n_lists: int = 0, prompt: bool = False) -> None:
         """``q`` and ``out`` [B, Hq, (T,) D]: the last ``tokens`` tokens of each sequence over the pages."""
         pool, lib, batch = self._layer(layer_idx), _native.byte_lib(), q.shape[0]
         indptr, flat, last = self._device_meta(batch)
         (qd, q), (od, _) = _vectors(q, q.dim() == 4), _vectors(out, q.dim() == 4)
+        call = [pool, _TYPES[q.dtype], byref(qd), byref(od), batch, self.num_q_heads, tokens, self._scale, indptr.data_ptr(),
+                flat.data_ptr(), last.data_ptr(), self._most_pages(batch)]
         with _native.on_device(self._device):
-            rc = lib.leankv_byte_attn(pool, _TYPES[q.dtype], byref(qd), byref(od), batch, self.num_q_heads, tokens, self._scale,
-                                      indptr.data_ptr(), flat.data_ptr(), last.data_ptr(), self._most_pages(batch), lists, n_lists,
-                                      self._workspace.data_ptr(), self._workspace.numel(), _native.current_stream())
+            if prompt:
+                rc = lib.leankv_byte_prompt_attn(*call, self._workspace.data_ptr(), self._workspace.numel(), _native.current_stream())
+            else:
+                rc = lib.leankv_byte_attn(*call, self.max_pages - self._free_count, lists, n_lists, self._workspace.data_ptr(), self._workspace.numel(),
+                                          _native.current_stream())
         _native.check(rc, "leankv_byte_attn", lib)
 
     def decode_attention(self, layer_idx: int, query: torch.Tensor) -> torch.Tensor:
@@ -235,7 +240,8 @@ class ByteKVCache(PagedKVCache):
             raise RuntimeError("prefill_attention: the chunk has not been appended to this sequence")
         out = torch.empty(batch, t_new, self.num_q_heads, self.head_dim, dtype=q.dtype, device=q.device).transpose(1, 2)
         if t_new:
-            self._attend(layer_idx, q, out, t_new)
+            rows = t_new * (self.num_q_heads // self.num_kv_heads)
+            self._attend(layer_idx, q, out, t_new, prompt=rows >= self._prompt_rows and q.dtype != torch.float32)
         return out if out.dtype == query.dtype else out.to(query.dtype)
 
     def kernel_status(self) -> int:

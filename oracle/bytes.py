@@ -105,16 +105,17 @@ class Cache:
         if n == 0:
             return out
         k, v = self.values(b, 0), self.values(b, 1)
+        first = n - q.shape[1]                          # position of the first query
         for hq in range(q.shape[0]):
             h = hq // group
-            for t in range(q.shape[1]):
-                end = n - q.shape[1] + t + 1
-                if end <= 0:
-                    continue
-                see = torch.arange(end) if chosen is None else torch.cat(
-                    [torch.arange(BLOCK * j, min(BLOCK * j + BLOCK, end)) for j in chosen[h].tolist() if j >= 0])
-                w = torch.softmax(k[h, see] @ q[hq, t] / math.sqrt(self.dim), 0)
-                out[hq, t] = w @ v[h, see]
+            if chosen is not None:
+                at = torch.cat([torch.arange(BLOCK * j, min(BLOCK * j + BLOCK, n)) for j in chosen[h].tolist() if j >= 0])
+                w = torch.softmax(q[hq] @ k[h, at].T / math.sqrt(self.dim), -1)
+                out[hq] = w @ v[h, at]
+                continue
+            for t in range(max(0, -first), q.shape[1]):                # what nobody sees does not enter, not even as 0 * NaN
+                w = torch.softmax(k[h, :first + t + 1] @ q[hq, t] / math.sqrt(self.dim), 0)
+                out[hq, t] = w @ v[h, :first + t + 1]
         return out
 
     def choose(self, b: int, q: torch.Tensor, blocks: int, sinks: int, recent: int) -> torch.Tensor:

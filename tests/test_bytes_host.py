@@ -151,18 +151,24 @@ def test_attention_checks_its_arguments():
     need = lib.leankv_byte_attn_workspace_bytes()
 
     def f(pool=None, q=None, out=None, **kw):
-        a = {**dict(B=1, heads=8, tokens=1, scale=0.1, ip=64, ids=64, last=64, pages=4, lists=None, n=0, ws=1 << 22, bytes=need, st=None), **kw}
-        dtype = a.pop("dtype", 0)
+        a = {**dict(B=1, heads=8, tokens=1, scale=0.1, ip=64, ids=64, last=64, pages=4, total=4, lists=None, n=0, ws=1 << 22, bytes=need, st=None), **kw}
+        dtype, prompt = a.pop("dtype", 0), a.pop("prompt", False)
+        if prompt:
+            del a["total"], a["lists"], a["n"]
+            return lib.leankv_byte_prompt_attn(ctypes.byref(pool or _pool()), dtype, ctypes.byref(q or _vec()), ctypes.byref(out or _vec()), *a.values())
         return lib.leankv_byte_attn(ctypes.byref(pool or _pool()), dtype, ctypes.byref(q or _vec()), ctypes.byref(out or _vec()), *a.values())
 
     for bad, code in BAD_POOLS:
-        assert f(_pool(**bad)) == code
+        assert f(_pool(**bad)) == code and f(_pool(**bad), prompt=True) == code
     for kw, code in ((dict(dtype=3), -1), (dict(B=0), -1), (dict(heads=0), -1), (dict(heads=7), -1), (dict(heads=34), -6), (dict(tokens=0), -1),
-                     (dict(B=1025), -6), (dict(ip=None), -1), (dict(ids=None), -1), (dict(last=None), -1), (dict(pages=-1), -1),
+                     (dict(B=1025), -6), (dict(ip=None), -1), (dict(ids=None), -1), (dict(last=None), -1), (dict(pages=-1), -1), (dict(total=-1), -1),
                      (dict(lists=64, n=0), -1), (dict(lists=64, n=4, tokens=2), -1), (dict(ws=None), -3), (dict(bytes=need - 1), -3),
                      (dict(ws=(1 << 22) + 4), -2), (dict(q=_vec(data=None)), -1), (dict(out=_vec(data=None)), -1), (dict(q=_vec(data=4)), -2),
                      (dict(out=_vec(head=4)), -2), (dict(q=_vec(token=12), tokens=2), -2), (dict(tokens=1 << 30), -6)):
         assert f(**kw) == code, kw
+        if "lists" not in kw and "total" not in kw:
+            assert f(**kw, prompt=True) == code, kw
+    assert f(dtype=2, prompt=True) == -5 and f(scale=0.0, prompt=True) == -1 and f(scale=math.nan, prompt=True) == -1
     assert lib.leankv_byte_status(None, None) == -1
 
 

@@ -5,6 +5,10 @@ form scores, weights and sums in 32 bits from exact codes and a query of 22 bits
 ``dim`` products in fp32 (tensor-core sums drop bits of 2^-22 of the largest term at worst), |s| up to some 20 in these tests, so a weight is off by at most
 2^-22 * 20 * 2 ~ 1e-5 of itself, and so is an output relative to its row; then one rounding to the output type, eps / 2 at most. Bound: relative 2-norm
 over a row ``eps / 2 + 2e-5``.
+
+The prompt kernel rounds each weight to fp16 (relative 2^-11 at most, both ways alike) before the value product. Its part of a row's error is at most
+2^-11 sum_t w_t |v_t|, which the rows of these tests, whose values have random signs, are not far above: ``|out| >= |v| / sqrt(n)`` in the mean and the errors
+add up like the values do, so that relative to the row it stays below 2^-11 again with a factor of 2 for small rows: bound ``eps / 2 + 2e-5 + 2^-10``.
 """
 
 import math
@@ -36,10 +40,10 @@ def row_errors(got, want):
     return ((got - want).norm(dim=-1) / size.clamp_min(1e-300))[size > 0]
 
 
-def close(got, want, dtype):
+def close(got, want, dtype, weights=False):
     err = row_errors(got, want)
     assert got.dtype == dtype
-    bound = torch.finfo(dtype).eps / 2 + 2e-5
+    bound = torch.finfo(dtype).eps / 2 + 2e-5 + (2.0 ** -10 if weights else 0.0)
     assert len(err) == 0 or float(err.max()) <= bound, (float(err.max()), bound)
 
 
@@ -84,11 +88,14 @@ class Pair:
         assert self.cache.kernel_status() == 0
 
     def check_prompt(self, tokens):
+        """Both kernels, whichever the number of rows would choose."""
         q = self.queries(tokens)
-        got = self.cache.prefill_attention(0, q.to(DEV))
         want = torch.stack([self.plain.attend(b, q[b]) for b in range(self.batch)])
-        close(got, want, self.dtype)
-        assert self.cache.kernel_status() == 0
+        for rows in (1, 1 << 30):
+            self.cache._prompt_rows = rows
+            got = self.cache.prefill_attention(0, q.to(DEV))
+            close(got, want, self.dtype, weights=rows == 1 and self.dtype != F32)
+            assert self.cache.kernel_status() == 0
 
     def check_sparse(self, blocks, sinks=1, recent=2):
         q = self.queries()
@@ -165,18 +172,20 @@ def test_a_block_that_holds_no_number_answers_nobody_who_sees_it(bad, which):
     got = p.cache.decode_attention(0, q.to(DEV)).cpu()
     assert bool(got[0, 2:].isnan().all())
     q20 = p.queries(20)
-    prompt = p.cache.prefill_attention(0, q20.to(DEV)).cpu()
-    assert bool(prompt[0, 2:].isnan().all())           # every token of the chunk shares the block or comes behind it
     q40 = p.queries(40)                                # positions 12 .. 51; those before 32 do not see block 2
-    wide = p.cache.prefill_attention(0, q40.to(DEV))
-    assert bool(wide[0, 2:, 20:].isnan().all())
-    want = [p.plain.attend(b, q40[b]) for b in range(2)]
-    close(wide[0, :2], want[0][:2], BF16)
-    close(wide[1], want[1], BF16)
     cut = obytes.Cache(2, 2, 64)
     cut.blocks = [[[row[:2] for row in seq] for seq in side] for side in p.plain.blocks]
     cut.n = [32, 32]
-    close(wide[0, 2:, :20], cut.attend(0, q40[0, :, :20])[2:], BF16)
+    for rows in (1, 1 << 30):                          # either kernel
+        p.cache._prompt_rows = rows
+        prompt = p.cache.prefill_attention(0, q20.to(DEV)).cpu()
+        assert bool(prompt[0, 2:].isnan().all())       # every token of the chunk shares the block or comes behind it
+        wide = p.cache.prefill_attention(0, q40.to(DEV))
+        assert bool(wide[0, 2:, 20:].isnan().all())
+        want = [p.plain.attend(b, q40[b]) for b in range(2)]
+        close(wide[0, :2], want[0][:2], BF16, rows == 1)
+        close(wide[1], want[1], BF16, rows == 1)
+        close(wide[0, 2:, :20], cut.attend(0, q40[0, :, :20])[2:], BF16, rows == 1)
     # the block counts as the best one of all
     sparse, chosen = p.cache.sparse_decode_attention(0, q.to(DEV), 3, 0, 1, return_blocks=True)
     if which == 0:
@@ -296,6 +305,50 @@ def test_prompt_attention_is_causal(dtype, dim, group, heads, past, tokens):
     p.check_prompt(tokens)
 
 
+@pytest.mark.parametrize("dtype, dim, group, heads, past, tokens", [
+    (F16, 128, 4, 2, 0, 260), (BF16, 128, 4, 1, 700, 130), (F16, 64, 3, 3, 129, 200), (BF16, 64, 16, 1, 1000, 40), (F16, 128, 1, 2, 2100, 300),
+    (BF16, 128, 7, 1, 383, 129), (F16, 64, 5, 1, 4000, 64)])
+def test_prompt_attention_over_several_tiles_and_shares(dtype, dim, group, heads, past, tokens):
+    p = Pair(2, heads, group, dim, dtype, pages=600, seed=past + tokens)
+    if past:
+        p.append(past)
+    p.append(50, batch=1)
+    p.append(tokens)
+    p.check_prompt(tokens)
+    q = p.queries(tokens).to(DEV)
+    p.cache._prompt_rows = 1
+    first = p.cache.prefill_attention(0, q)
+    assert all(torch.equal(p.cache.prefill_attention(0, q), first) for _ in range(3))
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-6, 1.0])
+def test_prompt_attention_on_values_of_different_magnitudes(scale):
+    """Value blocks whose scales differ by up to 2^20 under the largest one, which the weights do not prefer."""
+    p = Pair(1, 1, 2, 64, BF16, pages=80)
+    for i in range(20):
+        k = vectors(p.gen, 1, 1, 16, 64, BF16, large=False)
+        v = (vectors(p.gen, 1, 1, 16, 64, torch.float32, large=False) * scale * 2.0 ** -(i % 5 * 5)).to(BF16)
+        p.cache.append(0, k.to(DEV), v.to(DEV))
+        p.plain.append(k, v)
+    p.check_prompt(200)
+
+
+def test_prompt_attention_of_rows_whose_reference_moves():
+    """Scores that rise from key tile to key tile, beyond what weights in fp16 reach."""
+    p = Pair(1, 1, 4, 64, BF16, pages=80)
+    k = (torch.randn(1, 1, 700, 64, generator=p.gen) * 0.3 + (torch.arange(700) // 50 * 0.2)[None, None, :, None]).to(BF16)
+    v = vectors(p.gen, 1, 1, 700, 64, BF16, large=False)
+    p.cache.append(0, k.to(DEV), v.to(DEV))
+    p.plain.append(k, v)
+    q = (torch.rand(1, 4, 300, 64, generator=p.gen) * torch.tensor([1.0, 3.0, -2.0, 0.1])[None, :, None, None]).to(BF16)
+    p.cache._prompt_rows = 1
+    got = p.cache.prefill_attention(0, q.to(DEV))
+    want = p.plain.attend(0, q[0])[None]
+    # scores reach 130: 2^-22 of the largest product sums to 2e-5 * 130 / 20 in a weight; values of random sign as everywhere
+    err = row_errors(got, want)
+    assert float(err.max()) <= torch.finfo(BF16).eps / 2 + 2.0 ** -10 + 2e-4
+
+
 def test_prompt_attention_of_sequences_of_different_lengths():
     p = Pair(3, 2, 4, 128, F16)
     p.append(30, batch=1)
@@ -346,8 +399,10 @@ def test_other_strides_other_types_and_views():
     p.check_pages()
     q = torch.randn(2, 40, 6, 64, generator=p.gen).to(BF16)
     on = q.to(DEV)
-    whole = p.cache.prefill_attention(0, on.transpose(1, 2))
-    close(whole, torch.stack([p.plain.attend(b, q[b].transpose(0, 1)) for b in range(2)]), BF16)
+    for rows in (1, 1 << 30):
+        p.cache._prompt_rows = rows
+        whole = p.cache.prefill_attention(0, on.transpose(1, 2))
+        close(whole, torch.stack([p.plain.attend(b, q[b].transpose(0, 1)) for b in range(2)]), BF16, rows == 1)
     one = p.cache.decode_attention(0, on.transpose(1, 2)[:, :, 7])
     assert torch.equal(one, p.cache.decode_attention(0, on[:, 7].contiguous()))
     odd = torch.zeros(2, 6, 68, dtype=BF16, device=DEV)
@@ -465,6 +520,8 @@ def test_captured_calls_on_another_stream_replay_on_new_inputs():
         dense = p.cache.decode_attention(0, q)
         few, chosen = p.cache.sparse_decode_attention(0, q, 8, return_blocks=True)
         prompt = p.cache.prefill_attention(0, q[:, :, None].expand(-1, -1, 3, -1))
+        p.cache._prompt_rows = 1
+        other = p.cache.prefill_attention(0, q[:, :, None].expand(-1, -1, 3, -1))
     for _ in range(3):
         new = p.queries()
         q.copy_(new)
@@ -475,7 +532,9 @@ def test_captured_calls_on_another_stream_replay_on_new_inputs():
             want = p.plain.choose(b, new[b], 8, 1, 2)
             assert torch.equal(chosen[b].cpu(), want)
             close(few[b], p.plain.attend(b, new[b, :, None], want)[:, 0], F16)
-        close(prompt, torch.stack([p.plain.attend(b, new[b, :, None].expand(-1, 3, -1)) for b in range(2)]), F16)
+        want = torch.stack([p.plain.attend(b, new[b, :, None].expand(-1, 3, -1)) for b in range(2)])
+        close(prompt, want, F16)
+        close(other, want, F16, weights=True)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -513,6 +572,12 @@ def test_page_ids_outside_the_pool_are_reported_and_left_alone():
             close(got[b], p.plain.attend(b, q[b, :, None])[:, 0], F16)
         p.cache.sparse_decode_attention(0, q.to(DEV), 2, 0, 1)
         p.cache.prefill_attention(0, q[:, :, None].expand(-1, -1, 9, -1).to(DEV))
+        assert p.cache.kernel_status() == 2
+        p.cache._workspace[:4].zero_()
+        p.cache._prompt_rows = 1
+        got = p.cache.prefill_attention(0, q[:, :, None].to(DEV))
+        for b in (0, 2):
+            close(got[b], p.plain.attend(b, q[b, :, None]), F16, weights=True)
         assert p.cache.kernel_status() == 2
         p.cache._workspace[:4].zero_()
         assert p.cache[0][0].shape == (3, 2, 40, 64)
