@@ -34,10 +34,9 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kCtasPerSm = 4;
 constexpr int kMaxCluster = 8;
-constexpr int kFewPages = 4;                       // of a CTA: below, a smaller cluster
-constexpr int kPartPages = 32;                     // of a CTA: below, a triple is not cut into parts (joining them costs 2 - 3 us)
+constexpr int kFewPages = 8;                       // of a CTA: below, a smaller cluster
+constexpr int kPartPages = 16;                     // of a CTA: below, a triple is not cut into parts, nor into two (joining them costs 2 - 3 us)
 constexpr int kWavePages = 64;                     // of a CTA where there is more than one wave of them
 // A row's reference lies kLift below the largest score seen when it last moved, and moves when a score exceeds it by more than kReach: weights are at most
 // 2^15 in fp16, and one of 2^-24 of the largest is still a normal number there. Moving costs the rescaling of all sums.
@@ -129,7 +128,7 @@ __device__ __forceinline__ void store4_as(T* to, float4 v) {
 
 // kTiles: groups of eight rows.
 template <typename T, int D, int kTiles>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kThreads, 4) attn_kernel(const AttnParams p) {
     constexpr int kStages = stages(D);
     constexpr uint32_t kChunk = chunk_bytes(D);
     constexpr int kSteps = D / 16;                 // of the score product, and 16-channel tiles of the values'
@@ -583,39 +582,69 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_kernel(const AttnPa
     }
 }
 
+// How a launch is cut: CTAs of a cluster, pages of a part (0: triples are whole), clusters of the grid.
+struct Plan {
+    int ctas;
+    int part_pages;
+    long long clusters;
+};
+// room[i]: clusters of 2^i CTAs that the device holds at once; triples, their longest one's pages, all their pages.
+Plan make_plan(const int (&room)[4], long long triples, long long longest, long long total) {
+    int i = 0;
+    Plan plan;
+    if (triples > room[0]) {
+        // more than one wave: CTAs of kWavePages, which even out by themselves
+        while (i < 3 && longest > (kWavePages << i)) ++i;
+        plan.part_pages = kWavePages << i;
+    } else {
+        // as many CTAs of a triple as there is room for, with kFewPages each at least; parts where whole clusters fit more than once
+        while (i < 3 && room[i + 1] >= triples && longest > (kFewPages << i)) ++i;
+        const long long most = room[i] / triples, even = (longest + most - 1) / most;
+        plan.part_pages = (int)std::max(room[i] > triples ? std::min(even, (total + room[i] - triples - 1) / (room[i] - triples)) : even, (long long)kPartPages << i);
+    }
+    plan.ctas = 1 << i;
+    if (total / plan.part_pages + triples > kMaxParts)
+        plan.part_pages = (int)(triples >= kMaxParts ? longest : std::max<long long>(plan.part_pages, total / (kMaxParts - triples) + 1));
+    if (longest <= plan.part_pages || (triples <= room[0] && longest <= 2ll * kPartPages << i)) plan.part_pages = 0;
+    plan.clusters = plan.part_pages == 0 ? triples : total / plan.part_pages + triples;
+    return plan;
+}
+
 template <typename T, int D, int kTiles>
 int launch(const AttnParams& p, int max_pages_seq, long long total_pages, cudaStream_t st) {
     static std::atomic<unsigned long long> ready{0};             // a bit for each device
+    static int rooms[64][4];
     int dev = 0;
     LEANKV_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64) return LEANKV_ELIMIT;
     constexpr size_t smem = ring_bytes(D);
     if (((ready.load(std::memory_order_acquire) >> dev) & 1ull) == 0) {
         LEANKV_CUDA_TRY(cudaFuncSetAttribute(attn_kernel<T, D, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        for (int i = 0; i < 4; ++i) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(1u << i);
+            cfg.blockDim = dim3(kThreads);
+            cfg.dynamicSmemBytes = smem;
+            cudaLaunchAttribute attr;
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = 1u << i, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+            cfg.attrs = &attr, cfg.numAttrs = 1;
+            int n = 0;
+            LEANKV_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, attn_kernel<T, D, kTiles>, &cfg));
+            rooms[dev][i] = std::max(n, 1);
+        }
         ready.fetch_or(1ull << dev, std::memory_order_release);
     }
-    // Clusters: as many CTAs of a triple as the device holds at once, up to eight and no fewer pages each than kFewPages; beyond one wave kWavePages each. Parts:
-    // where whole clusters fit more than once, but not below kPartPages a CTA; bounded by the workspace.
-    const long long room = (long long)kCtasPerSm * sm_count(), triples = (long long)p.B * p.H * p.row_tiles;
-    const long long longest = p.lists == nullptr ? max_pages_seq : std::min(max_pages_seq, p.n_lists);
-    const long long total = (p.lists == nullptr ? std::min(total_pages, (long long)p.B * longest) : (long long)p.B * longest) * p.H * p.row_tiles;
-    const bool waves = triples > room;
-    int ctas = 1;
-    while (ctas < kMaxCluster && (waves ? longest > (long long)ctas * kWavePages : 2 * ctas * triples <= room && longest > (long long)ctas * kFewPages)) ctas *= 2;
-    const long long clusters = room / ctas;
-    long long part_pages = waves ? (long long)ctas * kWavePages
-                                 : std::min((longest + clusters / triples - 1) / (clusters / triples),
-                                            clusters > triples ? (total + clusters - triples - 1) / (clusters - triples) : longest);
-    part_pages = std::max({part_pages, (long long)ctas * kPartPages, 1ll});
-    if (total / part_pages + triples > kMaxParts) part_pages = triples >= kMaxParts ? longest : std::max(part_pages, total / (kMaxParts - triples) + 1);
+    const long long rows = (long long)p.H * p.row_tiles, longest = p.lists == nullptr ? max_pages_seq : std::min(max_pages_seq, p.n_lists);
+    const long long total = std::min(total_pages, p.B * longest) * rows;
+    if (p.B * rows > 0x7fffffffll || total > 0x7fffffffll) return LEANKV_ELIMIT;
+    const Plan plan = make_plan(rooms[dev], p.B * rows, longest, p.lists == nullptr ? total : p.B * longest * rows);
+    if (plan.clusters * plan.ctas > 0x7fffffffll) return LEANKV_ELIMIT;
     AttnParams q = p;
-    q.part_pages = longest <= part_pages ? 0 : (int)part_pages;
-    const long long units = q.part_pages == 0 ? triples : total / part_pages + triples;
-    if (units * ctas > 0x7fffffffll) return LEANKV_ELIMIT;
-    if (ctas == 1)
-        LEANKV_CUDA_TRY(launch_early(attn_kernel<T, D, kTiles>, dim3((unsigned)units), dim3(kThreads), smem, st, q));
-    else
-        LEANKV_CUDA_TRY(launch_cluster_kernel_ex(true, dim3(ctas), attn_kernel<T, D, kTiles>, dim3((unsigned)(units * ctas)), dim3(kThreads), smem, st, q));
+    q.part_pages = plan.part_pages;
+    const dim3 grid((unsigned)(plan.clusters * plan.ctas));
+    if (plan.ctas == 1) LEANKV_CUDA_TRY(launch_early(attn_kernel<T, D, kTiles>, grid, dim3(kThreads), smem, st, q));
+    else LEANKV_CUDA_TRY(launch_cluster_kernel_ex(true, dim3(plan.ctas), attn_kernel<T, D, kTiles>, grid, dim3(kThreads), smem, st, q));
     return LEANKV_OK;
 }
 

@@ -6,10 +6,12 @@
 // whole number: dp2a takes two 16-bit by 8-bit products at a time, sums are exact, and the choice does not depend on any order.
 // A record is 2 * dim + 16 bytes against 32 * dim + 16 of the block: the scores read 1/16 of the cache.
 //
-// score_kernel: a lane has 16 bytes of a record and its 16 numbers of P or N in registers; dim / 8 lanes share a record.
-// select_kernel: a CTA has a (sequence, kv head); a thread's scores stay in registers as whole numbers in the scores' order, and the border is found from the
-// top two bits at a time by counting (three counts a step, one barrier), which knows no worst case: a histogram's atomics meet in one bin, since scores
-// share their upper bits. Counting stops when the count is what is wanted. Positions come from one scan.
+// score_kernel: a CTA asks for the records of its blocks first and forms P and N while they come; a lane has 16 bytes of a record and its 16 numbers of P
+// or N in registers, dim / 8 lanes share a record.
+// select_kernel: a CTA has a (sequence, kv head); scores are whole numbers in the scores' order, kept in registers. The border is found in the range between the
+// smallest and the largest: 2048 bins, the one that holds the border becomes the next range (scores share their upper bits: bins of the number itself would all
+// be hit in one place; counting against three borders a step, 16 steps of a barrier each, took 23 us for 8193 blocks). Mostly two rounds. Positions come from ballots and
+// one scan, so that the list ascends.
 
 #include <algorithm>
 
@@ -19,9 +21,10 @@ namespace leankv {
 namespace bytes {
 namespace {
 
-constexpr int kScoreThreads = 128;
+constexpr int kScoreThreads = 128, kScoreWarps = kScoreThreads / 32;
 constexpr int kScoreBlocks = 64;                   // of a CTA
 constexpr int kPer = 16;                           // scores that a thread keeps in registers
+constexpr int kBins = 2048;
 
 struct SelectParams {
     const uint8_t* bounds;
@@ -37,64 +40,86 @@ struct SelectParams {
 template <typename T, int D>
 __global__ void __launch_bounds__(kScoreThreads) score_kernel(const SelectParams p) {
     constexpr int kLanes = D / 8;                  // of a record
-    __shared__ uint32_t s_amax[kScoreThreads / 32];
+    constexpr int kAtOnce = 32 / kLanes, kOfWarp = kScoreBlocks / kScoreWarps, kLoads = kOfWarp / kAtOnce;
+    constexpr int kHeads = LEANKV_BYTES_MAX_GROUP * (D / 8) / kScoreThreads;      // eights of the group's queries that a thread has at most
+    __shared__ uint32_t s_amax[kScoreWarps];
+    __shared__ __align__(16) short s_int[LEANKV_BYTES_MAX_GROUP][D];
     __shared__ __align__(16) short s_pn[2 * D];
     pdl_begin();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int h = blockIdx.y, b = blockIdx.z;
-    const int ip = p.indptr[b], pages = min(p.indptr[b + 1] - ip, p.max_pages), first = blockIdx.x * kScoreBlocks;
-    if (pages <= p.n_blocks || first >= pages) return;
+    const int ip = p.indptr[b], pages = min(p.indptr[b + 1] - ip, p.max_pages), first = blockIdx.x * kScoreBlocks + warp * kOfWarp;
+    if (pages <= p.n_blocks || (int)blockIdx.x * kScoreBlocks >= pages) return;
+
+    // ---- queries and records are asked for ----
     const T* q = static_cast<const T*>(p.q.data) + b * p.q.seq + (long long)h * p.G * p.q.head;
-    uint32_t amax = 0;
-    for (int i = tid; i < p.G * (D / 8); i += kScoreThreads) {
-        Eight<T> x;
-        x.load(q + (i / (D / 8)) * p.q.head + i % (D / 8) * 8);
+    const int eights = p.G * (D / 8);
+    Eight<T> x[kHeads];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(x.get(e)) & 0x7fffffffu);
+    for (int i = 0; i < kHeads; ++i) {
+        const int at = tid + i * kScoreThreads;
+        if (at < eights) x[i].load(q + (at / (D / 8)) * p.q.head + at % (D / 8) * 8);
+        else x[i].zero();
     }
+    int id = -1;                                   // of block first + lane
+    if (lane < kOfWarp && first + lane < pages) id = p.indices[ip + first + lane];
+    if ((unsigned)id >= (unsigned)p.n_pages) id = -1;
+    const int part = lane % kLanes, sub = lane / kLanes;
+    uint4 c[kLoads];
+    float scale[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const int mine = __shfl_sync(0xffffffffu, id, i * kAtOnce + sub);
+        const uint8_t* rec = p.bounds + ((size_t)max(mine, 0) * p.H + h) * bounds_bytes(D);
+        c[i] = __ldg(reinterpret_cast<const uint4*>(rec) + part);
+        scale[i] = part != 0 ? 0.f : mine < 0 ? -INFINITY : __ldg(reinterpret_cast<const float*>(rec + 2 * D));
+    }
+
+    // ---- P and N ----
+    uint32_t amax = 0;
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(x[i].get(e)) & 0x7fffffffu);
     amax = __reduce_max_sync(0xffffffffu, amax);
     if (lane == 0) s_amax[warp] = amax;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kScoreThreads / 32; ++w) amax = max(amax, s_amax[w]);
+    for (int w = 0; w < kScoreWarps; ++w) amax = max(amax, s_amax[w]);
     const bool finite = amax < 0x7f800000u;        // else every score is 0
     const float down = power_of_two(-least_exponent<2047>(min(amax, 0x7f7fffffu)));
-    if (tid < D / 8) {
-        int up[8], low[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) up[e] = low[e] = 0;
-        for (int g = 0; g < p.G; ++g) {
-            Eight<T> x;
-            x.load(q + g * p.q.head + 8 * tid);
+    for (int i = 0; i < kHeads; ++i) {
+        const int at = tid + i * kScoreThreads;
+        if (at >= eights) continue;
+        uint32_t w[4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int i = finite ? __float2int_rn(x.get(e) * down) : 0;
-                up[e] += max(i, 0);
-                low[e] += min(i, 0);
-            }
+        for (int e = 0; e < 4; ++e) {
+            const int lo = finite ? __float2int_rn(x[i].get(2 * e) * down) : 0, hi = finite ? __float2int_rn(x[i].get(2 * e + 1) * down) : 0;
+            w[e] = ((uint32_t)lo & 0xffffu) | ((uint32_t)hi << 16);
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            s_pn[8 * tid + e] = (short)up[e];
-            s_pn[D + 8 * tid + e] = (short)low[e];
-        }
+        *reinterpret_cast<uint4*>(&s_int[at / (D / 8)][at % (D / 8) * 8]) = make_uint4(w[0], w[1], w[2], w[3]);
     }
     __syncthreads();
-    const int part = lane % kLanes, sub = lane / kLanes;
+    if (tid < D) {
+        int up = 0, low = 0;
+        for (int g = 0; g < p.G; ++g) {
+            const int i = s_int[g][tid];
+            up += max(i, 0);
+            low += min(i, 0);
+        }
+        s_pn[tid] = (short)up;
+        s_pn[D + tid] = (short)low;
+    }
+    __syncthreads();
     int pn[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) pn[e] = reinterpret_cast<const int*>(s_pn)[8 * part + e];
-    constexpr int kAtOnce = 32 / kLanes;
+
     float* out = p.scores + ((long long)b * p.H + h) * p.max_pages;
-#pragma unroll 4
-    for (int i = 0; i < kScoreBlocks / (kScoreThreads / 32 * kAtOnce); ++i) {
-        const int j = first + (i * (kScoreThreads / 32) + warp) * kAtOnce + sub;
-        const int id = j < pages ? p.indices[ip + j] : -1;
-        const bool there = (unsigned)id < (unsigned)p.n_pages;
-        const uint8_t* rec = p.bounds + ((size_t)(there ? id : 0) * p.H + h) * bounds_bytes(D);
-        const uint4 c = __ldg(reinterpret_cast<const uint4*>(rec) + part);
-        const float scale = __ldg(reinterpret_cast<const float*>(rec + 2 * D));
-        const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
         int u = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -103,7 +128,8 @@ __global__ void __launch_bounds__(kScoreThreads) score_kernel(const SelectParams
         }
 #pragma unroll
         for (int o = 1; o < kLanes; o *= 2) u += __shfl_xor_sync(0xffffffffu, u, o);
-        if (part == 0 && j < pages) out[j] = there ? __int2float_rn(u) * scale : -INFINITY;
+        const int j = first + i * kAtOnce + sub;
+        if (part == 0 && j < pages) out[j] = scale[i] == -INFINITY ? -INFINITY : __int2float_rn(u) * scale[i];
     }
 }
 
@@ -115,9 +141,12 @@ __device__ __forceinline__ uint32_t ordered(float v) {
 
 template <int kThreads>
 __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) {
-    constexpr int kWarps = kThreads / 32;
-    __shared__ int s_count[2][3][kWarps];
-    __shared__ long long s_scan[kWarps];
+    constexpr int kWarps = kThreads / 32, kSlab = kPer * kThreads, kOwn = kBins / kThreads;      // kOwn: bins of a thread
+    __shared__ uint32_t s_low[kWarps], s_high[kWarps];
+    __shared__ int s_bin[kBins];
+    __shared__ int s_part[kWarps];
+    __shared__ int s_at, s_above, s_in;
+    __shared__ uint32_t s_rank[kPer * kWarps];     // chosen in any case | at the border << 16, of a warp's 32 scores; then those before them
     pdl_begin();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int h = blockIdx.x, b = blockIdx.y;
@@ -132,78 +161,132 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) 
         }
         return;
     }
-    // thread: blocks per * tid .. ; the first kPer in registers (all of them for up to kPer * kThreads blocks). Blocks that are taken or left in any case have the
-    // largest and smallest key
     const float* scores = p.scores + pair * p.max_pages;
-    const int per = (pages + kThreads - 1) / kThreads, base = tid * per;
-    auto key_at = [&](int i) -> uint32_t {         // 0: not there
-        const int j = base + i;
-        if (i >= per || j >= pages) return 0u;
-        if (j < p.sinks || j >= pages - p.recent) return 0xffffffffu;
-        return min(max(ordered(scores[j]), 1u), 0xfffffffeu);
-    };
+    const int first = p.sinks, last = pages - p.recent;                          // blocks that a score decides on: first .. last - 1
+    const int slabs = (pages + kSlab - 1) / kSlab;
     uint32_t key[kPer];
+    auto load = [&](int slab) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) key[i] = key_at(i);
-    auto over_all = [&](auto&& f) {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) f(i, key[i]);
-        for (int i = kPer; i < per; ++i) f(i, key_at(i));
+        for (int i = 0; i < kPer; ++i) {
+            const int j = slab * kSlab + i * kThreads + tid;
+            key[i] = j >= first && j < last ? ordered(scores[j]) : 0u;
+        }
     };
-    // the largest border with at least n_blocks keys at or above it
-    uint32_t border = 0;
-    int step = 0, at_border = pages;
-    for (int shift = 30; shift >= 0 && at_border != p.n_blocks; shift -= 2, step ^= 1) {
-        int n[3] = {0, 0, 0};
-        over_all([&](int, uint32_t k) {
+    auto decided = [&](int slab, int i) {
+        const int j = slab * kSlab + i * kThreads + tid;
+        return j >= first && j < last;
+    };
+
+    // ---- the range of the scores ----
+    uint32_t low = 0xffffffffu, high = 0u;
+    for (int slab = 0; slab < slabs; ++slab) {
+        load(slab);
 #pragma unroll
-            for (uint32_t x = 0; x < 3; ++x) n[x] += k >= border + ((x + 1) << shift) ? 1 : 0;
-        });
+        for (int i = 0; i < kPer; ++i)
+            if (decided(slab, i)) low = min(low, key[i]), high = max(high, key[i]);
+    }
+    low = __reduce_min_sync(0xffffffffu, low);
+    high = __reduce_max_sync(0xffffffffu, high);
+    if (lane == 0) s_low[warp] = low, s_high[warp] = high;
+    __syncthreads();
+    low = __reduce_min_sync(0xffffffffu, s_low[lane % kWarps]);
+    high = __reduce_max_sync(0xffffffffu, s_high[lane % kWarps]);
+
+    // ---- the border: all keys above it are chosen, and the first `room` of those that are it ----
+    int room = p.n_blocks - p.sinks - p.recent;    // of those in low .. high
+    uint32_t border = high;
+    if (room > 0) {
+        for (;;) {
+            const int bits = 32 - __clz((int)(high - low)), shift = bits > 11 ? bits - 11 : 0;
+            for (int i = tid; i < kBins; i += kThreads) s_bin[i] = 0;
+            __syncthreads();
+            for (int slab = 0; slab < slabs; ++slab) {
+                if (slabs > 1) load(slab);
 #pragma unroll
-        for (int x = 0; x < 3; ++x) {
-            const int sum = __reduce_add_sync(0xffffffffu, n[x]);
-            if (lane == 0) s_count[step][x][warp] = sum;
+                for (int i = 0; i < kPer; ++i)
+                    if (decided(slab, i) && key[i] >= low && key[i] <= high) atomicAdd(&s_bin[(key[i] - low) >> shift], 1);
+            }
+            __syncthreads();
+            int own[kOwn], sum = 0;                // thread: bins from the top down
+#pragma unroll
+            for (int i = 0; i < kOwn; ++i) {
+                own[i] = s_bin[kBins - 1 - (tid * kOwn + i)];
+                sum += own[i];
+            }
+            int incl = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const int add = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += add;
+            }
+            if (lane == 31) s_part[warp] = incl;
+            __syncthreads();
+            int above = incl - sum;
+            for (int w = 0; w < warp; ++w) above += s_part[w];
+#pragma unroll
+            for (int i = 0; i < kOwn; ++i) {
+                if (above < room && above + own[i] >= room) s_at = kBins - 1 - (tid * kOwn + i), s_above = above, s_in = own[i];
+                above += own[i];
+            }
+            __syncthreads();
+            room -= s_above;
+            low += (uint32_t)s_at << shift;
+            if (shift == 0 || s_in == room) break;
+            high = low + ((1u << shift) - 1u);
+        }
+        border = low;
+        // a bin that is chosen whole: everything from its lower end on
+        if (s_in == room) border = low - 1u, room = 0;
+    }
+
+    // ---- positions ----
+    int base = 0, base_at = 0;                     // chosen in any case, and at the border, in earlier slabs
+    for (int slab = 0; slab < slabs; ++slab) {
+        if (slabs > 1) load(slab);
+        uint32_t in[kPer], at[kPer];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int j = slab * kSlab + i * kThreads + tid;
+            const bool score = decided(slab, i);
+            in[i] = __ballot_sync(0xffffffffu, j < pages && (!score || (p.n_blocks > p.sinks + p.recent && key[i] > border)));
+            at[i] = __ballot_sync(0xffffffffu, score && room > 0 && key[i] == border);
+            if (lane == 0) s_rank[i * kWarps + warp] = (uint32_t)__popc(in[i]) | (uint32_t)__popc(at[i]) << 16;
         }
         __syncthreads();
-        uint32_t take = 0;
+        // kPer * kWarps sums: two of a thread at most; counts of a slab stay below 2^16
+        constexpr int kSums = kPer * kWarps;
+        static_assert(kSums <= kThreads, "one sum of a thread");
+        uint32_t mine = tid < kSums ? s_rank[tid] : 0u, incl = mine;
 #pragma unroll
-        for (int x = 0; x < 3; ++x) {
-            int all = lane < kWarps ? s_count[step][x][lane] : 0;
-            all = __reduce_add_sync(0xffffffffu, all);
-            if (all >= p.n_blocks) {
-                take = x + 1;
-                at_border = all;
-            }
+        for (int o = 1; o < 32; o *= 2) {
+            const uint32_t add = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += add;
         }
-        border += take << shift;
-    }
-    // all keys above the border, and the first of those at it
-    long long mine = 0;                            // above: low half, at: high half
-    over_all([&](int, uint32_t k) { mine += k > border ? 1ll : k == border && k != 0u ? 1ll << 32 : 0ll; });
-    long long incl = mine;
+        if (lane == 31) s_part[warp] = (int)incl;
+        __syncthreads();
+        uint32_t before = incl - mine, all = 0;
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) before += (uint32_t)s_part[w];
+            all += (uint32_t)s_part[w];
+        }
+        if (tid < kSums) s_rank[tid] = before;
+        __syncthreads();
+        const uint32_t lanes = (1u << lane) - 1u;
 #pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-        const long long add = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += add;
-    }
-    if (lane == 31) s_scan[warp] = incl;
-    __syncthreads();
-    long long before = incl - mine, all = 0;
-    for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += s_scan[w];
-        all += s_scan[w];
-    }
-    const int room = p.n_blocks - (int)(all & 0xffffffffll);      // of those at the border
-    int above = (int)(before & 0xffffffffll), at = (int)(before >> 32);
-    over_all([&](int i, uint32_t k) {
-        if (k > border || (k == border && k != 0u && at < room)) {
-            const int to = above + min(at, room);
-            blocks[to] = base + i;
-            block_pages[to] = p.indices[ip + base + i];
+        for (int i = 0; i < kPer; ++i) {
+            const bool is_in = in[i] >> lane & 1u, is_at = at[i] >> lane & 1u;
+            if (!is_in && !is_at) continue;
+            const uint32_t r = s_rank[i * kWarps + warp];
+            const int n_in = base + (int)(r & 0xffffu) + __popc(in[i] & lanes), n_at = base_at + (int)(r >> 16) + __popc(at[i] & lanes);
+            if (!is_in && n_at >= room) continue;
+            const int j = slab * kSlab + i * kThreads + tid, to = n_in + min(n_at, room);
+            blocks[to] = j;
+            block_pages[to] = p.indices[ip + j];
         }
-        above += k > border ? 1 : 0;
-        at += k == border && k != 0u ? 1 : 0;
-    });
+        base += (int)(all & 0xffffu);
+        base_at += (int)(all >> 16);
+    }
 }
 
 template <typename T, int D>
