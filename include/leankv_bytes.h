@@ -47,38 +47,52 @@ typedef struct {
 size_t leankv_byte_chunk_bytes(int dim);
 size_t leankv_byte_bounds_bytes(int dim);
 
-/* T new tokens of B sequences (k, v of `dtype`) become the last T tokens of each: the page table has been advanced already
+/* `tokens` new tokens of `batch` sequences (k, v of `dtype`) become the last ones of each: the page table has been advanced already
  * (leankv_paged_table_step). Sequence b owns the pages kv_page_indices[kv_indptr[b]] .. ; a page id outside 0 .. n_pages - 1 is
- * not written, nor is a sequence of fewer than T tokens. B <= LEANKV_BYTES_MAX_BATCH. */
-int leankv_byte_append(const leankv_byte_pool_t* pool /* host */, int dtype, const leankv_vectors_t* k /* host */,
-                       const leankv_vectors_t* v /* host */, int B, int T, const int32_t* kv_indptr,
-                       const int32_t* kv_page_indices, const int32_t* kv_last_page_len, void* stream);
+ * not written, nor is a sequence of fewer tokens. batch <= LEANKV_BYTES_MAX_BATCH. */
+typedef struct {
+    leankv_byte_pool_t pool;
+    int dtype, batch, tokens;
+    leankv_vectors_t k, v;
+    const int32_t* kv_indptr;
+    const int32_t* kv_page_indices;
+    const int32_t* kv_last_page_len;
+} leankv_byte_append_t;
+int leankv_byte_append(const leankv_byte_append_t* a /* host */, void* stream);
 
 /* The stored numbers of the first T positions of B sequences, as `dtype`: k_out, v_out [B][kv_heads][T][dim], zeros behind a sequence's
  * last token. A number beyond the type's range becomes its largest one. */
 int leankv_byte_unpack(const leankv_byte_pool_t* pool /* host */, int dtype, void* k_out, void* v_out, int B, int T,
                        const int32_t* kv_indptr, const int32_t* kv_page_indices, const int32_t* kv_last_page_len, void* stream);
 
-/* Attention of the last `tokens` tokens of each of B sequences over the cache, causal among themselves: q_heads / kv_heads (up to
+/* Attention of the last `tokens` tokens of each of `batch` sequences over the cache, causal among themselves: q_heads / kv_heads (up to
  * LEANKV_BYTES_MAX_GROUP) query heads share a kv head; q and out of `dtype`. Softmax statistics and sums are fp32. A sequence
  * without tokens, and a query before the first token, gets zeros.
  * max_pages_seq, total_pages: upper bounds of any sequence's pages and of all sequences' together, for the launch's shape.
- * blocks = NULL: every page. Else (tokens = 1) the pages of sequence b and kv head h are block_pages[(b * kv_heads + h) * n_blocks ..], as
+ * block_pages = NULL: every page. Else (tokens = 1) the pages of sequence b and kv head h are block_pages[(b * kv_heads + h) * n_blocks ..], as
  * many as there are blocks or n_blocks, the last of them the sequence's last page (leankv_byte_select writes such lists).
  * The workspace is zero-filled once; its first word is a status (0 = clean; leankv_byte_status): bit 0 a bounded wait ran out, bit 1 a page
  * id outside the pool, bit 2 more pages than total_pages (nothing was written). The launches of two streams need a workspace each. */
+typedef struct {
+    leankv_byte_pool_t pool;
+    int dtype, batch, q_heads, tokens;
+    leankv_vectors_t q, out;
+    float scale;
+    const int32_t* kv_indptr;
+    const int32_t* kv_page_indices;
+    const int32_t* kv_last_page_len;
+    int max_pages_seq;
+    long long total_pages;
+    const int32_t* block_pages;
+    int n_blocks;
+    void* workspace;
+    size_t workspace_bytes;
+} leankv_byte_attn_t;
 size_t leankv_byte_attn_workspace_bytes(void);       /* the same for all shapes */
-int leankv_byte_attn(const leankv_byte_pool_t* pool /* host */, int dtype, const leankv_vectors_t* q /* host */,
-                     const leankv_vectors_t* out /* host */, int B, int q_heads, int tokens, float scale, const int32_t* kv_indptr,
-                     const int32_t* kv_page_indices, const int32_t* kv_last_page_len, int max_pages_seq, long long total_pages,
-                     const int32_t* block_pages, int n_blocks, void* workspace, size_t workspace_bytes, void* stream);
-
+int leankv_byte_attn(const leankv_byte_attn_t* a /* host */, void* stream);
 /* The same for longer chunks of prompts, on tcgen05 (256 (token, head) rows against 128 keys at a time); q and out fp16 or bf16 (fp32:
- * LEANKV_EUNSUPPORTED), scale > 0. Weights enter the value product as fp16. The workspace is the one above. */
-int leankv_byte_prompt_attn(const leankv_byte_pool_t* pool /* host */, int dtype, const leankv_vectors_t* q /* host */,
-                            const leankv_vectors_t* out /* host */, int B, int q_heads, int tokens, float scale,
-                            const int32_t* kv_indptr, const int32_t* kv_page_indices, const int32_t* kv_last_page_len,
-                            int max_pages_seq, void* workspace, size_t workspace_bytes, void* stream);
+ * LEANKV_EUNSUPPORTED), scale > 0, block_pages NULL. Weights enter the value product as fp16. */
+int leankv_byte_prompt_attn(const leankv_byte_attn_t* a /* host */, void* stream);
 
 /* The blocks that one query token of each sequence reads, for each kv head: all of them where there are no more than n_blocks; else the
  * first `sinks`, the last `recent` (>= 1; sinks + recent <= n_blocks) and those with the largest score, ties to the lower block.
@@ -86,11 +100,20 @@ int leankv_byte_prompt_attn(const leankv_byte_pool_t* pool /* host */, int dtype
  *   u = sum over d of  max[d] * sum_g max(i, 0) + min[d] * sum_g min(i, 0)       (whole numbers below 2^31)
  *   score = fp32(u) * 2^e
  * an upper bound of the heads' summed scores over the block's tokens, up to the rounding of q. The score of a block whose scale is
- * NaN is larger than all others. Block numbers ascending, then -1: blocks [B][kv_heads][n_blocks]; the page of each in block_pages
- * (0 behind the last). scores: scratch of B * kv_heads * max_pages_seq fp32 words. */
-int leankv_byte_select(const leankv_byte_pool_t* pool /* host */, int dtype, const leankv_vectors_t* q /* host */, int B, int q_heads,
-                       const int32_t* kv_indptr, const int32_t* kv_page_indices, int max_pages_seq, int n_blocks, int sinks, int recent,
-                       int32_t* blocks, int32_t* block_pages, float* scores, void* stream);
+ * NaN is larger than all others. Block numbers ascending, then -1: blocks [batch][kv_heads][n_blocks]; the page of each in block_pages
+ * (0 behind the last). scores: scratch of batch * kv_heads * max_pages_seq fp32 words. */
+typedef struct {
+    leankv_byte_pool_t pool;
+    int dtype, batch, q_heads;
+    leankv_vectors_t q;
+    const int32_t* kv_indptr;
+    const int32_t* kv_page_indices;
+    int max_pages_seq, n_blocks, sinks, recent;
+    int32_t* blocks;
+    int32_t* block_pages;
+    float* scores;
+} leankv_byte_select_t;
+int leankv_byte_select(const leankv_byte_select_t* a /* host */, void* stream);
 
 /* Host copy of a workspace's status word (synchronises). */
 int leankv_byte_status(const void* workspace, int* status /* host */);

@@ -292,20 +292,42 @@ class Vectors(Structure):
     _fields_ = [("data", c_void_p), ("seq", c_longlong), ("head", c_longlong), ("token", c_longlong)]
 
 
+class ByteAppend(Structure):
+    """Mirror of ``leankv_byte_append_t``."""
+
+    _fields_ = [("pool", BytePool), ("dtype", c_int), ("batch", c_int), ("tokens", c_int), ("k", Vectors), ("v", Vectors),
+                ("kv_indptr", c_void_p), ("kv_page_indices", c_void_p), ("kv_last_page_len", c_void_p)]
+
+
+class ByteAttn(Structure):
+    """Mirror of ``leankv_byte_attn_t``."""
+
+    _fields_ = [("pool", BytePool), ("dtype", c_int), ("batch", c_int), ("q_heads", c_int), ("tokens", c_int),
+                ("q", Vectors), ("out", Vectors), ("scale", c_float),
+                ("kv_indptr", c_void_p), ("kv_page_indices", c_void_p), ("kv_last_page_len", c_void_p),
+                ("max_pages_seq", c_int), ("total_pages", c_longlong), ("block_pages", c_void_p), ("n_blocks", c_int),
+                ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
+
+
+class ByteSelect(Structure):
+    """Mirror of ``leankv_byte_select_t``."""
+
+    _fields_ = [("pool", BytePool), ("dtype", c_int), ("batch", c_int), ("q_heads", c_int), ("q", Vectors),
+                ("kv_indptr", c_void_p), ("kv_page_indices", c_void_p),
+                ("max_pages_seq", c_int), ("n_blocks", c_int), ("sinks", c_int), ("recent", c_int),
+                ("blocks", c_void_p), ("block_pages", c_void_p), ("scores", c_void_p)]
+
+
 BYTE_SIGNATURES = {
     "leankv_byte_chunk_bytes": (c_size_t, [c_int]),
     "leankv_byte_bounds_bytes": (c_size_t, [c_int]),
-    "leankv_byte_append": (c_int, [POINTER(BytePool), c_int, POINTER(Vectors), POINTER(Vectors), c_int, c_int, c_void_p, c_void_p,
-                                   c_void_p, c_void_p]),
+    "leankv_byte_append": (c_int, [POINTER(ByteAppend), c_void_p]),
     "leankv_byte_unpack": (c_int, [POINTER(BytePool), c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p,
                                    c_void_p]),
     "leankv_byte_attn_workspace_bytes": (c_size_t, []),
-    "leankv_byte_attn": (c_int, [POINTER(BytePool), c_int, POINTER(Vectors), POINTER(Vectors), c_int, c_int, c_int, c_float, c_void_p,
-                                 c_void_p, c_void_p, c_int, c_longlong, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
-    "leankv_byte_prompt_attn": (c_int, [POINTER(BytePool), c_int, POINTER(Vectors), POINTER(Vectors), c_int, c_int, c_int, c_float,
-                                        c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
-    "leankv_byte_select": (c_int, [POINTER(BytePool), c_int, POINTER(Vectors), c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
-                                   c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "leankv_byte_attn": (c_int, [POINTER(ByteAttn), c_void_p]),
+    "leankv_byte_prompt_attn": (c_int, [POINTER(ByteAttn), c_void_p]),
+    "leankv_byte_select": (c_int, [POINTER(ByteSelect), c_void_p]),
     "leankv_byte_status": (c_int, [c_void_p, POINTER(c_int)]),
 }
 _COMMON = ("leankv_strerror", "leankv_last_cuda_error", "leankv_abi_version")     # capi.cu, in every library

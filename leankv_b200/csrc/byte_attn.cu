@@ -662,37 +662,26 @@ using namespace leankv;
 
 extern "C" size_t leankv_byte_attn_workspace_bytes(void) { return bytes::kWorkspaceBytes; }
 
-extern "C" int leankv_byte_attn(const leankv_byte_pool_t* pool, int dtype, const leankv_vectors_t* q, const leankv_vectors_t* out, int B,
-                                int q_heads, int tokens, float scale, const int32_t* kv_indptr, const int32_t* kv_page_indices,
-                                const int32_t* kv_last_page_len, int max_pages_seq, long long total_pages, const int32_t* block_pages, int n_blocks,
-                                void* workspace, size_t workspace_bytes, void* stream) {
-    if (!bytes::good_pool(pool) || !bytes::good_type(dtype) || !q || !out || !q->data || !out->data || B <= 0 || tokens <= 0 || q_heads <= 0 ||
-        q_heads % pool->kv_heads != 0 || !kv_indptr || !kv_page_indices || !kv_last_page_len || max_pages_seq < 0 ||
-        total_pages < 0 || (block_pages != nullptr && (tokens != 1 || n_blocks <= 0)))
-        return LEANKV_EINVAL;
-    if (B > LEANKV_BYTES_MAX_BATCH || q_heads / pool->kv_heads > LEANKV_BYTES_MAX_GROUP) return LEANKV_ELIMIT;
-    if (!bytes::aligned_pool(pool) || !bytes::aligned_vectors(q, dtype, B, q_heads, tokens) ||
-        !bytes::aligned_vectors(out, dtype, B, q_heads, tokens) || !aligned16(workspace))
-        return LEANKV_EALIGN;
-    if (!workspace || workspace_bytes < bytes::kWorkspaceBytes) return LEANKV_EWORKSPACE;
+extern "C" int leankv_byte_attn(const leankv_byte_attn_t* a, void* stream) {
+    if (const int rc = bytes::check_attn(a, bytes::kWorkspaceBytes)) return rc;
     bytes::AttnParams p = {};
-    p.chunks = static_cast<const uint8_t*>(pool->chunks);
-    p.n_pages = pool->n_pages, p.H = pool->kv_heads, p.B = B, p.G = q_heads / pool->kv_heads, p.tokens = tokens;
-    const long long rows_all = (long long)tokens * p.G;
+    p.chunks = static_cast<const uint8_t*>(a->pool.chunks);
+    p.n_pages = a->pool.n_pages, p.H = a->pool.kv_heads, p.B = a->batch, p.G = a->q_heads / a->pool.kv_heads, p.tokens = a->tokens;
+    const long long rows_all = (long long)a->tokens * p.G;
     if (rows_all > (1ll << 24)) return LEANKV_ELIMIT;
     const int rows = rows_all <= 8 ? 8 : 16;
     p.row_tiles = (int)((rows_all + rows - 1) / rows);
-    p.q = *q, p.out = *out;
-    p.scale = scale * bytes::kLog2e;
-    p.indptr = kv_indptr, p.indices = kv_page_indices, p.last = kv_last_page_len;
-    p.lists = block_pages, p.n_lists = n_blocks;
-    p.status = static_cast<int*>(workspace);
+    p.q = a->q, p.out = a->out;
+    p.scale = a->scale * bytes::kLog2e;
+    p.indptr = a->kv_indptr, p.indices = a->kv_page_indices, p.last = a->kv_last_page_len;
+    p.lists = a->block_pages, p.n_lists = a->n_blocks;
+    p.status = static_cast<int*>(a->workspace);
     p.counters = reinterpret_cast<unsigned*>(p.status + bytes::kStatusWords);
-    p.partials = reinterpret_cast<float*>(p.counters + bytes::kCounters);
+    p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + bytes::kPartialsAt);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return dtype == LEANKV_BYTES_F16 ? bytes::launch<__half>(p, pool->dim, rows, max_pages_seq, total_pages, st)
-         : dtype == LEANKV_BYTES_BF16 ? bytes::launch<bf16>(p, pool->dim, rows, max_pages_seq, total_pages, st)
-                                      : bytes::launch<float>(p, pool->dim, rows, max_pages_seq, total_pages, st);
+    return a->dtype == LEANKV_BYTES_F16 ? bytes::launch<__half>(p, a->pool.dim, rows, a->max_pages_seq, a->total_pages, st)
+         : a->dtype == LEANKV_BYTES_BF16 ? bytes::launch<bf16>(p, a->pool.dim, rows, a->max_pages_seq, a->total_pages, st)
+                                         : bytes::launch<float>(p, a->pool.dim, rows, a->max_pages_seq, a->total_pages, st);
 }
 
 extern "C" int leankv_byte_status(const void* workspace, int* status) {

@@ -234,24 +234,25 @@ using namespace leankv;
 extern "C" size_t leankv_byte_chunk_bytes(int dim) { return dim == 64 || dim == 128 ? bytes::chunk_bytes(dim) : 0; }
 extern "C" size_t leankv_byte_bounds_bytes(int dim) { return dim == 64 || dim == 128 ? bytes::bounds_bytes(dim) : 0; }
 
-extern "C" int leankv_byte_append(const leankv_byte_pool_t* pool, int dtype, const leankv_vectors_t* k, const leankv_vectors_t* v, int B, int T,
-                                  const int32_t* kv_indptr, const int32_t* kv_page_indices, const int32_t* kv_last_page_len, void* stream) {
-    if (!bytes::good_pool(pool) || !bytes::good_type(dtype) || !k || !v || !k->data || !v->data || B <= 0 || T <= 0 || !kv_indptr ||
-        !kv_page_indices || !kv_last_page_len)
+extern "C" int leankv_byte_append(const leankv_byte_append_t* a, void* stream) {
+    if (!a || !bytes::good_pool(&a->pool) || !bytes::good_type(a->dtype) || !a->k.data || !a->v.data || a->batch <= 0 || a->tokens <= 0 ||
+        !a->kv_indptr || !a->kv_page_indices || !a->kv_last_page_len)
         return LEANKV_EINVAL;
-    if (B > LEANKV_BYTES_MAX_BATCH) return LEANKV_ELIMIT;
-    if (!bytes::aligned_pool(pool) || !bytes::aligned_vectors(k, dtype, B, pool->kv_heads, T) || !bytes::aligned_vectors(v, dtype, B, pool->kv_heads, T))
+    if (a->batch > LEANKV_BYTES_MAX_BATCH) return LEANKV_ELIMIT;
+    const leankv_byte_pool_t& pool = a->pool;
+    if (!bytes::aligned_pool(&pool) || !bytes::aligned_vectors(&a->k, a->dtype, a->batch, pool.kv_heads, a->tokens) ||
+        !bytes::aligned_vectors(&a->v, a->dtype, a->batch, pool.kv_heads, a->tokens))
         return LEANKV_EALIGN;
     bytes::AppendParams p = {};
-    p.chunks = static_cast<uint8_t*>(pool->chunks);
-    p.bounds = static_cast<uint8_t*>(pool->bounds);
-    p.H = pool->kv_heads, p.n_pages = pool->n_pages, p.B = B, p.T = T;
-    p.tiles = (int)(((long long)T + 2 * bytes::kPage - 2) / bytes::kPage);
-    p.k = *k, p.v = *v;
-    p.indptr = kv_indptr, p.indices = kv_page_indices, p.last = kv_last_page_len;
-    const long long grid = bytes::grid_of(B, p.H, p.tiles);
+    p.chunks = static_cast<uint8_t*>(pool.chunks);
+    p.bounds = static_cast<uint8_t*>(pool.bounds);
+    p.H = pool.kv_heads, p.n_pages = pool.n_pages, p.B = a->batch, p.T = a->tokens;
+    p.tiles = (int)(((long long)a->tokens + 2 * bytes::kPage - 2) / bytes::kPage);
+    p.k = a->k, p.v = a->v;
+    p.indptr = a->kv_indptr, p.indices = a->kv_page_indices, p.last = a->kv_last_page_len;
+    const long long grid = bytes::grid_of(p.B, p.H, p.tiles);
     if (grid == 0) return LEANKV_ELIMIT;
-    return bytes::by_type(dtype, pool->dim, [&](auto t, auto d) -> int {
+    return bytes::by_type(a->dtype, pool.dim, [&](auto t, auto d) -> int {
         LEANKV_CUDA_TRY(launch_early(bytes::append_kernel<decltype(t), decltype(d)::value>, dim3((unsigned)grid), dim3(bytes::kWarps * 32), 0,
                                      static_cast<cudaStream_t>(stream), p));
         return LEANKV_OK;

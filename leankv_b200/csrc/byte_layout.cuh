@@ -39,6 +39,19 @@ inline bool aligned_vectors(const leankv_vectors_t* x, int dtype, int seqs, int 
     return aligned16(x->data) && (seqs <= 1 || x->seq % piece == 0) && (heads <= 1 || x->head % piece == 0) && (tokens <= 1 || x->token % piece == 0);
 }
 
+// What both attention entries ask of their arguments.
+inline int check_attn(const leankv_byte_attn_t* a, size_t workspace_bytes) {
+    if (!a || !good_pool(&a->pool) || !good_type(a->dtype) || !a->q.data || !a->out.data || a->batch <= 0 || a->tokens <= 0 || a->q_heads <= 0 ||
+        a->q_heads % a->pool.kv_heads != 0 || !a->kv_indptr || !a->kv_page_indices || !a->kv_last_page_len || a->max_pages_seq < 0 || a->total_pages < 0 ||
+        (a->block_pages != nullptr && (a->tokens != 1 || a->n_blocks <= 0)))
+        return LEANKV_EINVAL;
+    if (a->batch > LEANKV_BYTES_MAX_BATCH || a->q_heads / a->pool.kv_heads > LEANKV_BYTES_MAX_GROUP) return LEANKV_ELIMIT;
+    if (!aligned_pool(&a->pool) || !aligned_vectors(&a->q, a->dtype, a->batch, a->q_heads, a->tokens) ||
+        !aligned_vectors(&a->out, a->dtype, a->batch, a->q_heads, a->tokens) || !aligned16(a->workspace))
+        return LEANKV_EALIGN;
+    return a->workspace && a->workspace_bytes >= workspace_bytes ? LEANKV_OK : LEANKV_EWORKSPACE;
+}
+
 // The smallest e >= -126 with amax <= 127 * 2^e (most = 127) or 2047 * 2^e (most = 2047); amax as its bits, finite.
 template <int kMost>
 __device__ __forceinline__ int least_exponent(uint32_t amax_bits) {

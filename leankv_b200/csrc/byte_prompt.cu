@@ -467,36 +467,28 @@ int launch(const PromptParams& p, int blocks, cudaStream_t st) {
 
 using namespace leankv;
 
-extern "C" int leankv_byte_prompt_attn(const leankv_byte_pool_t* pool, int dtype, const leankv_vectors_t* q, const leankv_vectors_t* out, int B,
-                                       int q_heads, int tokens, float scale, const int32_t* kv_indptr, const int32_t* kv_page_indices,
-                                       const int32_t* kv_last_page_len, int max_pages_seq, void* workspace, size_t workspace_bytes, void* stream) {
-    if (!bytes::good_pool(pool) || !bytes::good_type(dtype) || !q || !out || !q->data || !out->data || B <= 0 || tokens <= 0 || q_heads <= 0 ||
-        q_heads % pool->kv_heads != 0 || !kv_indptr || !kv_page_indices || !kv_last_page_len || max_pages_seq < 0 || !(scale > 0.f))
-        return LEANKV_EINVAL;
-    if (dtype == LEANKV_BYTES_F32) return LEANKV_EUNSUPPORTED;
-    if (B > LEANKV_BYTES_MAX_BATCH || q_heads / pool->kv_heads > LEANKV_BYTES_MAX_GROUP) return LEANKV_ELIMIT;
-    if (!bytes::aligned_pool(pool) || !bytes::aligned_vectors(q, dtype, B, q_heads, tokens) ||
-        !bytes::aligned_vectors(out, dtype, B, q_heads, tokens) || !aligned16(workspace))
-        return LEANKV_EALIGN;
-    if (!workspace || workspace_bytes < bytes::kWorkspaceBytes) return LEANKV_EWORKSPACE;
+extern "C" int leankv_byte_prompt_attn(const leankv_byte_attn_t* a, void* stream) {
+    if (const int rc = bytes::check_attn(a, bytes::kWorkspaceBytes)) return rc;
+    if (a->block_pages != nullptr || !(a->scale > 0.f)) return LEANKV_EINVAL;
+    if (a->dtype == LEANKV_BYTES_F32) return LEANKV_EUNSUPPORTED;
     bytes::PromptParams p = {};
-    p.chunks = static_cast<const uint8_t*>(pool->chunks);
-    p.n_pages = pool->n_pages, p.H = pool->kv_heads, p.B = B, p.G = q_heads / pool->kv_heads, p.tokens = tokens;
+    p.chunks = static_cast<const uint8_t*>(a->pool.chunks);
+    p.n_pages = a->pool.n_pages, p.H = a->pool.kv_heads, p.B = a->batch, p.G = a->q_heads / a->pool.kv_heads, p.tokens = a->tokens;
     p.tile_tokens = bytes::kRowsTile / p.G;
-    p.q = *q, p.out = *out;
-    p.scale = scale * bytes::kLog2e;
-    p.indptr = kv_indptr, p.indices = kv_page_indices, p.last = kv_last_page_len;
-    p.status = static_cast<int*>(workspace);
-    const long long blocks = ((long long)tokens + bytes::kTiles * p.tile_tokens - 1) / (bytes::kTiles * p.tile_tokens);
-    const long long ctas = blocks * p.H * B;
-    if (blocks > 65535 || (long long)p.H * B > 0x7fffffffll) return LEANKV_ELIMIT;
+    p.q = a->q, p.out = a->out;
+    p.scale = a->scale * bytes::kLog2e;
+    p.indptr = a->kv_indptr, p.indices = a->kv_page_indices, p.last = a->kv_last_page_len;
+    p.status = static_cast<int*>(a->workspace);
+    const long long blocks = ((long long)p.tokens + bytes::kTiles * p.tile_tokens - 1) / (bytes::kTiles * p.tile_tokens);
+    const long long ctas = blocks * p.H * p.B;
+    if (blocks > 65535 || (long long)p.H * p.B > 0x7fffffffll) return LEANKV_ELIMIT;
     // fewer CTAs than SMs share the keys, four key tiles each at least; the partial sums of so many CTAs fit the workspace
-    const long long key_tiles = ((long long)max_pages_seq + bytes::kPagesTile - 1) / bytes::kPagesTile;
+    const long long key_tiles = ((long long)a->max_pages_seq + bytes::kPagesTile - 1) / bytes::kPagesTile;
     const long long room = std::min(sm_count(), bytes::kPromptCtas) / ctas;
     p.n_splits = (int)std::max(1ll, std::min({room, key_tiles / 4, 16ll}));
-    p.ml_part = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + bytes::kPartialsAt);
+    p.ml_part = reinterpret_cast<float2*>(static_cast<uint8_t*>(a->workspace) + bytes::kPartialsAt);
     p.o_part = reinterpret_cast<float*>(p.ml_part + (size_t)bytes::kPromptCtas * bytes::kPromptRows);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (pool->dim == 128) return dtype == LEANKV_BYTES_F16 ? bytes::launch<__half, 128>(p, (int)blocks, st) : bytes::launch<bf16, 128>(p, (int)blocks, st);
-    return dtype == LEANKV_BYTES_F16 ? bytes::launch<__half, 64>(p, (int)blocks, st) : bytes::launch<bf16, 64>(p, (int)blocks, st);
+    if (a->pool.dim == 128) return a->dtype == LEANKV_BYTES_F16 ? bytes::launch<__half, 128>(p, (int)blocks, st) : bytes::launch<bf16, 128>(p, (int)blocks, st);
+    return a->dtype == LEANKV_BYTES_F16 ? bytes::launch<__half, 64>(p, (int)blocks, st) : bytes::launch<bf16, 64>(p, (int)blocks, st);
 }

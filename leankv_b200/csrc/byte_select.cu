@@ -305,24 +305,23 @@ int launch(const SelectParams& p, int B, cudaStream_t st) {
 
 using namespace leankv;
 
-extern "C" int leankv_byte_select(const leankv_byte_pool_t* pool, int dtype, const leankv_vectors_t* q, int B, int q_heads, const int32_t* kv_indptr,
-                                  const int32_t* kv_page_indices, int max_pages_seq, int n_blocks, int sinks, int recent, int32_t* blocks,
-                                  int32_t* block_pages, float* scores, void* stream) {
-    if (!bytes::good_pool(pool) || !bytes::good_type(dtype) || !q || !q->data || B <= 0 || q_heads <= 0 || q_heads % pool->kv_heads != 0 ||
-        !kv_indptr || !kv_page_indices || max_pages_seq < 0 || n_blocks <= 0 || sinks < 0 || recent < 1 || sinks > n_blocks - recent || !blocks ||
-        !block_pages || !scores)
+extern "C" int leankv_byte_select(const leankv_byte_select_t* a, void* stream) {
+    if (!a || !bytes::good_pool(&a->pool) || !bytes::good_type(a->dtype) || !a->q.data || a->batch <= 0 || a->q_heads <= 0 ||
+        a->q_heads % a->pool.kv_heads != 0 || !a->kv_indptr || !a->kv_page_indices || a->max_pages_seq < 0 || a->n_blocks <= 0 || a->sinks < 0 ||
+        a->recent < 1 || a->sinks > a->n_blocks - a->recent || !a->blocks || !a->block_pages || !a->scores)
         return LEANKV_EINVAL;
-    if (B > LEANKV_BYTES_MAX_BATCH || q_heads / pool->kv_heads > LEANKV_BYTES_MAX_GROUP || pool->kv_heads > 65535) return LEANKV_ELIMIT;
-    if (!bytes::aligned_pool(pool) || !bytes::aligned_vectors(q, dtype, B, q_heads, 1)) return LEANKV_EALIGN;
+    if (a->batch > LEANKV_BYTES_MAX_BATCH || a->q_heads / a->pool.kv_heads > LEANKV_BYTES_MAX_GROUP || a->pool.kv_heads > 65535) return LEANKV_ELIMIT;
+    if (!bytes::aligned_pool(&a->pool) || !bytes::aligned_vectors(&a->q, a->dtype, a->batch, a->q_heads, 1)) return LEANKV_EALIGN;
     bytes::SelectParams p = {};
-    p.bounds = static_cast<const uint8_t*>(pool->bounds);
-    p.H = pool->kv_heads, p.n_pages = pool->n_pages, p.G = q_heads / pool->kv_heads;
-    p.max_pages = max_pages_seq, p.n_blocks = n_blocks, p.sinks = sinks, p.recent = recent;
-    p.q = *q;
-    p.indptr = kv_indptr, p.indices = kv_page_indices;
-    p.scores = scores, p.blocks = blocks, p.block_pages = block_pages;
+    p.bounds = static_cast<const uint8_t*>(a->pool.bounds);
+    p.H = a->pool.kv_heads, p.n_pages = a->pool.n_pages, p.G = a->q_heads / a->pool.kv_heads;
+    p.max_pages = a->max_pages_seq, p.n_blocks = a->n_blocks, p.sinks = a->sinks, p.recent = a->recent;
+    p.q = a->q;
+    p.indptr = a->kv_indptr, p.indices = a->kv_page_indices;
+    p.scores = a->scores, p.blocks = a->blocks, p.block_pages = a->block_pages;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (pool->dim == 128)
-        return dtype == LEANKV_BYTES_F16 ? bytes::launch<__half, 128>(p, B, st) : dtype == LEANKV_BYTES_BF16 ? bytes::launch<bf16, 128>(p, B, st) : bytes::launch<float, 128>(p, B, st);
-    return dtype == LEANKV_BYTES_F16 ? bytes::launch<__half, 64>(p, B, st) : dtype == LEANKV_BYTES_BF16 ? bytes::launch<bf16, 64>(p, B, st) : bytes::launch<float, 64>(p, B, st);
+    const int B = a->batch;
+    if (a->pool.dim == 128)
+        return a->dtype == LEANKV_BYTES_F16 ? bytes::launch<__half, 128>(p, B, st) : a->dtype == LEANKV_BYTES_BF16 ? bytes::launch<bf16, 128>(p, B, st) : bytes::launch<float, 128>(p, B, st);
+    return a->dtype == LEANKV_BYTES_F16 ? bytes::launch<__half, 64>(p, B, st) : a->dtype == LEANKV_BYTES_BF16 ? bytes::launch<bf16, 64>(p, B, st) : bytes::launch<float, 64>(p, B, st);
 }

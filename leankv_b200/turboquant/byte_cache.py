@@ -33,16 +33,25 @@ from .paged_cache import PAGE, PagedKVCache
 _TYPES = {torch.float16: _native.BYTES_F16, torch.bfloat16: _native.BYTES_BF16, torch.float32: _native.BYTES_F32}
 
 
-def _vectors(t: torch.Tensor, token: bool = True) -> tuple:
-    """``[B, H, T, D]`` (or ``[B, H, D]``) as the kernels read it, and the tensor that they read: the one given where its vectors are
-    contiguous and begin at whole 16-byte pieces, else a copy."""
-    size = t.element_size()
-    strides = t.stride()
-    piece = 16 // size
-    if strides[-1] != 1 or t.data_ptr() % 16 or any(s % piece and n > 1 for s, n in zip(strides[:-1], t.shape[:-1])):
+def _readable(t: torch.Tensor) -> bool:
+    """Whether the kernels read ``t`` where it is: each vector contiguous, all of them from 16-byte boundaries on."""
+    piece = 16 // t.element_size()
+    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % piece == 0 or n == 1 for s, n in zip(t.stride()[:-1], t.shape[:-1]))
+
+
+def _point(v: _native.Vectors, t: torch.Tensor) -> torch.Tensor:
+    """Fills ``v`` from ``t`` ([B, H, T, D] or [B, H, D]); returns the tensor that ``v`` points to, ``t`` or a copy of it."""
+    if t.is_contiguous():
+        if t.data_ptr() % 16:
+            t = t.clone()
+    elif not _readable(t):
         t = t.clone(memory_format=torch.contiguous_format)
-        strides = t.stride()
-    return _native.Vectors(t.data_ptr(), strides[0], strides[1], strides[2] if token else 0), t
+    v.data = t.data_ptr()
+    strides = t.stride()
+    v.seq, v.head = strides[0], strides[1]
+    if len(strides) == 4:
+        v.token = strides[2]
+    return t
 
 
 class ByteKVCache(PagedKVCache):
@@ -72,9 +81,6 @@ class ByteKVCache(PagedKVCache):
         self._chunk, self._bound = 32 * head_dim + 16, 2 * head_dim + 16
         zeros = lambda n: torch.zeros(num_layers, max_pages, num_kv_heads, n, dtype=torch.uint8, device=self._device)
         self.kv_data, self.bounds = zeros(self._chunk), zeros(self._bound)
-        self._pools = [_native.BytePool(head_dim, num_kv_heads, max_pages, self.kv_data[i].data_ptr(), self.bounds[i].data_ptr())
-                       for i in range(num_layers)]
-
         self._seq_lengths: list[int] = []
         self._batch_size = 0
         self._free_count = max_pages
@@ -84,26 +90,53 @@ class ByteKVCache(PagedKVCache):
         # not on first use: a call that is being captured would record the clearing instead of doing it
         size = _native.byte_lib().leankv_byte_attn_workspace_bytes() if self._device.type == "cuda" else 0
         self._workspace = torch.zeros(size, dtype=torch.uint8, device=self._device)
-        self._scale = 1.0 / math.sqrt(head_dim)
-        self._prompt_rows = 128               # (token, query head) rows of a kv head from which a chunk goes to the prompt kernel
+        # (token, query head) rows of a kv head from which a chunk goes to the prompt kernel
+        self._prompt_rows = 128
+        # the calls' arguments, one set for each layer: a call fills in what changes
+        self._args = []
+        for i in range(num_layers):
+            pool = _native.BytePool(head_dim, num_kv_heads, max_pages, self.kv_data[i].data_ptr(), self.bounds[i].data_ptr())
+            attn = _native.ByteAttn(pool=pool, q_heads=num_q_heads, scale=1.0 / math.sqrt(head_dim), workspace=self._workspace.data_ptr(),
+                                    workspace_bytes=size)
+            self._args.append((_native.ByteAppend(pool=pool), attn, _native.ByteSelect(pool=pool, q_heads=num_q_heads)))
         self._alloc_tables(0)
+
+    def _alloc_tables(self, batch_cap: int):
+        super()._alloc_tables(batch_cap)
+        table = {"kv_indptr": self._kv_indptr, "kv_page_indices": self._kv_page_indices, "kv_last_page_len": self._kv_last}
+        for args in self._args:
+            for a in args:
+                for name, t in table.items():
+                    if hasattr(a, name):
+                        setattr(a, name, t.data_ptr())
+        self._step_args = (self._seq_len_dev.data_ptr(), self._block_table.data_ptr(), self._pps_cap, self._free_stack.data_ptr(),
+                           self._free_top.data_ptr(), self._kv_indptr.data_ptr(), self._kv_page_indices.data_ptr(),
+                           self._kv_last.data_ptr(), self._start_dev.data_ptr(), self._status.data_ptr())
+
+    def _table_step(self, t_new: int, batch: int):
+        with _native.on_device(self._device):
+            rc = _native.lib().leankv_paged_table_step(t_new, batch, *self._step_args, _native.current_stream())
+        _native.check(rc, "leankv_paged_table_step")
+        self._meta_batch = batch
 
     # ── arguments ──────────────────────────────────────────────────────
 
-    def _layer(self, layer_idx: int):
+    def _layer(self, layer_idx: int) -> tuple:
         if not 0 <= layer_idx < self.num_layers:
             raise RuntimeError(f"ByteKVCache has layers 0 .. {self.num_layers - 1}, not {layer_idx}")
-        return byref(self._pools[layer_idx])
+        return self._args[layer_idx]
 
     def _typed(self, t: torch.Tensor, name: str, *shape) -> torch.Tensor:
         """``t`` after the checks that every call makes; a type that the kernels do not read becomes the cache's own."""
-        _native.require_cuda(t, name)
-        if t.device.index != (self.kv_data.device.index):
+        if not t.is_cuda:
+            _native.require_cuda(t, name)
+        if t.get_device() != self.kv_data.get_device():
             raise RuntimeError(f"{name} is on {t.device}, the cache on {self.kv_data.device}")
-        if t.dim() != len(shape) or any(want is not None and n != want for n, want in zip(t.shape, shape)) or t.shape[0] < 1:
+        got = t.shape
+        if len(got) != len(shape) or any(want is not None and n != want for n, want in zip(got, shape)) or got[0] < 1:
             want = ", ".join("*" if n is None else str(n) for n in shape)
-            raise RuntimeError(f"{name} must be [{want}], not {list(t.shape)}")
-        if t.shape[0] > _native.BYTES_MAX_BATCH:
+            raise RuntimeError(f"{name} must be [{want}], not {list(got)}")
+        if got[0] > _native.BYTES_MAX_BATCH:
             raise RuntimeError(f"{name}: the page table holds up to {_native.BYTES_MAX_BATCH} sequences")
         return t if t.dtype in _TYPES else t.to(self._dtype)
 
@@ -121,7 +154,7 @@ class ByteKVCache(PagedKVCache):
         that all layers share; the other layers' tokens of the same step follow it."""
         k = self._typed(key_states, "key_states", None, self.num_kv_heads, None, self.head_dim)
         v = self._typed(value_states, "value_states", k.shape[0], self.num_kv_heads, k.shape[2], self.head_dim)
-        pool, lib = self._layer(layer_idx), _native.byte_lib()
+        args, lib = self._layer(layer_idx)[0], _native.byte_lib()
         batch, _, t_new, _ = k.shape
         if k.dtype != v.dtype:
             v = v.to(k.dtype)
@@ -142,23 +175,23 @@ class ByteKVCache(PagedKVCache):
                 known[b] += t_new
         elif len(self._seq_lengths) < batch or min(self._seq_lengths[:batch]) < t_new:
             raise RuntimeError("ByteKVCache: layer 0 has not appended these tokens yet")
-        indptr, flat, last = self._device_meta(batch)
-        (kd, k), (vd, v) = _vectors(k), _vectors(v)
+        self._device_meta(batch)
+        args.dtype, args.batch, args.tokens = _TYPES[k.dtype], batch, t_new
+        k, v = _point(args.k, k), _point(args.v, v)
         with _native.on_device(self._device):
-            rc = lib.leankv_byte_append(pool, _TYPES[k.dtype], byref(kd), byref(vd), batch, t_new, indptr.data_ptr(), flat.data_ptr(),
-                                        last.data_ptr(), _native.current_stream())
+            rc = lib.leankv_byte_append(byref(args), _native.current_stream())
         _native.check(rc, "leankv_byte_append", lib)
 
     def _gather_kv(self, layer_idx: int, batch_size: int):
         """Dense ``[B, Hkv, max_seq, D]`` K and V in the cache's type (zeros behind a sequence's last token)."""
-        pool, lib = self._layer(layer_idx), _native.byte_lib()
+        pool, lib = self._layer(layer_idx)[0].pool, _native.byte_lib()
         max_seq = max(self._seq_lengths[:batch_size], default=0)
         shape = (batch_size, self.num_kv_heads, max_seq, self.head_dim)
         keys, values = (torch.empty(shape, dtype=self._dtype, device=self._device) for _ in range(2))
         if batch_size and max_seq:
             indptr, flat, last = self._device_meta(batch_size)
             with _native.on_device(self._device):
-                rc = lib.leankv_byte_unpack(pool, _TYPES[self._dtype], keys.data_ptr(), values.data_ptr(), batch_size, max_seq,
+                rc = lib.leankv_byte_unpack(byref(pool), _TYPES[self._dtype], keys.data_ptr(), values.data_ptr(), batch_size, max_seq,
                                             indptr.data_ptr(), flat.data_ptr(), last.data_ptr(), _native.current_stream())
             _native.check(rc, "leankv_byte_unpack", lib)
         return keys, values
@@ -181,24 +214,23 @@ class ByteKVCache(PagedKVCache):
 
     def _attend(self, layer_idx: int, q: torch.Tensor, out: torch.Tensor, tokens: int, lists=None, n_lists: int = 0, prompt: bool = False) -> None:
         """``q`` and ``out`` [B, Hq, (T,) D]: the last ``tokens`` tokens of each sequence over the pages."""
-        pool, lib, batch = self._layer(layer_idx), _native.byte_lib(), q.shape[0]
-        indptr, flat, last = self._device_meta(batch)
-        (qd, q), (od, _) = _vectors(q, q.dim() == 4), _vectors(out, q.dim() == 4)
-        call = [pool, _TYPES[q.dtype], byref(qd), byref(od), batch, self.num_q_heads, tokens, self._scale, indptr.data_ptr(),
-                flat.data_ptr(), last.data_ptr(), self._most_pages(batch)]
+        a, lib, batch = self._layer(layer_idx)[1], _native.byte_lib(), q.shape[0]
+        self._device_meta(batch)
+        a.dtype, a.batch, a.tokens = _TYPES[q.dtype], batch, tokens
+        q = _point(a.q, q)
+        _point(a.out, out)
+        a.max_pages_seq, a.total_pages = self._most_pages(batch), self.max_pages - self._free_count
+        a.block_pages, a.n_blocks = lists, n_lists
         with _native.on_device(self._device):
-            if prompt:
-                rc = lib.leankv_byte_prompt_attn(*call, self._workspace.data_ptr(), self._workspace.numel(), _native.current_stream())
-            else:
-                rc = lib.leankv_byte_attn(*call, self.max_pages - self._free_count, lists, n_lists, self._workspace.data_ptr(), self._workspace.numel(),
-                                          _native.current_stream())
-        _native.check(rc, "leankv_byte_attn", lib)
+            rc = (lib.leankv_byte_prompt_attn if prompt else lib.leankv_byte_attn)(byref(a), _native.current_stream())
+        if rc:
+            _native.check(rc, "leankv_byte_attn", lib)
 
     def decode_attention(self, layer_idx: int, query: torch.Tensor) -> torch.Tensor:
         """``softmax(q K^T / sqrt(d)) V`` over every stored token of each sequence; query/out ``[B, Hq, D]``."""
         q = self._typed(query, "query", None, self.num_q_heads, self.head_dim)
         self._ensure_batch_size(q.shape[0])
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         self._attend(layer_idx, q, out, 1)
         return out if out.dtype == query.dtype else out.to(query.dtype)
 
@@ -212,24 +244,26 @@ class ByteKVCache(PagedKVCache):
         self.check_blocks(blocks, sinks, recent)
         batch = q.shape[0]
         self._ensure_batch_size(batch)
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         pages = self._most_pages(batch)
         if pages <= blocks and not return_blocks:
             self._attend(layer_idx, q, out, 1)
         else:
-            pool, lib = self._layer(layer_idx), _native.byte_lib()
-            indptr, flat, _ = self._device_meta(batch)
-            chosen, ids = torch.empty(2, batch, self.num_kv_heads, blocks, dtype=torch.int32, device=q.device)
-            scores = torch.empty(batch * self.num_kv_heads * max(pages, 1), dtype=torch.float32, device=q.device)
-            qd, q = _vectors(q, False)
+            a, lib = self._layer(layer_idx)[2], _native.byte_lib()
+            self._device_meta(batch)
+            n = batch * self.num_kv_heads * blocks
+            words = torch.empty(2 * n + batch * self.num_kv_heads * pages, dtype=torch.int32, device=q.device)
+            at = words.data_ptr()
+            a.dtype, a.batch = _TYPES[q.dtype], batch
+            q = _point(a.q, q)
+            a.max_pages_seq, a.n_blocks, a.sinks, a.recent = pages, blocks, sinks, recent
+            a.blocks, a.block_pages, a.scores = at, at + 4 * n, at + 8 * n
             with _native.on_device(self._device):
-                rc = lib.leankv_byte_select(pool, _TYPES[q.dtype], byref(qd), batch, self.num_q_heads, indptr.data_ptr(),
-                                            flat.data_ptr(), pages, blocks, sinks, recent, chosen.data_ptr(), ids.data_ptr(),
-                                            scores.data_ptr(), _native.current_stream())
+                rc = lib.leankv_byte_select(byref(a), _native.current_stream())
             _native.check(rc, "leankv_byte_select", lib)
-            self._attend(layer_idx, q, out, 1, ids.data_ptr(), blocks)
+            self._attend(layer_idx, q, out, 1, at + 4 * n, blocks)
         out = out if out.dtype == query.dtype else out.to(query.dtype)
-        return (out, chosen) if return_blocks else out
+        return (out, words[:n].view(batch, self.num_kv_heads, blocks)) if return_blocks else out
 
     def prefill_attention(self, layer_idx: int, query: torch.Tensor) -> torch.Tensor:
         """Causal attention of the last T tokens of every sequence (the chunk that ``append`` has just added) over everything up to

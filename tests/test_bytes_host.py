@@ -10,7 +10,7 @@ import torch
 
 from leankv_b200 import _native, combined
 from leankv_b200.turboquant import hf_attention
-from leankv_b200.turboquant.byte_cache import ByteKVCache, _vectors
+from leankv_b200.turboquant.byte_cache import ByteKVCache, _point
 from leankv_b200.turboquant.paged_cache import PagedKVCache
 from oracle import bytes as obytes
 
@@ -77,18 +77,37 @@ def test_tensors_on_the_cpu_are_refused():
 
 
 def test_vectors_are_read_where_they_are_or_copied():
+    d = _native.Vectors()
     x = torch.zeros(2, 3, 8, 64, dtype=torch.float16)
-    d, y = _vectors(x)
-    assert y is x and (d.seq, d.head, d.token) == (3 * 8 * 64, 8 * 64, 64)
+    assert _point(d, x) is x and (d.data, d.seq, d.head, d.token) == (x.data_ptr(), 3 * 8 * 64, 8 * 64, 64)
     view = torch.zeros(2, 8, 3, 64, dtype=torch.bfloat16).transpose(1, 2)
-    d, y = _vectors(view)
-    assert y is view and (d.seq, d.head, d.token) == (8 * 3 * 64, 64, 3 * 64)
+    assert _point(d, view) is view and (d.seq, d.head, d.token) == (8 * 3 * 64, 64, 3 * 64)
+    one_token = view[:, :, 5]
+    assert _point(d, one_token) is one_token and (d.data, d.seq, d.head) == (one_token.data_ptr(), 8 * 3 * 64, 64)
     for odd in (x.transpose(2, 3), torch.zeros(2, 3, 8, 68, dtype=torch.float16)[..., :64], x.reshape(-1)[4:-60].view(1, 1, -1, 64)[:, :, :2],
-                torch.zeros(2, 3, 8, 66)[..., :64]):
-        d, y = _vectors(odd)
-        assert y.is_contiguous() and torch.equal(y, odd) and y.data_ptr() % 16 == 0
+                torch.zeros(2, 3, 8, 66)[..., :64], torch.zeros(64 * 6 + 1, dtype=torch.float16)[1:].view(1, 1, 6, 64)):
+        y = _point(d, odd)
+        assert y is not odd and y.is_contiguous() and torch.equal(y, odd) and d.data == y.data_ptr() and y.data_ptr() % 16 == 0
     one = torch.zeros(1, 1, 1, 64, dtype=torch.float16).as_strided((1, 1, 1, 64), (3, 5, 7, 1))
-    assert _vectors(one)[1] is one                     # strides of extents of one are not used
+    assert _point(d, one) is one                       # strides of extents of one are not used
+
+
+def test_structures_mirror_the_header(tmp_path):
+    """Sizes and offsets of every field, from a compiled C program."""
+    import subprocess
+
+    kinds = {"leankv_byte_pool_t": _native.BytePool, "leankv_vectors_t": _native.Vectors, "leankv_byte_append_t": _native.ByteAppend,
+             "leankv_byte_attn_t": _native.ByteAttn, "leankv_byte_select_t": _native.ByteSelect}
+    lines = [f'printf("%zu {c}\\n", sizeof({c}));' for c in kinds]
+    lines += [f'printf("%zu {c}.{f[0]}\\n", offsetof({c}, {f[0]}));' for c, t in kinds.items() for f in t._fields_]
+    src = tmp_path / "s.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "leankv_bytes.h"\nint main(void) {\n' + "\n".join(lines) + "\nreturn 0; }\n")
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(tmp_path / "s")], check=True)
+    got = dict(reversed(line.split(" ")) for line in subprocess.run([str(tmp_path / "s")], capture_output=True, text=True, check=True).stdout.splitlines())
+    for c, t in kinds.items():
+        assert int(got[c]) == ctypes.sizeof(t)
+        for f in t._fields_:
+            assert int(got[f"{c}.{f[0]}"]) == getattr(t, f[0]).offset
 
 
 def test_optimize_model_checks_what_sparse_blocks_needs():
@@ -123,21 +142,22 @@ BAD_POOLS = [(dict(dim=96), -1), (dict(kv_heads=0), -1), (dict(n_pages=0), -1), 
              (dict(chunks=(1 << 20) + 8), -2), (dict(bounds=(2 << 20) + 4), -2)]
 
 
-def _append(lib, pool=None, dtype=0, k=None, v=None, B=1, T=1, indptr=64, ids=64, last=64):
-    return lib.leankv_byte_append(ctypes.byref(pool or _pool()), dtype, ctypes.byref(k or _vec()), ctypes.byref(v or _vec()), B, T, indptr, ids, last, None)
+def _append(lib, **kw):
+    f = {**dict(pool=_pool(), dtype=0, batch=1, tokens=1, k=_vec(), v=_vec(), kv_indptr=64, kv_page_indices=64, kv_last_page_len=64), **kw}
+    return lib.leankv_byte_append(ctypes.byref(_native.ByteAppend(**f)), None)
 
 
 def test_append_and_unpack_check_their_arguments():
     _no_gpu()
     lib = _native.byte_lib()
     for bad, code in BAD_POOLS:
-        assert _append(lib, _pool(**bad)) == code
+        assert _append(lib, pool=_pool(**bad)) == code
         assert lib.leankv_byte_unpack(ctypes.byref(_pool(**bad)), 0, 64, 64, 1, 1, 64, 64, 64, None) == code
-    assert lib.leankv_byte_append(None, 0, ctypes.byref(_vec()), ctypes.byref(_vec()), 1, 1, 64, 64, 64, None) == -1
-    for kw, code in ((dict(dtype=3), -1), (dict(dtype=-1), -1), (dict(B=0), -1), (dict(T=0), -1), (dict(B=1025), -6), (dict(indptr=None), -1),
-                     (dict(ids=None), -1), (dict(last=None), -1), (dict(k=_vec(data=None)), -1), (dict(v=_vec(data=24)), -2),
-                     (dict(k=_vec(head=1028)), -2), (dict(v=_vec(seq=4), B=2), -2), (dict(k=_vec(token=132), T=2), -2),
-                     (dict(k=_vec(token=2 * 128 + 2), T=2, dtype=2), -2), (dict(B=1024, T=2 ** 31 - 1), -6)):
+    assert lib.leankv_byte_append(None, None) == -1 and lib.leankv_byte_unpack(None, 0, 64, 64, 1, 1, 64, 64, 64, None) == -1
+    for kw, code in ((dict(dtype=3), -1), (dict(dtype=-1), -1), (dict(batch=0), -1), (dict(tokens=0), -1), (dict(batch=1025), -6), (dict(kv_indptr=None), -1),
+                     (dict(kv_page_indices=None), -1), (dict(kv_last_page_len=None), -1), (dict(k=_vec(data=None)), -1), (dict(v=_vec(data=24)), -2),
+                     (dict(k=_vec(head=1028)), -2), (dict(v=_vec(seq=4), batch=2), -2), (dict(k=_vec(token=132), tokens=2), -2),
+                     (dict(k=_vec(token=2 * 128 + 2), tokens=2, dtype=2), -2), (dict(batch=1024, tokens=2 ** 31 - 1), -6)):
         assert _append(lib, **kw) == code, kw
     f = lambda **kw: lib.leankv_byte_unpack(ctypes.byref(_pool()), *{**dict(dtype=0, k=64, v=64, B=1, T=1, ip=64, ids=64, last=64, st=None), **kw}.values())
     for kw, code in ((dict(dtype=5), -1), (dict(k=None), -1), (dict(v=None), -1), (dict(B=0), -1), (dict(T=0), -1), (dict(T=-3), -1), (dict(B=1025), -6),
@@ -150,42 +170,41 @@ def test_attention_checks_its_arguments():
     lib = _native.byte_lib()
     need = lib.leankv_byte_attn_workspace_bytes()
 
-    def f(pool=None, q=None, out=None, **kw):
-        a = {**dict(B=1, heads=8, tokens=1, scale=0.1, ip=64, ids=64, last=64, pages=4, total=4, lists=None, n=0, ws=1 << 22, bytes=need, st=None), **kw}
-        dtype, prompt = a.pop("dtype", 0), a.pop("prompt", False)
-        if prompt:
-            del a["total"], a["lists"], a["n"]
-            return lib.leankv_byte_prompt_attn(ctypes.byref(pool or _pool()), dtype, ctypes.byref(q or _vec()), ctypes.byref(out or _vec()), *a.values())
-        return lib.leankv_byte_attn(ctypes.byref(pool or _pool()), dtype, ctypes.byref(q or _vec()), ctypes.byref(out or _vec()), *a.values())
+    def f(prompt=False, **kw):
+        a = {**dict(pool=_pool(), dtype=0, batch=1, q_heads=8, tokens=1, q=_vec(), out=_vec(), scale=0.1, kv_indptr=64, kv_page_indices=64,
+                    kv_last_page_len=64, max_pages_seq=4, total_pages=4, workspace=1 << 22, workspace_bytes=need), **kw}
+        return (lib.leankv_byte_prompt_attn if prompt else lib.leankv_byte_attn)(ctypes.byref(_native.ByteAttn(**a)), None)
 
-    for bad, code in BAD_POOLS:
-        assert f(_pool(**bad)) == code and f(_pool(**bad), prompt=True) == code
-    for kw, code in ((dict(dtype=3), -1), (dict(B=0), -1), (dict(heads=0), -1), (dict(heads=7), -1), (dict(heads=34), -6), (dict(tokens=0), -1),
-                     (dict(B=1025), -6), (dict(ip=None), -1), (dict(ids=None), -1), (dict(last=None), -1), (dict(pages=-1), -1), (dict(total=-1), -1),
-                     (dict(lists=64, n=0), -1), (dict(lists=64, n=4, tokens=2), -1), (dict(ws=None), -3), (dict(bytes=need - 1), -3),
-                     (dict(ws=(1 << 22) + 4), -2), (dict(q=_vec(data=None)), -1), (dict(out=_vec(data=None)), -1), (dict(q=_vec(data=4)), -2),
-                     (dict(out=_vec(head=4)), -2), (dict(q=_vec(token=12), tokens=2), -2), (dict(tokens=1 << 30), -6)):
-        assert f(**kw) == code, kw
-        if "lists" not in kw and "total" not in kw:
-            assert f(**kw, prompt=True) == code, kw
-    assert f(dtype=2, prompt=True) == -5 and f(scale=0.0, prompt=True) == -1 and f(scale=math.nan, prompt=True) == -1
-    assert lib.leankv_byte_status(None, None) == -1
+    for prompt in (False, True):
+        for bad, code in BAD_POOLS:
+            assert f(prompt, pool=_pool(**bad)) == code
+        for kw, code in ((dict(dtype=3), -1), (dict(batch=0), -1), (dict(q_heads=0), -1), (dict(q_heads=7), -1), (dict(q_heads=34), -6), (dict(tokens=0), -1),
+                         (dict(batch=1025), -6), (dict(kv_indptr=None), -1), (dict(kv_page_indices=None), -1), (dict(kv_last_page_len=None), -1),
+                         (dict(max_pages_seq=-1), -1), (dict(total_pages=-1), -1), (dict(block_pages=64, n_blocks=0), -1),
+                         (dict(block_pages=64, n_blocks=4, tokens=2), -1), (dict(workspace=None), -3), (dict(workspace_bytes=need - 1), -3),
+                         (dict(workspace=(1 << 22) + 4), -2), (dict(q=_vec(data=None)), -1), (dict(out=_vec(data=None)), -1), (dict(q=_vec(data=4)), -2),
+                         (dict(out=_vec(head=4)), -2), (dict(q=_vec(token=12), tokens=2), -2), (dict(tokens=1 << 30), -6)):
+            assert f(prompt, **kw) == code, kw
+    assert f(True, dtype=2) == -5 and f(True, scale=0.0) == -1 and f(True, scale=math.nan) == -1 and f(True, block_pages=64, n_blocks=4) == -1
+    assert lib.leankv_byte_attn(None, None) == -1 and lib.leankv_byte_prompt_attn(None, None) == -1 and lib.leankv_byte_status(None, None) == -1
 
 
 def test_select_checks_its_arguments():
     _no_gpu()
     lib = _native.byte_lib()
 
-    def f(pool=None, q=None, dtype=0, **kw):
-        a = {**dict(B=1, heads=8, ip=64, ids=64, pages=40, n=8, sinks=1, recent=2, blocks=64, out=64, scores=64, st=None), **kw}
-        return lib.leankv_byte_select(ctypes.byref(pool or _pool()), dtype, ctypes.byref(q or _vec()), *a.values())
+    def f(**kw):
+        a = {**dict(pool=_pool(), dtype=0, batch=1, q_heads=8, q=_vec(), kv_indptr=64, kv_page_indices=64, max_pages_seq=40, n_blocks=8, sinks=1, recent=2,
+                    blocks=64, block_pages=64, scores=64), **kw}
+        return lib.leankv_byte_select(ctypes.byref(_native.ByteSelect(**a)), None)
 
     for bad, code in BAD_POOLS:
-        assert f(_pool(**bad)) == code
-    for kw, code in ((dict(dtype=9), -1), (dict(B=0), -1), (dict(heads=3), -1), (dict(heads=64), -6), (dict(ip=None), -1), (dict(ids=None), -1),
-                     (dict(pages=-1), -1), (dict(n=0), -1), (dict(sinks=-1), -1), (dict(recent=0), -1), (dict(sinks=7), -1), (dict(blocks=None), -1),
-                     (dict(out=None), -1), (dict(scores=None), -1), (dict(B=1025), -6), (dict(q=_vec(data=None)), -1), (dict(q=_vec(data=8)), -2),
-                     (dict(q=_vec(head=2)), -2)):
+        assert f(pool=_pool(**bad)) == code
+    assert lib.leankv_byte_select(None, None) == -1
+    for kw, code in ((dict(dtype=9), -1), (dict(batch=0), -1), (dict(q_heads=3), -1), (dict(q_heads=64), -6), (dict(kv_indptr=None), -1),
+                     (dict(kv_page_indices=None), -1), (dict(max_pages_seq=-1), -1), (dict(n_blocks=0), -1), (dict(sinks=-1), -1), (dict(recent=0), -1),
+                     (dict(sinks=7), -1), (dict(blocks=None), -1), (dict(block_pages=None), -1), (dict(scores=None), -1), (dict(batch=1025), -6),
+                     (dict(q=_vec(data=None)), -1), (dict(q=_vec(data=8)), -2), (dict(q=_vec(head=2)), -2)):
         assert f(**kw) == code, kw
 
 
