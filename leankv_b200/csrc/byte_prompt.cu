@@ -2,10 +2,11 @@
 //
 // A CTA takes 256 rows of a kv head, two tiles of 128 (query token, query head) pairs, against 128 keys (eight pages) at a time. Both row tiles use the same
 // keys and values, so that the codes are turned into fp16 operands once for 256 rows, inside this kernel:
-//   warps 8, 9   pages from memory into registers a whole key tile ahead; code + 128 behind the byte 0x64 is the fp16 number 1152 + code, one
-//                subtraction (keys) or fused multiply-add (values) makes it exact; 16-byte (8-byte) stores fill core matrices in order
-//   warp 10      S_r = Q_r K^T and O_r += P_r V of both row tiles, one thread issues
-//   warps 0 - 7  a thread a row: scores from tensor memory, maximum, weights back over the scores as fp16
+//   warps 8 - 11  pages from memory into registers a whole key tile ahead; code + 128 behind the byte 0x64 is the fp16 number 1152 + code, one
+//                 fused multiply-add makes it exact (and scales values); 16-byte (8-byte) stores fill core matrices in order
+//   warp 12       S_r = Q_r K^T and O_r += P_r V of both row tiles, one thread issues
+//   warps 0 - 7   a thread a row: scores from tensor memory, maximum, weights back over the scores as fp16
+// A row's 128 scores stay in registers, which the row warps take from the others (of the launch's 128 each: 184, converting warps 96, the last four 48).
 // The row tiles alternate: the products of one run under the exponentials of the other. Tensor memory: S of both (128 columns each), O of both (dim each).
 //
 // Exactness. Keys enter as their codes (the scale, one number for 16 keys, is multiplied to the scores in fp32), queries in fp16 with a power of two taken out
@@ -30,8 +31,8 @@ namespace {
 
 constexpr int kRowsTile = 128, kTiles = 2;
 constexpr int kKeysTile = 128, kPagesTile = kKeysTile / kPage;
-constexpr int kConvWarps = 2, kMmaWarp = 8 + kConvWarps;
-constexpr int kThreads = 32 * (kMmaWarp + 1);
+constexpr int kRowWarps = 8, kConvWarps = 4, kMmaWarp = kRowWarps + kConvWarps;
+constexpr int kThreads = 512;                         // four warpgroups: registers change hands by warpgroup
 constexpr int kPagesWarp = kPagesTile / kConvWarps;
 constexpr float kNoRef = -1.0e30f;
 constexpr float kLift = 7.f, kReach = 15.f;           // the reference of a row is its maximum - kLift when it moves, and moves beyond kReach above it
@@ -66,6 +67,12 @@ __device__ __forceinline__ uint32_t codes_times(uint32_t w, uint32_t sel, __half
 }
 // Position c of a page's 16 in the operands: the values' words hold tokens 2t, 2t + 1, 2t + 8, 2t + 9, and keys follow the same order.
 __host__ __device__ constexpr int token_at(int c) { return 2 * (c >> 2) + (c & 1) + 8 * ((c >> 1) & 1); }
+
+__device__ __forceinline__ float largest3(uint32_t a, uint32_t b, uint32_t c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
+    return d;
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams p) {
@@ -105,10 +112,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
     bool ok = true;
     const int tile = warp >> 2, row = tid & (kRowsTile - 1);             // of the row threads
     const int tok = tok0 + tile * p.tile_tokens + row / p.G;
-    const bool real = warp < 8 && row < p.tile_tokens * p.G && tok < p.tokens;
+    const bool real = warp < kRowWarps && row < p.tile_tokens * p.G && tok < p.tokens;
     const int head = kvh * p.G + row % p.G;
     float factor = 0.f;
-    if (warp < 8) {
+    if (warp < kRowWarps) {
         // ---- queries: a thread a row, fp16 with the row's power of two taken out ----
         uint8_t* to = s_q + tile * q_bytes(D);
         Eight<T> x[D / 8];
@@ -148,26 +155,74 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
         // ---- the largest exponent of the values that this CTA will see ----
         int top = 0;
         const int from = page0, to = min(page0 + n * kPagesTile, pages);
-        for (int i = from + tid - 256; i < to; i += 32 * kConvWarps) {
+        for (int i = from + tid - 32 * kRowWarps; i < to; i += 32 * kConvWarps) {
             const int id = p.indices[ip + i];
             if ((unsigned)id >= (unsigned)p.n_pages) continue;
             const uint32_t s = *reinterpret_cast<const uint32_t*>(p.chunks + ((size_t)id * p.H + kvh) * chunk_bytes(D) + 2 * half_bytes(D) + 4);
             if (s < 0x7f800000u) top = max(top, (int)(s >> 23));
         }
         top = __reduce_max_sync(0xffffffffu, top);
-        if (lane == 0) s_top[warp - 8] = top;
+        if (lane == 0) s_top[warp - kRowWarps] = top;
     }
     umma::fence_before_sync();
     __syncthreads();
     umma::fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
     const uint32_t tm_s = tmem, tm_o = tmem + 2 * kKeysTile;
-    const int top = max(max(s_top[0], s_top[1]), 1);  // biased exponent
-    float m = kNoRef, l = 0.f;
+    int top = 1;                                      // biased exponent
+#pragma unroll
+    for (int w = 0; w < kConvWarps; ++w) top = max(top, s_top[w]);
 
-    if (warp >= 8 && warp < kMmaWarp) {
+    if (warp >= kMmaWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        if (warp == kMmaWarp) {
+            // ---- products ----
+            auto scores = [&](int r, int j) {
+                if (umma::elect()) {
+                    const uint64_t a = umma::desc_k(umma::smem_addr(s_q + r * q_bytes(D)), D / 8), c = umma::desc_k(umma::smem_addr(s_k + (j & 1) * k_bytes(D)), D / 8);
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ++ks)
+                        umma::mma_f16_n(tm_s + r * kKeysTile, a + (uint64_t)ks * (2 * umma::kLbo >> 4), c + (uint64_t)ks * (2 * umma::kLbo >> 4), umma::idesc_n(kKeysTile), ks > 0);
+                    umma::commit(bar(kSFull + r));
+                    if (r == kTiles - 1 && j + 2 < n) umma::commit(bar(kKFree + (j & 1)));
+                }
+                __syncwarp();
+            };
+            if (n > 0) ok = all(wait2(kKFull, 0));
+            if (n > 0 && ok) {
+                umma::fence_after_sync();
+                for (int r = 0; r < kTiles; ++r) scores(r, 0);
+            }
+            for (int j = 0; j < n && ok; ++j) {
+                ok = all(wait2(kVFull, j));
+                for (int r = 0; r < kTiles && ok; ++r) {
+                    ok = all(wait1(kPFull + r, j));
+                    if (!ok) break;
+                    umma::fence_after_sync();
+                    if (umma::elect()) {
+                        const uint64_t c = umma::desc_k(umma::smem_addr(s_v + (j & 1) * k_bytes(D)), kKeysTile / 8);
+#pragma unroll
+                        for (int ks = 0; ks < kKeysTile / 16; ++ks)
+                            umma::mma_f16_ts(tm_o + r * D, tm_s + r * kKeysTile + 8 * ks, c + (uint64_t)ks * (2 * umma::kLbo >> 4), umma::idesc_n(D), j > 0 || ks > 0);
+                        umma::commit(bar(kPvDone + r));
+                        if (r == kTiles - 1 && j + 2 < n) umma::commit(bar(kVFree + (j & 1)));
+                    }
+                    __syncwarp();
+                    if (j + 1 < n) {                       // its scores go over these weights
+                        if (r == 0) ok = all(wait2(kKFull, j + 1));
+                        ok = ok && all(wait1(kPvDone + r, j));
+                        if (ok) {
+                            umma::fence_after_sync();
+                            scores(r, j + 1);
+                        }
+                    }
+                }
+            }
+        }
+    } else if (warp >= kRowWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
         // ---- codes to operands: a warp has pages kPagesWarp w .. of every key tile ----
-        const int first = (warp - 8) * kPagesWarp;
+        const int first = (warp - kRowWarps) * kPagesWarp;
         const int g = lane >> 2, t = lane & 3;
         constexpr int kLoads = D / 32;                // 16-byte pieces of a lane, of keys and of values
         uint4 kr[kPagesWarp][kLoads], vr[kPagesWarp][kLoads];
@@ -256,51 +311,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
             umma::fence_operands();
             umma::bar_arrive(bar(kVFull + (j & 1)));
         }
-    } else if (warp == kMmaWarp) {
-        // ---- products ----
-        auto scores = [&](int r, int j) {
-            if (umma::elect()) {
-                const uint64_t a = umma::desc_k(umma::smem_addr(s_q + r * q_bytes(D)), D / 8), c = umma::desc_k(umma::smem_addr(s_k + (j & 1) * k_bytes(D)), D / 8);
-#pragma unroll
-                for (int ks = 0; ks < D / 16; ++ks)
-                    umma::mma_f16_n(tm_s + r * kKeysTile, a + (uint64_t)ks * (2 * umma::kLbo >> 4), c + (uint64_t)ks * (2 * umma::kLbo >> 4), umma::idesc_n(kKeysTile), ks > 0);
-                umma::commit(bar(kSFull + r));
-                if (r == kTiles - 1 && j + 2 < n) umma::commit(bar(kKFree + (j & 1)));
-            }
-            __syncwarp();
-        };
-        if (n > 0) ok = all(wait2(kKFull, 0));
-        if (n > 0 && ok) {
-            umma::fence_after_sync();
-            for (int r = 0; r < kTiles; ++r) scores(r, 0);
-        }
-        for (int j = 0; j < n && ok; ++j) {
-            ok = all(wait2(kVFull, j));
-            for (int r = 0; r < kTiles && ok; ++r) {
-                ok = all(wait1(kPFull + r, j));
-                if (!ok) break;
-                umma::fence_after_sync();
-                if (umma::elect()) {
-                    const uint64_t c = umma::desc_k(umma::smem_addr(s_v + (j & 1) * k_bytes(D)), kKeysTile / 8);
-#pragma unroll
-                    for (int ks = 0; ks < kKeysTile / 16; ++ks)
-                        umma::mma_f16_ts(tm_o + r * D, tm_s + r * kKeysTile + 8 * ks, c + (uint64_t)ks * (2 * umma::kLbo >> 4), umma::idesc_n(D), j > 0 || ks > 0);
-                    umma::commit(bar(kPvDone + r));
-                    if (r == kTiles - 1 && j + 2 < n) umma::commit(bar(kVFree + (j & 1)));
-                }
-                __syncwarp();
-                if (j + 1 < n) {                       // its scores go over these weights
-                    if (r == 0) ok = all(wait2(kKFull, j + 1));
-                    ok = ok && all(wait1(kPvDone + r, j));
-                    if (ok) {
-                        umma::fence_after_sync();
-                        scores(r, j + 1);
-                    }
-                }
-            }
-        }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
         // ---- rows ----
+        float m = kNoRef, l = 0.f;
         const int lane0 = 32 * (warp & 3);
         const int qpos = start + (real ? tok : last_tok);       // rows that are none see what the last token sees; nothing of theirs is kept
         const uint32_t tm = tm_s + tile * kKeysTile, to = tm_o + tile * D;
@@ -334,12 +348,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
             float best = kNoRef;
 #pragma unroll
             for (int i = 0; i < kPagesTile; ++i) {
-                float top4[4];
-#pragma unroll
-                for (int x = 0; x < 4; ++x) top4[x] = __uint_as_float(s[i >> 1][16 * (i & 1) + x]);
-#pragma unroll
-                for (int x = 4; x < 16; ++x) top4[x & 3] = fmaxf(top4[x & 3], __uint_as_float(s[i >> 1][16 * (i & 1) + x]));
-                best = fmaxf(best, fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * ks[i]);
+                const uint32_t* v = &s[i >> 1][16 * (i & 1)];
+                float a = largest3(v[0], v[1], v[2]), c = largest3(v[3], v[4], v[5]);
+                a = largest3(__float_as_uint(a), v[6], v[7]), c = largest3(__float_as_uint(c), v[8], v[9]);
+                a = largest3(__float_as_uint(a), v[10], v[11]), c = largest3(__float_as_uint(c), v[12], v[13]);
+                best = fmaxf(best, largest3(__float_as_uint(a), __float_as_uint(c), __float_as_uint(fmaxf(__uint_as_float(v[14]), __uint_as_float(v[15])))) * ks[i]);
             }
             const bool raise = best > m + kReach;
             if (__any_sync(0xffffffffu, raise)) {
@@ -408,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
         }
         if (real && p.n_splits > 1) p.ml_part[(long long)split * p.B * p.tokens * (p.H * p.G) + vec] = make_float2(m, ok ? l : NAN);
     }
-    if (warp >= 8 && !ok && lane == 0) atomicOr(p.status, kTimedOut);
+    if (warp >= kRowWarps && !ok && lane == 0) atomicOr(p.status, kTimedOut);
     umma::fence_before_sync();
     __syncthreads();
     if (warp == kMmaWarp) {
