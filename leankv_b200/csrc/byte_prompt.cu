@@ -57,7 +57,7 @@ struct PromptParams {
     int* status;
 };
 
-enum { kQFull, kKFull, kVFull = kKFull + 2, kKFree = kVFull + 2, kVFree = kKFree + 2, kSFull = kVFree + 2, kPFull = kSFull + 2, kPvDone = kPFull + 2, kBars = kPvDone + 2 };
+enum { kQFull, kKFull, kVFull = kKFull + 2, kKFree = kVFull + 2, kVFree = kKFree + 2, kSFull = kVFree + 2, kPHalf = kSFull + 2, kPFull = kPHalf + 2, kPvDone = kPFull + 2, kBars = kPvDone + 2 };
 
 // Codes of a word's bytes 0, 1 / 2, 3 times s: (1024 + byte) s - 1152 s in one rounding of an exact number.
 __device__ __forceinline__ uint32_t codes_times(uint32_t w, uint32_t sel, __half2 s, __half2 off) {
@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
     if (warp == kMmaWarp) umma::tmem_alloc_n(umma::smem_addr(&s_tmem), 512);
     if (tid == 0) {
         for (int b = 0; b < kBars; ++b) {
-            const int count = b >= kKFull && b < kKFree ? 32 * kConvWarps : b >= kPFull && b < kPvDone ? kRowsTile : 1;
+            const int count = b >= kKFull && b < kKFree ? 32 * kConvWarps : b >= kPHalf && b < kPvDone ? kRowsTile : 1;
             umma::bar_init_n(bar(b), count);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -196,18 +196,24 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
             for (int j = 0; j < n && ok; ++j) {
                 ok = all(wait2(kVFull, j));
                 for (int r = 0; r < kTiles && ok; ++r) {
-                    ok = all(wait1(kPFull + r, j));
-                    if (!ok) break;
-                    umma::fence_after_sync();
-                    if (umma::elect()) {
-                        const uint64_t c = umma::desc_k(umma::smem_addr(s_v + (j & 1) * k_bytes(D)), kKeysTile / 8);
+                    const uint64_t c = umma::desc_k(umma::smem_addr(s_v + (j & 1) * k_bytes(D)), kKeysTile / 8);
 #pragma unroll
-                        for (int ks = 0; ks < kKeysTile / 16; ++ks)
-                            umma::mma_f16_ts(tm_o + r * D, tm_s + r * kKeysTile + 8 * ks, c + (uint64_t)ks * (2 * umma::kLbo >> 4), umma::idesc_n(D), j > 0 || ks > 0);
-                        umma::commit(bar(kPvDone + r));
-                        if (r == kTiles - 1 && j + 2 < n) umma::commit(bar(kVFree + (j & 1)));
+                    for (int part = 0; part < 2; ++part) {
+                        ok = ok && all(wait1((part == 0 ? kPHalf : kPFull) + r, j));
+                        if (!ok) break;
+                        umma::fence_after_sync();
+                        if (umma::elect()) {
+#pragma unroll
+                            for (int ks = part * 4; ks < part * 4 + 4; ++ks)
+                                umma::mma_f16_ts(tm_o + r * D, tm_s + r * kKeysTile + 8 * ks, c + (uint64_t)ks * (2 * umma::kLbo >> 4), umma::idesc_n(D), j > 0 || ks > 0);
+                            if (part == 1) {
+                                umma::commit(bar(kPvDone + r));
+                                if (r == kTiles - 1 && j + 2 < n) umma::commit(bar(kVFree + (j & 1)));
+                            }
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
+                    if (!ok) break;
                     if (j + 1 < n) {                       // its scores go over these weights
                         if (r == 0) ok = all(wait2(kKFull, j + 1));
                         ok = ok && all(wait1(kPvDone + r, j));
@@ -223,7 +229,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
         asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
         // ---- codes to operands: a warp has pages kPagesWarp w .. of every key tile ----
         const int first = (warp - kRowWarps) * kPagesWarp;
-        const int g = lane >> 2, t = lane & 3;
+        // values: lanes of half a warp have eight channels of the same tokens' half, so that their stores fill a core matrix
+        const int g = lane >> 1 & 7, t = 2 * (lane >> 4) + (lane & 1);
         constexpr int kLoads = D / 32;                // 16-byte pieces of a lane, of keys and of values
         uint4 kr[kPagesWarp][kLoads], vr[kPagesWarp][kLoads];
         float2 sc[kPagesWarp];
@@ -252,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
         auto load_values = [&](const uint8_t* chunk, int i) {
 #pragma unroll
             for (int x = 0; x < kLoads; ++x)
-                vr[i][x] = chunk == nullptr ? none : __ldg(reinterpret_cast<const uint4*>(chunk + half_bytes(D)) + x * 32 + lane);
+                vr[i][x] = chunk == nullptr ? none : __ldg(reinterpret_cast<const uint4*>(chunk + half_bytes(D)) + x * 32 + 4 * g + t);
         };
         int ids = page_of(0), ids_next = page_of(1);
 #pragma unroll
@@ -381,6 +388,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
                     w16[x / 2] = *reinterpret_cast<const uint32_t*>(&h);
                 }
                 umma::st16_async(w16, tm, lane0, 16 * c);
+                if (c == 1) {                          // the first 64 keys' product begins
+                    umma::stored();
+                    umma::fence_before_sync();
+                    umma::bar_arrive(bar(kPHalf + tile));
+                }
             }
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             umma::stored();
