@@ -370,30 +370,35 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
                 if (j > 0) scale_outputs(to, lane0, D, f);
             }
             Two sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+            // the masked form apart from the other: one loop for both spends two instructions a weight on masks that are not there
+            auto weights = [&](auto masked) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t w16[16];
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t w16[16];
 #pragma unroll
-                for (int x = 0; x < 32; x += 2) {
-                    const float k = ks[2 * c + (x >> 4)];
-                    Two w = fma2({__uint_as_float(s[c][x]), __uint_as_float(s[c][x + 1])}, {k, k}, {-m, -m});
-                    w.x = ex2(w.x);
-                    w.y = ex2(w.y);
-                    if (cut) {                         // a scale that is no number does not reach a row that does not see its block
-                        if (32 * c + (x & 16) + token_at(x & 15) > k1) w.x = 0.f;
-                        if (32 * c + (x & 16) + token_at((x + 1) & 15) > k1) w.y = 0.f;
+                    for (int x = 0; x < 32; x += 2) {
+                        const float k = ks[2 * c + (x >> 4)];
+                        Two w = fma2({__uint_as_float(s[c][x]), __uint_as_float(s[c][x + 1])}, {k, k}, {-m, -m});
+                        w.x = ex2(w.x);
+                        w.y = ex2(w.y);
+                        if constexpr (decltype(masked)::value) {         // a scale that is no number does not reach a row that does not see its block
+                            if (32 * c + (x & 16) + token_at(x & 15) > k1) w.x = 0.f;
+                            if (32 * c + (x & 16) + token_at((x + 1) & 15) > k1) w.y = 0.f;
+                        }
+                        sum[(x >> 1) & 1] = add2(sum[(x >> 1) & 1], w);
+                        const __half2 h = __floats2half2_rn(w.x, w.y);
+                        w16[x / 2] = *reinterpret_cast<const uint32_t*>(&h);
                     }
-                    sum[(x >> 1) & 1] = add2(sum[(x >> 1) & 1], w);
-                    const __half2 h = __floats2half2_rn(w.x, w.y);
-                    w16[x / 2] = *reinterpret_cast<const uint32_t*>(&h);
+                    umma::st16_async(w16, tm, lane0, 16 * c);
+                    if (c == 1) {                      // the first 64 keys' product begins
+                        umma::stored();
+                        umma::fence_before_sync();
+                        umma::bar_arrive(bar(kPHalf + tile));
+                    }
                 }
-                umma::st16_async(w16, tm, lane0, 16 * c);
-                if (c == 1) {                          // the first 64 keys' product begins
-                    umma::stored();
-                    umma::fence_before_sync();
-                    umma::bar_arrive(bar(kPHalf + tile));
-                }
-            }
+            };
+            if (cut) weights(std::true_type());
+            else weights(std::false_type());
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             umma::stored();
             umma::fence_before_sync();
