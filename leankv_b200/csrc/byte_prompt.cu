@@ -57,7 +57,7 @@ struct PromptParams {
     int* status;
 };
 
-enum { kQFull, kKFull, kVFull = kKFull + 2, kKFree = kVFull + 2, kVFree = kKFree + 2, kSFull = kVFree + 2, kPHalf = kSFull + 2, kPFull = kPHalf + 2, kPvDone = kPFull + 2, kBars = kPvDone + 2 };
+enum { kQFull, kKFull = kQFull + 2, kVFull = kKFull + 2, kKFree = kVFull + 2, kVFree = kKFree + 2, kSFull = kVFree + 2, kPHalf = kSFull + 2, kPFull = kPHalf + 2, kPvDone = kPFull + 2, kBars = kPvDone + 2 };
 
 // Codes of a word's bytes 0, 1 / 2, 3 times s: (1024 + byte) s - 1152 s in one rounding of an exact number.
 __device__ __forceinline__ uint32_t codes_times(uint32_t w, uint32_t sel, __half2 s, __half2 off) {
@@ -91,14 +91,21 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
     auto wait1 = [&](int b, int j) { return umma::bar_wait(bar(b), (uint32_t)(j & 1)); };                       // one for every key tile
     auto all = [&](bool done) { return __all_sync(0xffffffffu, done) != 0; };
 
-    if (warp == kMmaWarp) umma::tmem_alloc_n(umma::smem_addr(&s_tmem), 512);
     if (tid == 0) {
         for (int b = 0; b < kBars; ++b) {
-            const int count = b >= kKFull && b < kKFree ? 32 * kConvWarps : b >= kPHalf && b < kPvDone ? kRowsTile : 1;
+            const int count = b >= kKFull && b < kKFree ? 32 * kConvWarps : b < kKFull || (b >= kPHalf && b < kPvDone) ? kRowsTile : 1;
             umma::bar_init_n(bar(b), count);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    // tensor memory behind the wait (a launch ahead may hold some); later launches come when this one ends
+    pdl_wait();
+    if (warp == kMmaWarp) umma::tmem_alloc_n(umma::smem_addr(&s_tmem), 512);
+    umma::fence_before_sync();
+    __syncthreads();
+    umma::fence_after_sync();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
+    const uint32_t tm_s = tmem, tm_o = tmem + 2 * kKeysTile;
 
     const int kvh = blockIdx.x % p.H, b = blockIdx.x / p.H, split = blockIdx.z;
     const int ip = p.indptr[b], pages = p.indptr[b + 1] - ip;
@@ -114,65 +121,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
     const int tok = tok0 + tile * p.tile_tokens + row / p.G;
     const bool real = warp < kRowWarps && row < p.tile_tokens * p.G && tok < p.tokens;
     const int head = kvh * p.G + row % p.G;
-    float factor = 0.f;
-    if (warp < kRowWarps) {
-        // ---- queries: a thread a row, fp16 with the row's power of two taken out ----
-        uint8_t* to = s_q + tile * q_bytes(D);
-        Eight<T> x[D / 8];
-        uint32_t amax = 0;
-        const T* src = static_cast<const T*>(p.q.data) + b * p.q.seq + (long long)head * p.q.head + (long long)tok * p.q.token;
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-            if (real) x[c].load(src + 8 * c);
-            else x[c].zero();
-        }
-        int e2 = 0;
-        if constexpr (std::is_same<T, bf16>::value) {
-#pragma unroll
-            for (int c = 0; c < D / 8; ++c)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(x[c].get(e)) & 0x7fffffffu);
-            e2 = max((int)(amax >> 23) - 127 - 14, -126);
-        }
-        const float down = power_of_two(-e2);
-        factor = power_of_two(e2) * p.scale;
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-            uint32_t w[4];
-            if constexpr (std::is_same<T, bf16>::value) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const __half2 v = __floats2half2_rn(x[c].get(2 * e) * down, x[c].get(2 * e + 1) * down);
-                    w[e] = *reinterpret_cast<const uint32_t*>(&v);
-                }
-            } else {
-                w[0] = x[c].a.x, w[1] = x[c].a.y, w[2] = x[c].a.z, w[3] = x[c].a.w;
-            }
-            *reinterpret_cast<uint4*>(to + umma::offset_k(row, c, D / 8)) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        umma::fence_operands();
-    } else if (warp < kMmaWarp) {
-        // ---- the largest exponent of the values that this CTA will see ----
-        int top = 0;
-        const int from = page0, to = min(page0 + n * kPagesTile, pages);
-        for (int i = from + tid - 32 * kRowWarps; i < to; i += 32 * kConvWarps) {
-            const int id = p.indices[ip + i];
-            if ((unsigned)id >= (unsigned)p.n_pages) continue;
-            const uint32_t s = *reinterpret_cast<const uint32_t*>(p.chunks + ((size_t)id * p.H + kvh) * chunk_bytes(D) + 2 * half_bytes(D) + 4);
-            if (s < 0x7f800000u) top = max(top, (int)(s >> 23));
-        }
-        top = __reduce_max_sync(0xffffffffu, top);
-        if (lane == 0) s_top[warp - kRowWarps] = top;
-    }
-    umma::fence_before_sync();
-    __syncthreads();
-    umma::fence_after_sync();
-    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
-    const uint32_t tm_s = tmem, tm_o = tmem + 2 * kKeysTile;
-    int top = 1;                                      // biased exponent
-#pragma unroll
-    for (int w = 0; w < kConvWarps; ++w) top = max(top, s_top[w]);
-
     if (warp >= kMmaWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
         if (warp == kMmaWarp) {
@@ -189,9 +137,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
                 __syncwarp();
             };
             if (n > 0) ok = all(wait2(kKFull, 0));
-            if (n > 0 && ok) {
+            for (int r = 0; r < kTiles && ok && n > 0; ++r) {
+                ok = all(wait1(kQFull + r, 0));
                 umma::fence_after_sync();
-                for (int r = 0; r < kTiles; ++r) scores(r, 0);
+                if (ok) scores(r, 0);
             }
             for (int j = 0; j < n && ok; ++j) {
                 ok = all(wait2(kVFull, j));
@@ -269,6 +218,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
             load_values(chunk, i);
         }
         const __half2 one = __half2half2(__ushort_as_half(0x3c00)), minus = __half2half2(__ushort_as_half(0xe480));      // 1, -1152
+        int top = 1;                                  // biased exponent
         for (int j = 0; j < n && ok; ++j) {
             if (j >= 2) ok = all(wait2(kKFree, j - 2));
             if (!ok) break;
@@ -295,6 +245,24 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
             }
             umma::fence_operands();
             umma::bar_arrive(bar(kKFull + (j & 1)));
+            if (j == 0) {
+                // ---- the largest exponent of the values that this CTA will see ----
+                int e = 1;
+                const int to = min(page0 + n * kPagesTile, pages);
+#pragma unroll 4
+                for (int i = page0 + tid - 32 * kRowWarps; i < to; i += 32 * kConvWarps) {
+                    const int id = p.indices[ip + i];
+                    const uint32_t s = (unsigned)id >= (unsigned)p.n_pages
+                                           ? 0u
+                                           : __ldg(reinterpret_cast<const uint32_t*>(p.chunks + ((size_t)id * p.H + kvh) * chunk_bytes(D) + 2 * half_bytes(D) + 4));
+                    if (s < 0x7f800000u) e = max(e, (int)(s >> 23));
+                }
+                e = __reduce_max_sync(0xffffffffu, e);
+                if (lane == 0) s_top[warp - kRowWarps] = e;
+                asm volatile("bar.sync 1, %0;" ::"n"(32 * kConvWarps) : "memory");
+#pragma unroll
+                for (int w = 0; w < kConvWarps; ++w) top = max(top, s_top[w]);
+            }
             if (j >= 2) ok = all(wait2(kVFree, j - 2));
             if (!ok) break;
             uint8_t* v_to = s_v + (j & 1) * k_bytes(D);
@@ -320,6 +288,43 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+        // ---- queries: a thread a row, fp16 with the row's power of two taken out ----
+        uint8_t* q_to = s_q + tile * q_bytes(D);
+        Eight<T> x[D / 8];
+        uint32_t amax = 0;
+        const T* src = static_cast<const T*>(p.q.data) + b * p.q.seq + (long long)head * p.q.head + (long long)tok * p.q.token;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+            if (real) x[c].load(src + 8 * c);
+            else x[c].zero();
+        }
+        int e2 = 0;
+        if constexpr (std::is_same<T, bf16>::value) {
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(x[c].get(e)) & 0x7fffffffu);
+            e2 = max((int)(amax >> 23) - 127 - 14, -126);
+        }
+        const float down = power_of_two(-e2);
+        const float factor = power_of_two(e2) * p.scale;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+            uint32_t w[4];
+            if constexpr (std::is_same<T, bf16>::value) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const __half2 v = __floats2half2_rn(x[c].get(2 * e) * down, x[c].get(2 * e + 1) * down);
+                    w[e] = *reinterpret_cast<const uint32_t*>(&v);
+                }
+            } else {
+                w[0] = x[c].a.x, w[1] = x[c].a.y, w[2] = x[c].a.z, w[3] = x[c].a.w;
+            }
+            *reinterpret_cast<uint4*>(q_to + umma::offset_k(row, c, D / 8)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        umma::fence_operands();
+        umma::bar_arrive(bar(kQFull + tile));
+
         // ---- rows ----
         float m = kNoRef, l = 0.f;
         const int lane0 = 32 * (warp & 3);
@@ -408,35 +413,53 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
         umma::fence_after_sync();
         if (!ok && lane == 0) atomicOr(p.status, kTimedOut);
 
-        // ---- out ----
+        // ---- out: a warp's 32 rows through its own part of the queries (all scores have been formed), 256 bytes of each at a time ----
         const float inv = !ok ? NAN : l == 0.f ? 0.f : 1.f / l;
+        int top = 1;
+#pragma unroll
+        for (int w = 0; w < kConvWarps; ++w) top = n > 0 ? max(top, s_top[w]) : 1;
         const float back = __uint_as_float((uint32_t)top << 23);
-        const long long vec = ((long long)b * p.tokens + tok) * (p.H * p.G) + head;
-        T* dst = static_cast<T*>(p.out.data) + b * p.out.seq + (long long)head * p.out.head + (long long)tok * p.out.token;
-        float* part = p.o_part + ((long long)split * p.B * p.tokens * (p.H * p.G) + vec) * D;
+        const long long n_vec = (long long)p.B * p.tokens * (p.H * p.G);
+        uint8_t* stage = s_q + tile * q_bytes(D) + (warp & 3) * (q_bytes(D) / 4);
+        // pieces of 16 bytes: a row has kPieces of the stage, in an order of its own so that neither side meets a bank twice
+        auto leave = [&](auto kind, auto&& where) {
+            using U = decltype(kind);
+            constexpr int kEach = 16 / sizeof(U), kPieces = D / 8, kCols = kPieces * kEach;       // columns in the stage at a time
+            static_assert(kPieces == 8 || kPieces == 16, "dim 64 or 128");
 #pragma unroll
-        for (int c0 = 0; c0 < D; c0 += 32) {
-            uint32_t o[32];
-            __syncwarp();
-            if (n > 0) umma::ld32(o, to, lane0, c0);
-            if (!real) continue;
+            for (int c0 = 0; c0 < D; c0 += kCols) {
+                __syncwarp();
 #pragma unroll
-            for (int x = 0; x < 32; x += 8) {
-                float v[8];
+                for (int c1 = 0; c1 < kCols; c1 += 32) {
+                    uint32_t o[32];
+                    if (n > 0) umma::ld32(o, to, lane0, c0 + c1);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = n > 0 ? __uint_as_float(o[x + e]) * inv * back : 0.f;
-                if (p.n_splits > 1) {
-                    reinterpret_cast<float4*>(part + c0 + x)[0] = make_float4(v[0], v[1], v[2], v[3]);
-                    reinterpret_cast<float4*>(part + c0 + x)[1] = make_float4(v[4], v[5], v[6], v[7]);
-                } else {
-                    uint32_t w[4];
+                    for (int x = 0; x < 32; x += kEach) {
+                        float v[kEach];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) w[e] = pack_as<T>(v[2 * e], v[2 * e + 1]);
-                    *reinterpret_cast<uint4*>(dst + c0 + x) = make_uint4(w[0], w[1], w[2], w[3]);
+                        for (int e = 0; e < kEach; ++e) v[e] = n > 0 ? __uint_as_float(o[x + e]) * inv * back : 0.f;
+                        uint4 w;
+                        if constexpr (kEach == 4) w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+                        else w = make_uint4(pack_as<T>(v[0], v[1]), pack_as<T>(v[2], v[3]), pack_as<T>(v[4], v[5]), pack_as<T>(v[6], v[7]));
+                        *reinterpret_cast<uint4*>(stage + lane * (kPieces * 16) + (((c1 + x) / kEach ^ lane) & (kPieces - 1)) * 16) = w;
+                    }
+                }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) {
+                    const int r = (32 / kPieces) * i + lane / kPieces, piece = lane % kPieces, in_tile = lane0 + r;
+                    const int r_tok = tok0 + tile * p.tile_tokens + in_tile / p.G;
+                    const uint4 w = *reinterpret_cast<const uint4*>(stage + r * (kPieces * 16) + ((piece ^ r) & (kPieces - 1)) * 16);
+                    if (in_tile < p.tile_tokens * p.G && r_tok < p.tokens) *reinterpret_cast<uint4*>(where(kvh * p.G + in_tile % p.G, r_tok) + c0 + piece * kEach) = w;
                 }
             }
+        };
+        if (p.n_splits > 1) {
+            leave(0.f, [&](int h, int k) { return p.o_part + (split * n_vec + ((long long)b * p.tokens + k) * (p.H * p.G) + h) * D; });
+            if (real) p.ml_part[split * n_vec + ((long long)b * p.tokens + tok) * (p.H * p.G) + head] = make_float2(m, ok ? l : NAN);
+        } else {
+            leave(T(), [&](int h, int k) { return static_cast<T*>(p.out.data) + b * p.out.seq + (long long)h * p.out.head + (long long)k * p.out.token; });
         }
-        if (real && p.n_splits > 1) p.ml_part[(long long)split * p.B * p.tokens * (p.H * p.G) + vec] = make_float2(m, ok ? l : NAN);
     }
     if (warp >= kRowWarps && !ok && lane == 0) atomicOr(p.status, kTimedOut);
     umma::fence_before_sync();
@@ -483,7 +506,7 @@ int launch(const PromptParams& p, int blocks, cudaStream_t st) {
         LEANKV_CUDA_TRY(cudaFuncSetAttribute(prompt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(D)));
         ready.fetch_or(1ull << dev, std::memory_order_release);
     }
-    LEANKV_CUDA_TRY(launch_plain(prompt_kernel<T, D>, dim3((unsigned)(p.H * p.B), (unsigned)blocks, (unsigned)p.n_splits), dim3(kThreads), smem_bytes(D), st, p));
+    LEANKV_CUDA_TRY(launch_early(prompt_kernel<T, D>, dim3((unsigned)(p.H * p.B), (unsigned)blocks, (unsigned)p.n_splits), dim3(kThreads), smem_bytes(D), st, p));
     if (p.n_splits > 1) {
         const long long work = (long long)p.B * p.tokens * p.H * p.G * (D / 4);
         LEANKV_CUDA_TRY(launch_early(join_kernel<T, D>, dim3((unsigned)((work + 255) / 256)), dim3(256), 0, st, p));
