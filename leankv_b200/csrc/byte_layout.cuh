@@ -151,6 +151,18 @@ template <typename T> struct Eight {
     uint4 a;
     __device__ void load(const T* p) { a = __ldg(reinterpret_cast<const uint4*>(p)); }
     __device__ void zero() { a = make_uint4(0, 0, 0, 0); }
+    // the largest magnitude so far, two numbers' bits side by side; `bits` makes it the bits of one fp32 number
+    __device__ uint32_t largest(uint32_t m) const {
+        m = __vmaxu2(m, a.x & 0x7fff7fffu);
+        m = __vmaxu2(m, a.y & 0x7fff7fffu);
+        m = __vmaxu2(m, a.z & 0x7fff7fffu);
+        return __vmaxu2(m, a.w & 0x7fff7fffu);
+    }
+    __device__ static uint32_t bits(uint32_t m) {
+        const uint32_t one = max(m & 0xffffu, m >> 16);
+        if constexpr (std::is_same<T, bf16>::value) return one << 16;
+        else return __float_as_uint(__half2float(__ushort_as_half((unsigned short)one)));
+    }
     __device__ float get(int i) const {
         const uint32_t w = i < 2 ? a.x : i < 4 ? a.y : i < 6 ? a.z : a.w;
         if constexpr (sizeof(T) == 2 && std::is_same<T, bf16>::value) return __uint_as_float((i & 1) ? w & 0xffff0000u : w << 16);
@@ -164,6 +176,12 @@ template <> struct Eight<float> {
         b = __ldg(reinterpret_cast<const float4*>(p) + 1);
     }
     __device__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+    __device__ uint32_t largest(uint32_t m) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(get(i)) & 0x7fffffffu);
+        return m;
+    }
+    __device__ static uint32_t bits(uint32_t m) { return m; }
     __device__ float get(int i) const {
         const float4& v = i < 4 ? a : b;
         return (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;

@@ -90,8 +90,10 @@ class ByteKVCache(PagedKVCache):
         # not on first use: a call that is being captured would record the clearing instead of doing it
         size = _native.byte_lib().leankv_byte_attn_workspace_bytes() if self._device.type == "cuda" else 0
         self._workspace = torch.zeros(size, dtype=torch.uint8, device=self._device)
-        # (token, query head) rows of a kv head from which a chunk goes to the prompt kernel
-        self._prompt_rows = 128
+        # pages read by 16 (token, query head) rows at a time from which a chunk goes to the prompt kernel. Up to there the kernel for few tokens
+        # is faster (us, 8 kv heads of 4, few tokens' / prompt kernel: 32 tokens after 1000, 4 thousand of these pages, 17 / 24; 128 after 1000, 18 thousand, 30 / 27;
+        # 8 after 8000, 8 thousand, 26 / 27; 16 after 8000, 16 thousand, 36 / 27; 128 after none, 2 thousand, 9 / 13)
+        self._prompt_work = 10_000
         # the calls' arguments, one set for each layer: a call fills in what changes
         self._args = []
         for i in range(num_layers):
@@ -274,8 +276,9 @@ class ByteKVCache(PagedKVCache):
             raise RuntimeError("prefill_attention: the chunk has not been appended to this sequence")
         out = torch.empty(batch, t_new, self.num_q_heads, self.head_dim, dtype=q.dtype, device=q.device).transpose(1, 2)
         if t_new:
-            rows = t_new * (self.num_q_heads // self.num_kv_heads)
-            self._attend(layer_idx, q, out, t_new, prompt=rows >= self._prompt_rows and q.dtype != torch.float32)
+            tiles = -(-t_new * (self.num_q_heads // self.num_kv_heads) // 16)
+            work = batch * self.num_kv_heads * tiles * self._most_pages(batch)
+            self._attend(layer_idx, q, out, t_new, prompt=work > self._prompt_work and q.dtype != torch.float32)
         return out if out.dtype == query.dtype else out.to(query.dtype)
 
     def kernel_status(self) -> int:

@@ -88,13 +88,13 @@ class Pair:
         assert self.cache.kernel_status() == 0
 
     def check_prompt(self, tokens):
-        """Both kernels, whichever the number of rows would choose."""
+        """Both kernels, whichever the work would choose."""
         q = self.queries(tokens)
         want = torch.stack([self.plain.attend(b, q[b]) for b in range(self.batch)])
-        for rows in (1, 1 << 30):
-            self.cache._prompt_rows = rows
+        for work in (0, 1 << 60):
+            self.cache._prompt_work = work
             got = self.cache.prefill_attention(0, q.to(DEV))
-            close(got, want, self.dtype, weights=rows == 1 and self.dtype != F32)
+            close(got, want, self.dtype, weights=work == 0 and self.dtype != F32)
             assert self.cache.kernel_status() == 0
 
     def check_sparse(self, blocks, sinks=1, recent=2):
@@ -176,16 +176,16 @@ def test_a_block_that_holds_no_number_answers_nobody_who_sees_it(bad, which):
     cut = obytes.Cache(2, 2, 64)
     cut.blocks = [[[row[:2] for row in seq] for seq in side] for side in p.plain.blocks]
     cut.n = [32, 32]
-    for rows in (1, 1 << 30):                          # either kernel
-        p.cache._prompt_rows = rows
+    for work in (0, 1 << 60):                          # either kernel
+        p.cache._prompt_work = work
         prompt = p.cache.prefill_attention(0, q20.to(DEV)).cpu()
         assert bool(prompt[0, 2:].isnan().all())       # every token of the chunk shares the block or comes behind it
         wide = p.cache.prefill_attention(0, q40.to(DEV))
         assert bool(wide[0, 2:, 20:].isnan().all())
         want = [p.plain.attend(b, q40[b]) for b in range(2)]
-        close(wide[0, :2], want[0][:2], BF16, rows == 1)
-        close(wide[1], want[1], BF16, rows == 1)
-        close(wide[0, 2:, :20], cut.attend(0, q40[0, :, :20])[2:], BF16, rows == 1)
+        close(wide[0, :2], want[0][:2], BF16, work == 0)
+        close(wide[1], want[1], BF16, work == 0)
+        close(wide[0, 2:, :20], cut.attend(0, q40[0, :, :20])[2:], BF16, work == 0)
     # the block counts as the best one of all
     sparse, chosen = p.cache.sparse_decode_attention(0, q.to(DEV), 3, 0, 1, return_blocks=True)
     if which == 0:
@@ -316,7 +316,7 @@ def test_prompt_attention_over_several_tiles_and_shares(dtype, dim, group, heads
     p.append(tokens)
     p.check_prompt(tokens)
     q = p.queries(tokens).to(DEV)
-    p.cache._prompt_rows = 1
+    p.cache._prompt_work = 0
     first = p.cache.prefill_attention(0, q)
     assert all(torch.equal(p.cache.prefill_attention(0, q), first) for _ in range(3))
 
@@ -341,7 +341,7 @@ def test_prompt_attention_of_rows_whose_reference_moves():
     p.cache.append(0, k.to(DEV), v.to(DEV))
     p.plain.append(k, v)
     q = (torch.rand(1, 4, 300, 64, generator=p.gen) * torch.tensor([1.0, 3.0, -2.0, 0.1])[None, :, None, None]).to(BF16)
-    p.cache._prompt_rows = 1
+    p.cache._prompt_work = 0
     got = p.cache.prefill_attention(0, q.to(DEV))
     want = p.plain.attend(0, q[0])[None]
     # scores reach 130: 2^-22 of the largest product sums to 2e-5 * 130 / 20 in a weight; values of random sign as everywhere
@@ -399,10 +399,10 @@ def test_other_strides_other_types_and_views():
     p.check_pages()
     q = torch.randn(2, 40, 6, 64, generator=p.gen).to(BF16)
     on = q.to(DEV)
-    for rows in (1, 1 << 30):
-        p.cache._prompt_rows = rows
+    for work in (0, 1 << 60):
+        p.cache._prompt_work = work
         whole = p.cache.prefill_attention(0, on.transpose(1, 2))
-        close(whole, torch.stack([p.plain.attend(b, q[b].transpose(0, 1)) for b in range(2)]), BF16, rows == 1)
+        close(whole, torch.stack([p.plain.attend(b, q[b].transpose(0, 1)) for b in range(2)]), BF16, work == 0)
     one = p.cache.decode_attention(0, on.transpose(1, 2)[:, :, 7])
     assert torch.equal(one, p.cache.decode_attention(0, on[:, 7].contiguous()))
     odd = torch.zeros(2, 6, 68, dtype=BF16, device=DEV)
@@ -520,7 +520,7 @@ def test_captured_calls_on_another_stream_replay_on_new_inputs():
         dense = p.cache.decode_attention(0, q)
         few, chosen = p.cache.sparse_decode_attention(0, q, 8, return_blocks=True)
         prompt = p.cache.prefill_attention(0, q[:, :, None].expand(-1, -1, 3, -1))
-        p.cache._prompt_rows = 1
+        p.cache._prompt_work = 0
         other = p.cache.prefill_attention(0, q[:, :, None].expand(-1, -1, 3, -1))
     for _ in range(3):
         new = p.queries()
@@ -574,7 +574,7 @@ def test_page_ids_outside_the_pool_are_reported_and_left_alone():
         p.cache.prefill_attention(0, q[:, :, None].expand(-1, -1, 9, -1).to(DEV))
         assert p.cache.kernel_status() == 2
         p.cache._workspace[:4].zero_()
-        p.cache._prompt_rows = 1
+        p.cache._prompt_work = 0
         got = p.cache.prefill_attention(0, q[:, :, None].to(DEV))
         for b in (0, 2):
             close(got[b], p.plain.attend(b, q[b, :, None]), F16, weights=True)
