@@ -37,7 +37,7 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kMaxCluster = 8;
 constexpr int kFewPages = 8;                       // of a CTA: below, a smaller cluster
 constexpr int kPartPages = 16;                     // of a CTA: below, a triple is not cut into parts, nor into two (joining them costs 2 - 3 us)
-constexpr int kWavePages = 64;                     // of a CTA where there is more than one wave of them
+constexpr int kWavePages = 96;                     // of a CTA where there is more than one wave of them
 // A row's reference lies kLift below the largest score seen when it last moved, and moves when a score exceeds it by more than kReach: weights are at most
 // 2^15 in fp16, and one of 2^-24 of the largest is still a normal number there. Moving costs the rescaling of all sums.
 constexpr float kLift = 10.f, kReach = 15.f;
@@ -593,12 +593,18 @@ Plan make_plan(const int (&room)[4], long long triples, long long longest, long 
     int i = 0;
     Plan plan;
     if (triples > room[0]) {
-        // more than one wave: CTAs of kWavePages, which even out by themselves
-        while (i < 3 && longest > (kWavePages << i)) ++i;
-        plan.part_pages = kWavePages << i;
+        // more than one wave: single CTAs, which start as others end; clusters would wait for all of theirs (256 sequences of 500 tokens, 8 kv heads: 54 us, clusters
+        // of two / four 76 / 113; 80 of 4096, of 96 pages each / whole / clusters of two 124 / 133 / 122)
+        plan.part_pages = kWavePages;
     } else {
         // as many CTAs of a triple as there is room for, with kFewPages each at least; parts where whole clusters fit more than once
         while (i < 3 && room[i + 1] >= triples && longest > (kFewPages << i)) ++i;
+        // long streams in parts: smaller clusters if those fill the device by a tenth more (4 sequences of 32781 tokens: 512 CTAs in clusters of eight
+        // 55.4 us, 576 in clusters of two 52.1; one of 16384, 16 pages a CTA: 16.9 and 18.6)
+        auto used = [&](int k) { return room[k] / triples * triples << k; };
+        if (longest * triples > 64ll * used(i))
+            for (int k = i - 1; k >= 0; --k)
+                if (10 * used(k) >= 11 * used(i)) i = k;
         const long long most = room[i] / triples, even = (longest + most - 1) / most;
         plan.part_pages = (int)std::max(room[i] > triples ? std::min(even, (total + room[i] - triples - 1) / (room[i] - triples)) : even, (long long)kPartPages << i);
     }
