@@ -122,6 +122,33 @@ def test_optimize_model_checks_what_sparse_blocks_needs():
         hf_attention.enable_paged_attention(object(), _cpu_cache(), sparse_blocks=2)
 
 
+def test_decode_steps_are_routed_to_the_chosen_blocks():
+    """One-token steps go to ``sparse_decode_attention`` where the cache is set to it, and back when the plug-in is taken out."""
+    asked = []
+
+    class Cache:
+        fused_decode, fused_prefill, sparse_blocks = True, False, 5
+
+        def sparse_decode_attention(self, layer, q, blocks):
+            asked.append((layer, tuple(q.shape), blocks))
+            return q
+
+        def decode_attention(self, layer, q):
+            asked.append((layer, tuple(q.shape), None))
+            return q
+
+    class Module:
+        layer_idx = 3
+        _leankv_paged_cache = Cache()
+
+    q = torch.zeros(2, 6, 1, 64)
+    out, _ = hf_attention.paged_attention_forward(Module(), q, q, q, None)
+    assert out.shape == (2, 1, 6, 64)
+    Module._leankv_paged_cache.sparse_blocks = None
+    hf_attention.paged_attention_forward(Module(), q, q, q, None)
+    assert asked == [(3, (2, 6, 64), 5), (3, (2, 6, 64), None)]
+
+
 # ── the C ABI: refused before any launch ─────────────────────────────────────────────────────────────────────
 
 def _no_gpu():

@@ -584,3 +584,60 @@ def test_page_ids_outside_the_pool_are_reported_and_left_alone():
         assert torch.equal(p.cache.kv_data, before)
     flat.copy_(good)
     p.check_decode()
+
+
+# ── HuggingFace models ───────────────────────────────────────────────────────────────────────────────────────
+
+def _model(dtype):
+    from transformers import MistralConfig, MistralForCausalLM
+
+    torch.manual_seed(0)
+    cfg = MistralConfig(vocab_size=512, hidden_size=384, intermediate_size=768, num_hidden_layers=2, num_attention_heads=6, num_key_value_heads=2,
+                        head_dim=64, max_position_embeddings=512, rope_theta=1e6, tie_word_embeddings=False)
+    return MistralForCausalLM(cfg).to(dtype).to(DEV).eval()
+
+
+def _run(model, cache, prompts, forced):
+    logits = []
+    with torch.no_grad():
+        for ids in prompts:
+            logits.append(model(ids, past_key_values=cache, use_cache=True).logits.float().cpu())
+        for tok in forced:
+            logits.append(model(tok.reshape(-1, 1).to(DEV), past_key_values=cache, use_cache=True).logits[:, -1].float().cpu())
+    return logits
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_a_model_on_the_8_bit_cache_answers_as_on_its_dense_keys_and_values(dtype):
+    """Both routes use the same stored numbers; they differ by roundings of 16-bit attention and projections, a few eps of the logits each."""
+    from leankv_b200.combined import optimize_model, reset_optimizations
+
+    model = _model(dtype)
+    gen = torch.Generator().manual_seed(6)
+    prompts = [torch.randint(0, 512, (2, n), generator=gen).to(DEV) for n in (45, 21)]
+    forced = [torch.randint(0, 512, (2,), generator=gen) for _ in range(20)]
+    _, dense = optimize_model(model, use_paged_cache=True, turboquant_bits=8, max_pages=64)
+    assert isinstance(dense, ByteKVCache) and dense._dtype == dtype
+    want = _run(model, dense, prompts, forced)
+    for kw in (dict(), dict(fused_prefill=True), dict(fused_prefill=True, sparse_blocks=6)):
+        _, cache = optimize_model(model, use_paged_cache=True, turboquant_bits=8, max_pages=64, fused_attention=True, **kw)
+        got = _run(model, cache, prompts, forced)
+        errs = [float((a - b).norm() / b.norm()) for a, b in zip(got, want)]
+        assert max(errs) < 10 * torch.finfo(dtype).eps + 1e-3, (kw, errs)          # six blocks are all of 87 tokens
+        assert cache.kernel_status() == 0 and cache.get_seq_length() == 45 + 21 + 20
+        reset_optimizations(model)
+        assert not cache.fused_decode and cache.sparse_blocks is None
+
+
+def test_generate_reads_few_blocks():
+    from leankv_b200.combined import optimize_model, reset_optimizations
+
+    model = _model(F16)
+    ids = torch.randint(0, 512, (1, 200), generator=torch.Generator().manual_seed(1)).to(DEV)
+    _, cache = optimize_model(model, use_paged_cache=True, turboquant_bits=8, max_pages=64, fused_attention=True, fused_prefill=True, sparse_blocks=4)
+    calls = []
+    inner = cache.sparse_decode_attention
+    cache.sparse_decode_attention = lambda layer, q, blocks: calls.append((layer, blocks)) or inner(layer, q, blocks)
+    out = model.generate(ids, past_key_values=cache, max_new_tokens=9, do_sample=False, pad_token_id=0)
+    assert out.shape == (1, 209) and calls == [(layer, 4) for _ in range(8) for layer in range(2)]
+    reset_optimizations(model)
