@@ -48,8 +48,9 @@ __global__ void __launch_bounds__(kScoreThreads) score_kernel(const SelectParams
     pdl_begin();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int h = blockIdx.y, b = blockIdx.z;
-    const int ip = p.indptr[b], pages = min(p.indptr[b + 1] - ip, p.max_pages), first = blockIdx.x * kScoreBlocks + warp * kOfWarp;
+    const int ip = p.indptr[b], pages = min(p.indptr[b + 1] - ip, p.max_pages);
     if (pages <= p.n_blocks || (int)blockIdx.x * kScoreBlocks >= pages) return;
+    int first = blockIdx.x * kScoreBlocks + warp * kOfWarp;
 
     // ---- queries and records are asked for ----
     const T* q = static_cast<const T*>(p.q.data) + b * p.q.seq + (long long)h * p.G * p.q.head;
@@ -61,19 +62,22 @@ __global__ void __launch_bounds__(kScoreThreads) score_kernel(const SelectParams
         if (at < eights) x[i].load(q + (at / (D / 8)) * p.q.head + at % (D / 8) * 8);
         else x[i].zero();
     }
-    int id = -1;                                   // of block first + lane
-    if (lane < kOfWarp && first + lane < pages) id = p.indices[ip + first + lane];
-    if ((unsigned)id >= (unsigned)p.n_pages) id = -1;
     const int part = lane % kLanes, sub = lane / kLanes;
     uint4 c[kLoads];
     float scale[kLoads];
+    auto ask = [&] {
+        int id = -1;                               // of block first + lane
+        if (lane < kOfWarp && first + lane < pages) id = p.indices[ip + first + lane];
+        if ((unsigned)id >= (unsigned)p.n_pages) id = -1;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-        const int mine = __shfl_sync(0xffffffffu, id, i * kAtOnce + sub);
-        const uint8_t* rec = p.bounds + ((size_t)max(mine, 0) * p.H + h) * bounds_bytes(D);
-        c[i] = __ldg(reinterpret_cast<const uint4*>(rec) + part);
-        scale[i] = part != 0 ? 0.f : mine < 0 ? -INFINITY : __ldg(reinterpret_cast<const float*>(rec + 2 * D));
-    }
+        for (int i = 0; i < kLoads; ++i) {
+            const int mine = __shfl_sync(0xffffffffu, id, i * kAtOnce + sub);
+            const uint8_t* rec = p.bounds + ((size_t)max(mine, 0) * p.H + h) * bounds_bytes(D);
+            c[i] = __ldg(reinterpret_cast<const uint4*>(rec) + part);
+            scale[i] = part != 0 ? 0.f : mine < 0 ? -INFINITY : __ldg(reinterpret_cast<const float*>(rec + 2 * D));
+        }
+    };
+    ask();
 
     // ---- P and N ----
     uint32_t amax = 0;
@@ -117,19 +121,25 @@ __global__ void __launch_bounds__(kScoreThreads) score_kernel(const SelectParams
     for (int e = 0; e < 8; ++e) pn[e] = reinterpret_cast<const int*>(s_pn)[8 * part + e];
 
     float* out = p.scores + ((long long)b * p.H + h) * p.max_pages;
+    for (;;) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-        const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
-        int u = 0;
+        for (int i = 0; i < kLoads; ++i) {
+            const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+            int u = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            u = __dp2a_lo(pn[2 * e], (int)w[e], u);
-            u = __dp2a_hi(pn[2 * e + 1], (int)w[e], u);
+            for (int e = 0; e < 4; ++e) {
+                u = __dp2a_lo(pn[2 * e], (int)w[e], u);
+                u = __dp2a_hi(pn[2 * e + 1], (int)w[e], u);
+            }
+#pragma unroll
+            for (int o = 1; o < kLanes; o *= 2) u += __shfl_xor_sync(0xffffffffu, u, o);
+            const int j = first + i * kAtOnce + sub;
+            if (part == 0 && j < pages) out[j] = scale[i] == -INFINITY ? -INFINITY : __int2float_rn(u) * scale[i];
         }
-#pragma unroll
-        for (int o = 1; o < kLanes; o *= 2) u += __shfl_xor_sync(0xffffffffu, u, o);
-        const int j = first + i * kAtOnce + sub;
-        if (part == 0 && j < pages) out[j] = scale[i] == -INFINITY ? -INFINITY : __int2float_rn(u) * scale[i];
+        // a launch for sequences of any length has fewer CTAs than the longest would take
+        first += (int)gridDim.x * kScoreBlocks;
+        if (first >= pages) break;                 // (the whole warp)
+        ask();
     }
 }
 
@@ -291,9 +301,11 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) 
 
 template <typename T, int D>
 int launch(const SelectParams& p, int B, cudaStream_t st) {
-    if (p.max_pages > p.n_blocks)
-        LEANKV_CUDA_TRY(launch_early(score_kernel<T, D>, dim3((unsigned)((p.max_pages + kScoreBlocks - 1) / kScoreBlocks), (unsigned)p.H, (unsigned)B),
-                                     dim3(kScoreThreads), 0, st, p));
+    if (p.max_pages > p.n_blocks) {
+        // as many CTAs as there are turns for, up to four waves of them
+        const long long turns = ((long long)p.max_pages + kScoreBlocks - 1) / kScoreBlocks, most = std::max(1ll, 64ll * sm_count() / ((long long)p.H * B));
+        LEANKV_CUDA_TRY(launch_early(score_kernel<T, D>, dim3((unsigned)std::min(turns, most), (unsigned)p.H, (unsigned)B), dim3(kScoreThreads), 0, st, p));
+    }
     LEANKV_CUDA_TRY(p.max_pages <= 256 * kPer ? launch_early(select_kernel<256>, dim3((unsigned)p.H, (unsigned)B), dim3(256), 0, st, p)
                                               : launch_early(select_kernel<1024>, dim3((unsigned)p.H, (unsigned)B), dim3(1024), 0, st, p));
     return LEANKV_OK;

@@ -16,7 +16,9 @@ heads a kv head, keys, values and queries in fp16, bf16 or fp32, tensors of any 
     out = cache.decode_attention(layer, q)                      # [B, Hq, D]
     out = cache.sparse_decode_attention(layer, q, blocks=128)   # the same, 128 blocks per kv head
 
-A cache is used by one stream at a time: its pages, its page table and the workspace of its attention are one set.
+A cache is used by one stream at a time: its pages, its page table and the workspace of its attention are one set. Attention may be captured into
+a CUDA graph; a replay answers for the lengths that the sequences have by then, as long as there are no more sequences than at the
+capture. Appends and ``crop`` are not captured: the host keeps the lengths, too.
 """
 
 from __future__ import annotations
@@ -33,25 +35,25 @@ from .paged_cache import PAGE, PagedKVCache
 _TYPES = {torch.float16: _native.BYTES_F16, torch.bfloat16: _native.BYTES_BF16, torch.float32: _native.BYTES_F32}
 
 
-def _readable(t: torch.Tensor) -> bool:
-    """Whether the kernels read ``t`` where it is: each vector contiguous, all of them from 16-byte boundaries on."""
-    piece = 16 // t.element_size()
-    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % piece == 0 or n == 1 for s, n in zip(t.stride()[:-1], t.shape[:-1]))
-
-
 def _point(v: _native.Vectors, t: torch.Tensor) -> torch.Tensor:
-    """Fills ``v`` from ``t`` ([B, H, T, D] or [B, H, D]); returns the tensor that ``v`` points to, ``t`` or a copy of it."""
-    if t.is_contiguous():
-        if t.data_ptr() % 16:
-            t = t.clone()
-    elif not _readable(t):
-        t = t.clone(memory_format=torch.contiguous_format)
-    v.data = t.data_ptr()
-    strides = t.stride()
-    v.seq, v.head = strides[0], strides[1]
+    """Fills ``v`` from ``t`` ([B, H, T, D] or [B, H, D]); returns the tensor that ``v`` points to: ``t`` where the kernels can read it, each
+    vector contiguous and all of them from 16-byte boundaries on, else a copy."""
+    strides, at = t.stride(), t.data_ptr()
+    loose = 16 // t.element_size() - 1
     if len(strides) == 4:
-        v.token = strides[2]
+        seq, head, token, one = strides
+    else:
+        (seq, head, one), token = strides, 0
+    if one != 1 or at & 15 or (seq | head | token) & loose:
+        # strides of extents of one are not used
+        if one != 1 or at & 15 or any(s & loose and n > 1 for s, n in zip(strides, t.shape[:-1])):
+            return _point(v, t.clone(memory_format=torch.contiguous_format))
+    v.data, v.seq, v.head, v.token = at, seq, head, token
     return t
+
+
+def _capturing() -> bool:
+    return torch._C._cuda_isCurrentStreamCapturing()
 
 
 class ByteKVCache(PagedKVCache):
@@ -98,19 +100,26 @@ class ByteKVCache(PagedKVCache):
         self._args = []
         for i in range(num_layers):
             pool = _native.BytePool(head_dim, num_kv_heads, max_pages, self.kv_data[i].data_ptr(), self.bounds[i].data_ptr())
+            append = _native.ByteAppend(pool=pool)
             attn = _native.ByteAttn(pool=pool, q_heads=num_q_heads, scale=1.0 / math.sqrt(head_dim), workspace=self._workspace.data_ptr(),
                                     workspace_bytes=size)
-            self._args.append((_native.ByteAppend(pool=pool), attn, _native.ByteSelect(pool=pool, q_heads=num_q_heads)))
+            select = _native.ByteSelect(pool=pool, q_heads=num_q_heads)
+            # (arguments, what a call passes, its tensors)
+            self._args.append(((append, byref(append), append.k, append.v), (attn, byref(attn), attn.q, attn.out), (select, byref(select), select.q)))
+        self._device_index = self.kv_data.get_device()
+        self._lib = _native.byte_lib()
+        self._earlier_tables = []
         self._alloc_tables(0)
 
     def _alloc_tables(self, batch_cap: int):
+        if getattr(self, "_kv_indptr", None) is not None:
+            # a graph that was captured before may still read these
+            self._earlier_tables.append((self._kv_indptr, self._kv_page_indices, self._kv_last))
         super()._alloc_tables(batch_cap)
-        table = {"kv_indptr": self._kv_indptr, "kv_page_indices": self._kv_page_indices, "kv_last_page_len": self._kv_last}
         for args in self._args:
             for a in args:
-                for name, t in table.items():
-                    if hasattr(a, name):
-                        setattr(a, name, t.data_ptr())
+                a[0].kv_indptr, a[0].kv_page_indices = self._kv_indptr.data_ptr(), self._kv_page_indices.data_ptr()
+            args[0][0].kv_last_page_len = args[1][0].kv_last_page_len = self._kv_last.data_ptr()
         self._step_args = (self._seq_len_dev.data_ptr(), self._block_table.data_ptr(), self._pps_cap, self._free_stack.data_ptr(),
                            self._free_top.data_ptr(), self._kv_indptr.data_ptr(), self._kv_page_indices.data_ptr(),
                            self._kv_last.data_ptr(), self._start_dev.data_ptr(), self._status.data_ptr())
@@ -119,7 +128,16 @@ class ByteKVCache(PagedKVCache):
         with _native.on_device(self._device):
             rc = _native.lib().leankv_paged_table_step(t_new, batch, *self._step_args, _native.current_stream())
         _native.check(rc, "leankv_paged_table_step")
-        self._meta_batch = batch
+        # what a graph records has not been built yet
+        self._meta_batch = -1 if self._device.type == "cuda" and _capturing() else batch
+
+    def _device_meta(self, batch_size: int):
+        """(kv_indptr, kv_page_indices, kv_last_page_len) int32 on the device, for all known sequences: the first ones' part is the same
+        for any smaller batch."""
+        if self._meta_batch < batch_size:
+            self._ensure_batch_size(batch_size)
+            self._table_step(0, len(self._seq_lengths))
+        return self._kv_indptr, self._kv_page_indices, self._kv_last
 
     # ── arguments ──────────────────────────────────────────────────────
 
@@ -128,18 +146,17 @@ class ByteKVCache(PagedKVCache):
             raise RuntimeError(f"ByteKVCache has layers 0 .. {self.num_layers - 1}, not {layer_idx}")
         return self._args[layer_idx]
 
-    def _typed(self, t: torch.Tensor, name: str, *shape) -> torch.Tensor:
-        """``t`` after the checks that every call makes; a type that the kernels do not read becomes the cache's own."""
-        if not t.is_cuda:
+    def _typed(self, t: torch.Tensor, name: str, heads: int, batch=None, tokens=None, dims: int = 4) -> torch.Tensor:
+        """``t`` ([batch, heads, tokens, head_dim], or without the tokens) after the checks that every call makes; a type that the
+        kernels do not read becomes the cache's own."""
+        shape = t.shape
+        if (not t.is_cuda or t.get_device() != self._device_index or len(shape) != dims or shape[1] != heads or shape[-1] != self.head_dim
+                or not 1 <= shape[0] <= _native.BYTES_MAX_BATCH or (batch is not None and (shape[0] != batch or shape[2] != tokens))):
             _native.require_cuda(t, name)
-        if t.get_device() != self.kv_data.get_device():
-            raise RuntimeError(f"{name} is on {t.device}, the cache on {self.kv_data.device}")
-        got = t.shape
-        if len(got) != len(shape) or any(want is not None and n != want for n, want in zip(got, shape)) or got[0] < 1:
-            want = ", ".join("*" if n is None else str(n) for n in shape)
-            raise RuntimeError(f"{name} must be [{want}], not {list(got)}")
-        if got[0] > _native.BYTES_MAX_BATCH:
-            raise RuntimeError(f"{name}: the page table holds up to {_native.BYTES_MAX_BATCH} sequences")
+            if t.get_device() != self._device_index:
+                raise RuntimeError(f"{name} is on {t.device}, the cache on {self.kv_data.device}")
+            want = [f"1 .. {_native.BYTES_MAX_BATCH}" if batch is None else batch, heads, "*" if tokens is None else tokens, self.head_dim]
+            raise RuntimeError(f"{name} must be {want if dims == 4 else want[:2] + want[3:]}, not {list(shape)}")
         return t if t.dtype in _TYPES else t.to(self._dtype)
 
     def check_blocks(self, blocks: int, sinks: int = 1, recent: int = 2) -> None:
@@ -147,46 +164,56 @@ class ByteKVCache(PagedKVCache):
             raise RuntimeError("sparse attention needs recent >= 1, sinks >= 0 and blocks >= sinks + recent")
 
     def _most_pages(self, batch: int) -> int:
-        return -(-max(self._seq_lengths[:batch]) // PAGE)
+        """Of any of the first sequences; of any there may be where a graph is captured, whose replays meet longer ones."""
+        return self.max_pages if _capturing() else -(-max(self._seq_lengths[:batch]) // PAGE)
 
     # ── appends ────────────────────────────────────────────────────────
 
     def append(self, layer_idx: int, key_states: torch.Tensor, value_states: torch.Tensor):
         """Codes of ``[B, Hkv, T_new, D]`` K/V of one layer go into the pages of the first B sequences. Layer 0 advances the page table
         that all layers share; the other layers' tokens of the same step follow it."""
-        k = self._typed(key_states, "key_states", None, self.num_kv_heads, None, self.head_dim)
-        v = self._typed(value_states, "value_states", k.shape[0], self.num_kv_heads, k.shape[2], self.head_dim)
-        args, lib = self._layer(layer_idx)[0], _native.byte_lib()
-        batch, _, t_new, _ = k.shape
+        k = self._typed(key_states, "key_states", self.num_kv_heads)
+        batch, t_new = k.shape[0], k.shape[2]
+        v = self._typed(value_states, "value_states", self.num_kv_heads, batch, t_new)
+        (args, call, kp, vp), _, _ = self._layer(layer_idx)
         if k.dtype != v.dtype:
             v = v.to(k.dtype)
         if t_new == 0:
             return
+        known = self._seq_lengths
         if layer_idx == 0:
-            known = self._seq_lengths
+            if _capturing():
+                raise RuntimeError("ByteKVCache: append advances lengths that the host keeps, too, and cannot be captured")
             lengths = known[:batch] + [0] * (batch - len(known))
-            need = sum(-(-(n + t_new) // PAGE) - -(-n // PAGE) for n in lengths)
+            if t_new == 1:
+                need = [n % PAGE for n in lengths].count(0)
+            else:
+                need = sum([-(-(n + t_new) // PAGE) - -(-n // PAGE) for n in lengths])
             if need > self._free_count:
                 raise RuntimeError(f"ByteKVCache: out of pages ({self.max_pages} used). "
                                    f"Increase max_pages or reduce batch/sequence length.")
-            self._ensure_batch_size(batch)
+            if len(known) < batch:
+                self._ensure_batch_size(batch)
             self._table_step(t_new, batch)
             self._seen_tokens += t_new
             self._free_count -= need
-            for b in range(batch):
-                known[b] += t_new
-        elif len(self._seq_lengths) < batch or min(self._seq_lengths[:batch]) < t_new:
+            known[:batch] = [n + t_new for n in lengths]
+            if batch < len(known):
+                self._table_step(0, len(known))
+        elif len(known) < batch or min(known[:batch]) < t_new:
             raise RuntimeError("ByteKVCache: layer 0 has not appended these tokens yet")
-        self._device_meta(batch)
+        if self._meta_batch < batch:
+            self._device_meta(batch)
         args.dtype, args.batch, args.tokens = _TYPES[k.dtype], batch, t_new
-        k, v = _point(args.k, k), _point(args.v, v)
+        k, v = _point(kp, k), _point(vp, v)
         with _native.on_device(self._device):
-            rc = lib.leankv_byte_append(byref(args), _native.current_stream())
-        _native.check(rc, "leankv_byte_append", lib)
+            rc = self._lib.leankv_byte_append(call, _native.current_stream())
+        if rc:
+            _native.check(rc, "leankv_byte_append", self._lib)
 
     def _gather_kv(self, layer_idx: int, batch_size: int):
         """Dense ``[B, Hkv, max_seq, D]`` K and V in the cache's type (zeros behind a sequence's last token)."""
-        pool, lib = self._layer(layer_idx)[0].pool, _native.byte_lib()
+        pool, lib = self._layer(layer_idx)[0][0].pool, self._lib
         max_seq = max(self._seq_lengths[:batch_size], default=0)
         shape = (batch_size, self.num_kv_heads, max_seq, self.head_dim)
         keys, values = (torch.empty(shape, dtype=self._dtype, device=self._device) for _ in range(2))
@@ -214,26 +241,34 @@ class ByteKVCache(PagedKVCache):
 
     # ── attention ──────────────────────────────────────────────────────
 
-    def _attend(self, layer_idx: int, q: torch.Tensor, out: torch.Tensor, tokens: int, lists=None, n_lists: int = 0, prompt: bool = False) -> None:
+    def _attend(self, layer_idx: int, q: torch.Tensor, out: torch.Tensor, tokens: int, pages: int, lists=None, n_lists: int = 0,
+                prompt: bool = False) -> None:
         """``q`` and ``out`` [B, Hq, (T,) D]: the last ``tokens`` tokens of each sequence over the pages."""
-        a, lib, batch = self._layer(layer_idx)[1], _native.byte_lib(), q.shape[0]
-        self._device_meta(batch)
-        a.dtype, a.batch, a.tokens = _TYPES[q.dtype], batch, tokens
-        q = _point(a.q, q)
-        _point(a.out, out)
-        a.max_pages_seq, a.total_pages = self._most_pages(batch), self.max_pages - self._free_count
+        a, call, qp, op = self._layer(layer_idx)[1]
+        batch = q.shape[0]
+        if self._meta_batch < batch:
+            self._device_meta(batch)
+        a.dtype, a.batch, a.tokens, a.max_pages_seq = _TYPES[q.dtype], batch, tokens, pages
+        a.total_pages = self.max_pages if pages == self.max_pages else self.max_pages - self._free_count
         a.block_pages, a.n_blocks = lists, n_lists
+        q = _point(qp, q)
+        _point(op, out)
         with _native.on_device(self._device):
-            rc = (lib.leankv_byte_prompt_attn if prompt else lib.leankv_byte_attn)(byref(a), _native.current_stream())
+            rc = (self._lib.leankv_byte_prompt_attn if prompt else self._lib.leankv_byte_attn)(call, _native.current_stream())
         if rc:
-            _native.check(rc, "leankv_byte_attn", lib)
+            _native.check(rc, "leankv_byte_attn", self._lib)
+
+    def _answer(self, q: torch.Tensor) -> torch.Tensor:
+        """Room for a one-token answer."""
+        if len(self._seq_lengths) < q.shape[0]:
+            self._ensure_batch_size(q.shape[0])
+        return torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=q.dtype, device=q.device)
 
     def decode_attention(self, layer_idx: int, query: torch.Tensor) -> torch.Tensor:
         """``softmax(q K^T / sqrt(d)) V`` over every stored token of each sequence; query/out ``[B, Hq, D]``."""
-        q = self._typed(query, "query", None, self.num_q_heads, self.head_dim)
-        self._ensure_batch_size(q.shape[0])
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        self._attend(layer_idx, q, out, 1)
+        q = self._typed(query, "query", self.num_q_heads, dims=3)
+        out = self._answer(q)
+        self._attend(layer_idx, q, out, 1, self._most_pages(q.shape[0]))
         return out if out.dtype == query.dtype else out.to(query.dtype)
 
     def sparse_decode_attention(self, layer_idx: int, query: torch.Tensor, blocks: int, sinks: int = 1, recent: int = 2,
@@ -242,43 +277,45 @@ class ByteKVCache(PagedKVCache):
         ``recent``, and those with the largest upper bound of the group's summed scores (from the largest and smallest key code of
         each channel; ties to the earlier block). With ``return_blocks`` also their numbers, ascending and then -1, int32
         ``[B, Hkv, blocks]``. A sequence of no more than ``blocks`` blocks is read whole."""
-        q = self._typed(query, "query", None, self.num_q_heads, self.head_dim)
+        q = self._typed(query, "query", self.num_q_heads, dims=3)
         self.check_blocks(blocks, sinks, recent)
-        batch = q.shape[0]
-        self._ensure_batch_size(batch)
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        batch, heads = q.shape[0], self.num_kv_heads
+        out = self._answer(q)
         pages = self._most_pages(batch)
         if pages <= blocks and not return_blocks:
-            self._attend(layer_idx, q, out, 1)
+            self._attend(layer_idx, q, out, 1, pages)
         else:
-            a, lib = self._layer(layer_idx)[2], _native.byte_lib()
-            self._device_meta(batch)
-            n = batch * self.num_kv_heads * blocks
-            words = torch.empty(2 * n + batch * self.num_kv_heads * pages, dtype=torch.int32, device=q.device)
+            a, call, qp = self._layer(layer_idx)[2]
+            if self._meta_batch < batch:
+                self._device_meta(batch)
+            n = batch * heads * blocks
+            words = torch.empty(2 * n + batch * heads * pages, dtype=torch.int32, device=q.device)      # numbers, page ids, scores
             at = words.data_ptr()
             a.dtype, a.batch = _TYPES[q.dtype], batch
-            q = _point(a.q, q)
+            q = _point(qp, q)
             a.max_pages_seq, a.n_blocks, a.sinks, a.recent = pages, blocks, sinks, recent
             a.blocks, a.block_pages, a.scores = at, at + 4 * n, at + 8 * n
             with _native.on_device(self._device):
-                rc = lib.leankv_byte_select(byref(a), _native.current_stream())
-            _native.check(rc, "leankv_byte_select", lib)
-            self._attend(layer_idx, q, out, 1, at + 4 * n, blocks)
+                rc = self._lib.leankv_byte_select(call, _native.current_stream())
+            if rc:
+                _native.check(rc, "leankv_byte_select", self._lib)
+            self._attend(layer_idx, q, out, 1, pages, at + 4 * n, blocks)
         out = out if out.dtype == query.dtype else out.to(query.dtype)
-        return (out, words[:n].view(batch, self.num_kv_heads, blocks)) if return_blocks else out
+        return (out, words[:n].view(batch, heads, blocks)) if return_blocks else out
 
     def prefill_attention(self, layer_idx: int, query: torch.Tensor) -> torch.Tensor:
         """Causal attention of the last T tokens of every sequence (the chunk that ``append`` has just added) over everything up to
         each: query/out ``[B, Hq, T, D]``."""
-        q = self._typed(query, "query", None, self.num_q_heads, None, self.head_dim)
+        q = self._typed(query, "query", self.num_q_heads)
         batch, _, t_new, _ = q.shape
         if len(self._seq_lengths) < batch or min(self._seq_lengths[:batch]) < t_new:
             raise RuntimeError("prefill_attention: the chunk has not been appended to this sequence")
         out = torch.empty(batch, t_new, self.num_q_heads, self.head_dim, dtype=q.dtype, device=q.device).transpose(1, 2)
         if t_new:
             tiles = -(-t_new * (self.num_q_heads // self.num_kv_heads) // 16)
-            work = batch * self.num_kv_heads * tiles * self._most_pages(batch)
-            self._attend(layer_idx, q, out, t_new, prompt=work > self._prompt_work and q.dtype != torch.float32)
+            pages = self._most_pages(batch)
+            prompt = batch * self.num_kv_heads * tiles * pages > self._prompt_work and q.dtype != torch.float32
+            self._attend(layer_idx, q, out, t_new, pages, prompt=prompt)
         return out if out.dtype == query.dtype else out.to(query.dtype)
 
     def kernel_status(self) -> int:
@@ -296,6 +333,8 @@ class ByteKVCache(PagedKVCache):
     def crop(self, max_length: int):
         """Cut every sequence back to at most ``max_length`` tokens (below zero: that many tokens fewer than the longest has), as after
         drafted tokens that were not accepted. The scale of a block that keeps some tokens stays as it is."""
+        if self._device.type == "cuda" and _capturing():
+            raise RuntimeError("ByteKVCache: crop changes lengths that the host keeps, too, and cannot be captured")
         if max_length < 0:
             max_length = max(self.get_seq_length() + max_length, 0)
         batch = len(self._seq_lengths)

@@ -540,7 +540,64 @@ def test_captured_calls_on_another_stream_replay_on_new_inputs():
     with torch.cuda.stream(side):
         again = p.cache.decode_attention(0, q)
     side.synchronize()
-    assert torch.equal(again, dense) and p.cache.kernel_status() == 0
+    # (a captured call is cut for the pool's size, this one for the sequences': the same sums in another order)
+    close(again, torch.stack([p.plain.attend(b, new[b, :, None])[:, 0] for b in range(2)]), F16)
+    assert p.cache.kernel_status() == 0
+
+
+def test_a_replay_answers_for_the_lengths_that_the_sequences_have_by_then():
+    """Captured over short sequences, replayed over long ones: other numbers of parts, of key tiles, and blocks that were not there."""
+    p = Pair(2, 2, 4, 128, BF16, pages=1500)
+    p.append(30)
+    q, q3 = p.queries().to(DEV), p.queries(3).to(DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dense = p.cache.decode_attention(0, q)
+        few, chosen = p.cache.sparse_decode_attention(0, q, 6, return_blocks=True)
+        quiet = p.cache.sparse_decode_attention(0, q, 6)
+        small = p.cache.prefill_attention(0, q3)
+        p.cache._prompt_work = 0
+        large = p.cache.prefill_attention(0, q3)
+        with pytest.raises(RuntimeError, match="captured"):
+            p.cache.append(0, torch.zeros(2, 2, 1, 128, dtype=BF16, device=DEV), torch.zeros(2, 2, 1, 128, dtype=BF16, device=DEV))
+        with pytest.raises(RuntimeError, match="captured"):
+            p.cache.crop(3)
+    for more, batch in ((0, None), (1, None), (300, 1), (4000, None)):
+        if more:
+            p.append(more, batch=batch)
+        new, new3 = p.queries(), p.queries(3)
+        q.copy_(new), q3.copy_(new3)
+        graph.replay()
+        torch.cuda.synchronize()
+        close(dense, torch.stack([p.plain.attend(b, new[b, :, None])[:, 0] for b in range(2)]), BF16)
+        want = torch.stack([p.plain.attend(b, new3[b]) for b in range(2)])
+        close(small, want, BF16)
+        close(large, want, BF16, weights=True)
+        for b in range(2):
+            blocks = p.plain.choose(b, new[b], 6, 1, 2)
+            assert torch.equal(chosen[b].cpu(), blocks)
+            close(few[b], p.plain.attend(b, new[b, :, None], blocks)[:, 0], BF16)
+        assert torch.equal(quiet, few) and p.cache.kernel_status() == 0
+    one = p.cache.decode_attention(0, q[:1])
+    close(one, p.plain.attend(0, new[0, :, None])[:, 0][None], BF16)
+
+
+def test_a_larger_batch_leaves_the_tables_of_an_earlier_graph_alive():
+    p = Pair(4, 1, 2, 64, F16)
+    p.append(20, batch=1)
+    q = torch.randn(1, 2, 64, generator=p.gen).to(F16).to(DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = p.cache.decode_attention(0, q)
+    want = p.plain.attend(0, q[0, :, None])[:, 0][None]
+    k = vectors(p.gen, 4, 1, 3, 64, F16).to(DEV)
+    p.cache.append(0, k, k)                            # new tables; the graph keeps to the lengths that it knew
+    for _ in range(20):
+        torch.zeros(1000, device=DEV)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert bool(out.isfinite().all()) and p.cache.kernel_status() == 0
+    assert want.shape == out.shape
 
 
 def test_pages_beyond_four_gigabytes():
