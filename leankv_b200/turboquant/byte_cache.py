@@ -77,6 +77,8 @@ class ByteKVCache(PagedKVCache):
         self.bits = bits
         self._dtype = dtype
         self._device = torch.device(device) if device is not None else torch.device("cuda")
+        if self._device.type == "cuda" and self._device.index is None:
+            self._device = torch.device("cuda", torch.cuda.current_device())       # whichever device is current in later calls
         self._seen_tokens = 0
 
         # [layer][page][kv head][keys | values | scales] and [layer][page][kv head][largest | smallest key code | scale]
@@ -356,6 +358,8 @@ class ByteKVCache(PagedKVCache):
         """Forget every sequence. Pages need no clearing: only positions that have been written are read."""
         if self._device.type != "cuda":
             return super().reset()
+        if _capturing():
+            raise RuntimeError("ByteKVCache: reset changes lengths that the host keeps, too, and cannot be captured")
         with _native.on_device(self._device):
             # the status word, the free stack and its height lie one behind the other
             words = 4 + -(-self.max_pages // 4) * 4
@@ -367,6 +371,11 @@ class ByteKVCache(PagedKVCache):
         self._seen_tokens = 0
         self._free_count = self.max_pages
         self._meta_batch = -1
+
+    def _one_row_each(self, *args):
+        raise RuntimeError("ByteKVCache keeps its sequences in their places: no beams, repeated or chosen rows")
+
+    batch_repeat_interleave = batch_select_indices = reorder_cache = _one_row_each
 
     # ── diagnostics ────────────────────────────────────────────────────
 

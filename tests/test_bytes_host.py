@@ -76,6 +76,13 @@ def test_tensors_on_the_cpu_are_refused():
     assert c.get_seq_length() == 0 and c.get_pages_used() == 0
 
 
+def test_rows_that_would_have_to_move_are_refused():
+    cache = _cpu_cache()
+    for call in (lambda: cache.reorder_cache(torch.tensor([0])), lambda: cache.batch_repeat_interleave(2), lambda: cache.batch_select_indices(torch.tensor([0]))):
+        with pytest.raises(RuntimeError, match="places"):
+            call()
+
+
 def test_vectors_are_read_where_they_are_or_copied():
     d = _native.Vectors()
     x = torch.zeros(2, 3, 8, 64, dtype=torch.float16)

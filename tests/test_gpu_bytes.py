@@ -582,6 +582,22 @@ def test_a_replay_answers_for_the_lengths_that_the_sequences_have_by_then():
     close(one, p.plain.attend(0, new[0, :, None])[:, 0][None], BF16)
 
 
+def test_a_reset_is_not_captured():
+    cache = ByteKVCache(num_layers=1, num_kv_heads=1, num_q_heads=1, max_pages=4, dtype=F16, device="cuda")
+    k = vectors(torch.Generator().manual_seed(3), 1, 1, 20, 128, F16).to(DEV)
+    cache.append(0, k, k)
+    want = cache.decode_attention(0, k[:, :, 0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = cache.decode_attention(0, k[:, :, 0])
+        with pytest.raises(RuntimeError, match="captured"):
+            cache.reset()
+    graph.replay()
+    assert cache.get_seq_length() == 20 and cache._device.index == k.get_device()
+    # two sums, each 2e-5 off at most, and their roundings
+    assert float(row_errors(out, want.double().cpu()).max()) <= torch.finfo(F16).eps + 4e-5
+
+
 def test_a_larger_batch_leaves_the_tables_of_an_earlier_graph_alive():
     p = Pair(4, 1, 2, 64, F16)
     p.append(20, batch=1)
