@@ -110,6 +110,7 @@ class ByteKVCache(PagedKVCache):
             self._args.append(((append, byref(append), append.k, append.v), (attn, byref(attn), attn.q, attn.out), (select, byref(select), select.q)))
         self._device_index = self.kv_data.get_device()
         self._lib = _native.byte_lib()
+        self._captured = False                # an attention call was: graphs may be replayed
         self._earlier_tables = []
         self._alloc_tables(0)
 
@@ -167,7 +168,10 @@ class ByteKVCache(PagedKVCache):
 
     def _most_pages(self, batch: int) -> int:
         """Of any of the first sequences; of any there may be where a graph is captured, whose replays meet longer ones."""
-        return self.max_pages if _capturing() else -(-max(self._seq_lengths[:batch]) // PAGE)
+        if _capturing():
+            self._captured = True
+            return self.max_pages
+        return -(-max(self._seq_lengths[:batch]) // PAGE)
 
     # ── appends ────────────────────────────────────────────────────────
 
@@ -353,6 +357,8 @@ class ByteKVCache(PagedKVCache):
                 self._free_count += -(-n // PAGE) - kept
                 self._seq_lengths[b] = max_length
         self._meta_batch = -1
+        if self._captured:                    # a replay reads the flat arrays without a call of this class in between
+            self._table_step(0, batch)
 
     def reset(self):
         """Forget every sequence. Pages need no clearing: only positions that have been written are read."""
@@ -360,12 +366,18 @@ class ByteKVCache(PagedKVCache):
             return super().reset()
         if _capturing():
             raise RuntimeError("ByteKVCache: reset changes lengths that the host keeps, too, and cannot be captured")
+        # the status word, the free stack and its height lie one behind the other; before them the flat arrays and the lengths, as long as there was
+        # never more than one sequence
+        whole = self._batch_cap == 1
+        at = (self._seq_len_dev if whole else self._status).data_ptr()
+        zeros = (self._free_stack.data_ptr() - at) // 4
         with _native.on_device(self._device):
-            # the status word, the free stack and its height lie one behind the other
-            words = 4 + -(-self.max_pages // 4) * 4
-            rc = _native.lib().leankv_paged_table_begin(self._status.data_ptr(), 4, self.max_pages, words, _native.current_stream())
+            rc = _native.lib().leankv_paged_table_begin(at, zeros, self.max_pages, zeros + -(-self.max_pages // 4) * 4, _native.current_stream())
         _native.check(rc, "leankv_paged_table_begin")
-        self._seq_len_dev.zero_()
+        if not whole:
+            self._seq_len_dev.zero_()
+            if self._captured and self._seq_lengths:
+                self._table_step(0, len(self._seq_lengths))
         self._seq_lengths = []
         self._batch_size = 0
         self._seen_tokens = 0

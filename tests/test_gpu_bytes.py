@@ -598,6 +598,31 @@ def test_a_reset_is_not_captured():
     assert float(row_errors(out, want.double().cpu()).max()) <= torch.finfo(F16).eps + 4e-5
 
 
+@pytest.mark.parametrize("batch", [1, 3])
+def test_a_replay_behind_a_crop_or_a_reset_reads_what_is_left(batch):
+    p = Pair(batch, 2, 4, 64, F16)
+    p.append(40)
+    q = p.queries().to(DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = p.cache.decode_attention(0, q)
+    p.cache.crop(21)
+    p.plain.crop(21)
+    graph.replay()
+    close(out, torch.stack([p.plain.attend(b, q[b, :, None].cpu())[:, 0] for b in range(batch)]), F16)
+    p.cache.reset()
+    graph.replay()
+    assert not bool(out.any())
+    k = vectors(p.gen, batch, 2, 5, 64, F16).to(DEV)
+    p.cache.append(0, k, k)
+    graph.replay()
+    torch.cuda.synchronize()
+    fresh = obytes.Cache(batch, 2, 64)
+    fresh.append(k.cpu(), k.cpu())
+    close(out, torch.stack([fresh.attend(b, q[b, :, None].cpu())[:, 0] for b in range(batch)]), F16)
+    assert p.cache.get_pages_used() == batch and p.cache.page_table_status() == 0 and p.cache.kernel_status() == 0
+
+
 def test_a_larger_batch_leaves_the_tables_of_an_earlier_graph_alive():
     p = Pair(4, 1, 2, 64, F16)
     p.append(20, batch=1)
