@@ -24,6 +24,7 @@
 #include <atomic>
 #include <type_traits>
 
+#include "byte_cluster.cuh"
 #include "byte_layout.cuh"
 #include "byte_workspace.cuh"
 #include "umma.cuh"
@@ -34,7 +35,6 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMaxCluster = 8;
 constexpr int kFewPages = 8;                       // of a CTA: below, a smaller cluster
 constexpr int kPartPages = 16;                     // of a CTA: below, a triple is not cut into parts, nor into two (joining them costs 2 - 3 us)
 constexpr int kWavePages = 96;                     // of a CTA where there is more than one wave of them
@@ -98,26 +98,6 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 __device__ __forceinline__ float2 unpack_f16(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
-
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// Numbers at a shared address of this CTA's, as the CTA `rank` of the cluster has them there.
-__device__ __forceinline__ uint32_t peer(uint32_t at, int rank) {
-    uint32_t there;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
-    return there;
-}
-__device__ __forceinline__ float2 peer_f32x2(uint32_t at, int rank) {
-    float2 v;
-    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(peer(at, rank)));
-    return v;
-}
-__device__ __forceinline__ float4 peer_f32x4(uint32_t at, int rank) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(peer(at, rank)));
-    return v;
-}
 
 template <typename T>
 __device__ __forceinline__ void store4_as(T* to, float4 v) {

@@ -15,12 +15,18 @@
 // largest weight still has all its places; their sum is fp32 before that rounding.
 //
 // Bound: a key tile is 4 x 512 tensor cycles (dim 128) and 2 x 1024 cycles of ex2; operand reads (192 KB) and the converted tiles (64 KB written) take the
-// same time of shared memory's 128 bytes a cycle.
+// same time of shared memory's 128 bytes a cycle. It takes some 3600: a row tile's rows have 128 scores for 2400 cycles and then nothing for 1250, until the last weights
+// are multiplied (400) and the next scores formed over them (580, and 270 on the way); two row tiles are what tensor memory holds, and what one leaves the other does not fill.
+// 4096 tokens, 8 kv heads of 4, bf16: 142 us, 970 TFLOP/s; 8192: 489, 1124; 512 behind 3584: 47.8; dim 64, 4096: 123.
+//
+// Long caches behind few rows: a cluster's CTAs share the keys of a block of rows, each leaves its sums in its shared memory, and each joins a part of the rows from there
+// (through the workspace and a second kernel: 512 behind 3584 52.4 us).
 
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
 
+#include "byte_cluster.cuh"
 #include "byte_layout.cuh"
 #include "byte_workspace.cuh"
 #include "tile_softmax.cuh"
@@ -51,9 +57,7 @@ struct PromptParams {
     const int32_t* indptr;
     const int32_t* indices;
     const int32_t* last;
-    int n_splits;
-    float* o_part;                                    // [split][B][tokens][heads][dim], each divided by its own sum
-    float2* ml_part;                                  // [split][B][tokens][heads]: reference and sum
+    int n_splits;                                     // CTAs of a cluster, which share a block's keys
     int* status;
 };
 
@@ -74,13 +78,16 @@ __device__ __forceinline__ float largest3(uint32_t a, uint32_t b, uint32_t c) {
     return d;
 }
 
-template <typename T, int D>
+// kShared: a cluster's CTAs share the keys of a block of rows. A kernel of its own: with both ends in one, and their registers, the row loop of either took 5 to 10 % longer
+// (8192 tokens: 523 against 491 us).
+template <typename T, int D, bool kShared>
 __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams p) {
     extern __shared__ __align__(16) uint8_t s_raw[];
     __shared__ __align__(8) uint64_t s_bar[kBars];
     __shared__ uint32_t s_tmem;
     __shared__ int s_top[kConvWarps];
     __shared__ __align__(16) float s_ks[kScaleSlots][kPagesTile];
+    __shared__ __align__(8) float2 s_ml[kTiles * kRowsTile];          // reference and sum of a row
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     uint8_t* base = s_raw + ((1024u - (umma::smem_addr(s_raw) & 1023u)) & 1023u);
     uint8_t* s_q = base;                              // two row tiles
@@ -107,13 +114,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
     const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
     const uint32_t tm_s = tmem, tm_o = tmem + 2 * kKeysTile;
 
-    const int kvh = blockIdx.x % p.H, b = blockIdx.x / p.H, split = blockIdx.z;
+    const int kvh = blockIdx.x % p.H, b = blockIdx.x / p.H, split = kShared ? blockIdx.z : 0;
     const int ip = p.indptr[b], pages = p.indptr[b + 1] - ip;
     const int start = pages > 0 ? (pages - 1) * kPage + p.last[b] - p.tokens : -p.tokens;      // position of the chunk's first token
     const int block = (int)gridDim.y - 1 - (int)blockIdx.y;                                    // the longest first
     const int tok0 = block * kTiles * p.tile_tokens, last_tok = min(tok0 + kTiles * p.tile_tokens, p.tokens) - 1;
     const int n_all = start + last_tok < 0 ? 0 : (start + last_tok) / kKeysTile + 1;
-    const int t0 = (int)((long long)n_all * split / p.n_splits), n = (int)((long long)n_all * (split + 1) / p.n_splits) - t0;
+    const int t0 = kShared ? (int)((long long)n_all * split / p.n_splits) : 0, n = kShared ? (int)((long long)n_all * (split + 1) / p.n_splits) - t0 : n_all;
     const int page0 = t0 * kPagesTile;
 
     bool ok = true;
@@ -153,7 +160,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
                         umma::fence_after_sync();
                         if (umma::elect()) {
 #pragma unroll
-                            for (int ks = part * 4; ks < part * 4 + 4; ++ks)
+                            for (int ks = part * 6; ks < 6 + part * 2; ++ks)
                                 umma::mma_f16_ts(tm_o + r * D, tm_s + r * kKeysTile + 8 * ks, c + (uint64_t)ks * (2 * umma::kLbo >> 4), umma::idesc_n(D), j > 0 || ks > 0);
                             if (part == 1) {
                                 umma::commit(bar(kPvDone + r));
@@ -211,12 +218,22 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
                 vr[i][x] = chunk == nullptr ? none : __ldg(reinterpret_cast<const uint4*>(chunk + half_bytes(D)) + x * 32 + 4 * g + t);
         };
         int ids = page_of(0), ids_next = page_of(1);
+        // the values' scales of the CTA's pages: a thread's first two are asked for now
+        const int to = min(page0 + n * kPagesTile, pages);
+        auto page_id = [&](int i) { return i < to ? p.indices[ip + i] : -1; };
+        auto value_scale = [&](int id) {
+            return (unsigned)id >= (unsigned)p.n_pages ? 0u : __ldg(reinterpret_cast<const uint32_t*>(p.chunks + ((size_t)id * p.H + kvh) * chunk_bytes(D) + 2 * half_bytes(D) + 4));
+        };
+        constexpr int kConvThreads = 32 * kConvWarps;
+        const int own = page0 + tid - 32 * kRowWarps;
+        const int id0 = page_id(own), id1 = page_id(own + kConvThreads);
 #pragma unroll
         for (int i = 0; i < kPagesWarp; ++i) {
             const uint8_t* chunk = chunk_of(ids, i);
             load_keys(chunk, i);
             load_values(chunk, i);
         }
+        const uint32_t scale0 = value_scale(id0), scale1 = value_scale(id1);
         const __half2 one = __half2half2(__ushort_as_half(0x3c00)), minus = __half2half2(__ushort_as_half(0xe480));      // 1, -1152
         int top = 1;                                  // biased exponent
         for (int j = 0; j < n && ok; ++j) {
@@ -248,15 +265,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
             if (j == 0) {
                 // ---- the largest exponent of the values that this CTA will see ----
                 int e = 1;
-                const int to = min(page0 + n * kPagesTile, pages);
-#pragma unroll 4
-                for (int i = page0 + tid - 32 * kRowWarps; i < to; i += 32 * kConvWarps) {
-                    const int id = p.indices[ip + i];
-                    const uint32_t s = (unsigned)id >= (unsigned)p.n_pages
-                                           ? 0u
-                                           : __ldg(reinterpret_cast<const uint32_t*>(p.chunks + ((size_t)id * p.H + kvh) * chunk_bytes(D) + 2 * half_bytes(D) + 4));
+                auto look = [&](uint32_t s) {
                     if (s < 0x7f800000u) e = max(e, (int)(s >> 23));
-                }
+                };
+                look(scale0);
+                look(scale1);
+#pragma unroll 4
+                for (int i = own + 2 * kConvThreads; i < to; i += kConvThreads) look(value_scale(page_id(i)));
                 e = __reduce_max_sync(0xffffffffu, e);
                 if (lane == 0) s_top[warp - kRowWarps] = e;
                 asm volatile("bar.sync 1, %0;" ::"n"(32 * kConvWarps) : "memory");
@@ -290,14 +305,26 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
         asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
         // ---- queries: a thread a row, fp16 with the row's power of two taken out ----
         uint8_t* q_to = s_q + tile * q_bytes(D);
-        Eight<T> x[D / 8];
+        // a warp's 32 rows come by whole vectors and turn to a row a thread through where they will lie (a thread that asks for its own row's pieces: 32 rows in one load)
+        constexpr int kPieces = D / 8;
+        Eight<T> x[kPieces];
         uint32_t amax = 0;
-        const T* src = static_cast<const T*>(p.q.data) + b * p.q.seq + (long long)head * p.q.head + (long long)tok * p.q.token;
+        const long long mine = real ? (long long)head * p.q.head + (long long)tok * p.q.token : -1;
+        const T* src = static_cast<const T*>(p.q.data) + b * p.q.seq + lane % kPieces * 8;
+        uint8_t* turn = q_to + (warp & 3) * (q_bytes(D) / 4);
+        auto at = [&](int r, int piece) { return reinterpret_cast<uint4*>(turn + r * (16 * kPieces) + ((piece ^ r) & (kPieces - 1)) * 16); };
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-            if (real) x[c].load(src + 8 * c);
-            else x[c].zero();
+        for (int i = 0; i < kPieces; ++i) {
+            const long long from = __shfl_sync(0xffffffffu, mine, (32 / kPieces) * i + lane / kPieces);
+            if (from >= 0) x[i].load(src + from);
+            else x[i].zero();
         }
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) *at((32 / kPieces) * i + lane / kPieces, lane % kPieces) = x[i].a;
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c) x[c].a = *at(lane, c);
+        __syncwarp();
         int e2 = 0;
         if constexpr (std::is_same<T, bf16>::value) {
 #pragma unroll
@@ -322,6 +349,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
             }
             *reinterpret_cast<uint4*>(q_to + umma::offset_k(row, c, D / 8)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
+        // for the scales. The wait for key tile j comes before what the next tile of its buffer depends on: the queries, later the weights of tile j - 1
+        if (n > 0) ok = all(wait2(kKFull, 0));
         umma::fence_operands();
         umma::bar_arrive(bar(kQFull + tile));
 
@@ -330,8 +359,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
         const int lane0 = 32 * (warp & 3);
         const int qpos = start + (real ? tok : last_tok);       // rows that are none see what the last token sees; nothing of theirs is kept
         const uint32_t tm = tm_s + tile * kKeysTile, to = tm_o + tile * D;
-        for (int j = 0; j < n; ++j) {
-            ok = all(wait2(kVFull, j) && wait1(kSFull + tile, j));       // the first for the scales; its next phase needs these rows' weights
+        for (int j = 0; j < n && ok; ++j) {
+            ok = all(wait1(kSFull + tile, j));
             if (!ok) break;
             umma::fence_after_sync();
             uint32_t s[4][32];
@@ -395,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
                         w16[x / 2] = *reinterpret_cast<const uint32_t*>(&h);
                     }
                     umma::st16_async(w16, tm, lane0, 16 * c);
-                    if (c == 1) {                      // the first 64 keys' product begins
+                    if (c == 2) {                      // the first 96 keys' product begins (64: 157 us where this takes 154)
                         umma::stored();
                         umma::fence_before_sync();
                         umma::bar_arrive(bar(kPHalf + tile));
@@ -406,60 +435,124 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
             else weights(std::false_type());
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             umma::stored();
+            if (j + 1 < n) ok = all(wait2(kKFull, j + 1));
             umma::fence_before_sync();
             umma::bar_arrive(bar(kPFull + tile));
         }
-        if (ok && n > 0) ok = all(wait1(kPvDone + tile, n - 1));
+        if (ok && n > 0) ok = all(wait1(kPvDone + tile, n - 1) && wait2(kVFull, n - 1));       // the second for the values' largest exponent
         umma::fence_after_sync();
         if (!ok && lane == 0) atomicOr(p.status, kTimedOut);
 
-        // ---- out: a warp's 32 rows through its own part of the queries (all scores have been formed), 256 bytes of each at a time ----
+        // ---- out ----
         const float inv = !ok ? NAN : l == 0.f ? 0.f : 1.f / l;
         int top = 1;
 #pragma unroll
         for (int w = 0; w < kConvWarps; ++w) top = n > 0 ? max(top, s_top[w]) : 1;
         const float back = __uint_as_float((uint32_t)top << 23);
-        const long long n_vec = (long long)p.B * p.tokens * (p.H * p.G);
-        uint8_t* stage = s_q + tile * q_bytes(D) + (warp & 3) * (q_bytes(D) / 4);
-        // pieces of 16 bytes: a row has kPieces of the stage, in an order of its own so that neither side meets a bank twice
-        auto leave = [&](auto kind, auto&& where) {
-            using U = decltype(kind);
-            constexpr int kEach = 16 / sizeof(U), kPieces = D / 8, kCols = kPieces * kEach;       // columns in the stage at a time
-            static_assert(kPieces == 8 || kPieces == 16, "dim 64 or 128");
+        const int reciprocal = (65535 + p.G) / p.G;   // i / G is i * reciprocal >> 16 for i below 128
+        auto target = [&](int r) -> T* {              // where row r of the CTA's 256 goes, or null
+            const int in_tile = r & (kRowsTile - 1), in_tok = in_tile * reciprocal >> 16, r_tok = tok0 + (r / kRowsTile) * p.tile_tokens + in_tok;
+            if (in_tile >= p.tile_tokens * p.G || r_tok >= p.tokens) return nullptr;
+            return static_cast<T*>(p.out.data) + b * p.out.seq + (long long)(kvh * p.G + in_tile - in_tok * p.G) * p.out.head + (long long)r_tok * p.out.token;
+        };
+        const float by = inv * back;
+        // pieces of 16 bytes, in an order of each row's own so that neither side meets a bank twice
+        if constexpr (!kShared) {
+            // a warp's 32 rows through its own part of the queries (all scores have been formed), so that whole vectors leave
+            uint32_t o[D / 32][32];
+            if (n > 0) {
 #pragma unroll
-            for (int c0 = 0; c0 < D; c0 += kCols) {
-                __syncwarp();
+                for (int c = 0; c < D / 32; ++c) umma::ld32_async(o[c], to, lane0, 32 * c);
+                umma::settle(o[0]);
 #pragma unroll
-                for (int c1 = 0; c1 < kCols; c1 += 32) {
-                    uint32_t o[32];
-                    if (n > 0) umma::ld32(o, to, lane0, c0 + c1);
+                for (int c = 1; c < D / 32; ++c) umma::settled(o[c]);
+            }
+            auto number = [&](int c) { return n > 0 ? __uint_as_float(o[c >> 5][c & 31]) * by : 0.f; };
+            uint8_t* stage = s_q + tile * q_bytes(D) + (warp & 3) * (q_bytes(D) / 4);
+            __syncwarp();
 #pragma unroll
-                    for (int x = 0; x < 32; x += kEach) {
-                        float v[kEach];
+            for (int c = 0; c < kPieces; ++c)
+                *reinterpret_cast<uint4*>(stage + lane * (kPieces * 16) + ((c ^ lane) & (kPieces - 1)) * 16) =
+                    make_uint4(pack_as<T>(number(8 * c), number(8 * c + 1)), pack_as<T>(number(8 * c + 2), number(8 * c + 3)), pack_as<T>(number(8 * c + 4), number(8 * c + 5)),
+                               pack_as<T>(number(8 * c + 6), number(8 * c + 7)));
+            __syncwarp();
 #pragma unroll
-                        for (int e = 0; e < kEach; ++e) v[e] = n > 0 ? __uint_as_float(o[x + e]) * inv * back : 0.f;
-                        uint4 w;
-                        if constexpr (kEach == 4) w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-                        else w = make_uint4(pack_as<T>(v[0], v[1]), pack_as<T>(v[2], v[3]), pack_as<T>(v[4], v[5]), pack_as<T>(v[6], v[7]));
-                        *reinterpret_cast<uint4*>(stage + lane * (kPieces * 16) + (((c1 + x) / kEach ^ lane) & (kPieces - 1)) * 16) = w;
+            for (int i = 0; i < kPieces; ++i) {
+                const int r = (32 / kPieces) * i + lane / kPieces, piece = lane % kPieces;
+                const uint4 w = *reinterpret_cast<const uint4*>(stage + r * (kPieces * 16) + ((piece ^ r) & (kPieces - 1)) * 16);
+                T* dst = target(kRowsTile * tile + lane0 + r);
+                if (dst != nullptr) *reinterpret_cast<uint4*>(dst + 8 * piece) = w;
+            }
+        } else {
+            // ---- the shares of a row's keys, in order: each CTA of the cluster joins a part of the rows, from where all of them left theirs ----
+            constexpr int kFours = D / 4;             // 16-byte pieces of a row of sums
+            asm volatile("bar.sync 2, %0;" ::"n"(32 * kRowWarps) : "memory");       // keys and values have been read: the sums lie over them
+            float4* mine_at = reinterpret_cast<float4*>(s_k) + (size_t)tid * kFours;
+#pragma unroll
+            for (int c0 = 0; c0 < D; c0 += 32) {
+                uint32_t o[32];
+                if (n > 0) umma::ld32(o, to, lane0, c0);
+                auto number = [&](int x) { return n > 0 ? __uint_as_float(o[x]) * by : 0.f; };
+#pragma unroll
+                for (int x = 0; x < 32; x += 4) mine_at[(c0 + x) / 4 ^ (lane & (kFours - 1))] = make_float4(number(x), number(x + 1), number(x + 2), number(x + 3));
+            }
+            s_ml[tid] = make_float2(m, ok ? l : NAN);
+            __syncwarp();
+            cluster_sync();
+            // what each share counts (over the scales, which are behind us), then four numbers of a row at a time, eight such in flight
+            const int from = kTiles * kRowsTile * split / p.n_splits, rows = kTiles * kRowsTile * (split + 1) / p.n_splits - from;
+            const uint32_t at0 = umma::smem_addr(s_k), ml0 = umma::smem_addr(s_ml) + 8 * from;
+            float* factor_of = reinterpret_cast<float*>(s_q);         // [row][share]
+            if (tid < rows) {
+                float2 ml[kMaxCluster];
+                float best = kNoRef, sum = 0.f;
+#pragma unroll
+                for (int k = 0; k < kMaxCluster; ++k) {
+                    ml[k] = k < p.n_splits ? peer_f32x2(ml0 + 8 * tid, k) : make_float2(kNoRef, 0.f);
+                    best = fmaxf(best, ml[k].x);
+                }
+#pragma unroll
+                for (int k = 0; k < kMaxCluster; ++k) {
+                    ml[k].y *= ex2(ml[k].x - best);
+                    sum += ml[k].y;
+                }
+                const float part = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+                for (int k = 0; k < kMaxCluster; ++k)
+                    if (k < p.n_splits) factor_of[tid * kMaxCluster + k] = ml[k].y * part;
+            }
+            asm volatile("bar.sync 2, %0;" ::"n"(32 * kRowWarps) : "memory");
+            constexpr int kAtOnce = 8, kRowsOnce = 32 * kRowWarps / kFours;
+            const int piece = tid % kFours;
+            for (int r0 = tid / kFours; r0 < rows; r0 += kAtOnce * kRowsOnce) {
+                float4 v[kAtOnce];
+#pragma unroll
+                for (int x = 0; x < kAtOnce; ++x) v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int k = 0; k < p.n_splits; ++k) {
+                    float4 y[kAtOnce];
+#pragma unroll
+                    for (int x = 0; x < kAtOnce; ++x) {
+                        const int r = from + min(r0 + x * kRowsOnce, rows - 1);
+                        y[x] = peer_f32x4(at0 + 16 * (r * kFours + (piece ^ (r & (kFours - 1)))), k);
+                    }
+#pragma unroll
+                    for (int x = 0; x < kAtOnce; ++x) {
+                        const float w = factor_of[min(r0 + x * kRowsOnce, rows - 1) * kMaxCluster + k];
+                        v[x].x = fmaf(y[x].x, w, v[x].x), v[x].y = fmaf(y[x].y, w, v[x].y), v[x].z = fmaf(y[x].z, w, v[x].z), v[x].w = fmaf(y[x].w, w, v[x].w);
                     }
                 }
-                __syncwarp();
 #pragma unroll
-                for (int i = 0; i < kPieces; ++i) {
-                    const int r = (32 / kPieces) * i + lane / kPieces, piece = lane % kPieces, in_tile = lane0 + r;
-                    const int r_tok = tok0 + tile * p.tile_tokens + in_tile / p.G;
-                    const uint4 w = *reinterpret_cast<const uint4*>(stage + r * (kPieces * 16) + ((piece ^ r) & (kPieces - 1)) * 16);
-                    if (in_tile < p.tile_tokens * p.G && r_tok < p.tokens) *reinterpret_cast<uint4*>(where(kvh * p.G + in_tile % p.G, r_tok) + c0 + piece * kEach) = w;
+                for (int x = 0; x < kAtOnce; ++x) {
+                    T* dst = r0 + x * kRowsOnce < rows ? target(from + r0 + x * kRowsOnce) : nullptr;
+                    if (dst != nullptr) *reinterpret_cast<uint2*>(dst + 4 * piece) = make_uint2(pack_as<T>(v[x].x, v[x].y), pack_as<T>(v[x].z, v[x].w));
                 }
             }
-        };
-        if (p.n_splits > 1) {
-            leave(0.f, [&](int h, int k) { return p.o_part + (split * n_vec + ((long long)b * p.tokens + k) * (p.H * p.G) + h) * D; });
-            if (real) p.ml_part[split * n_vec + ((long long)b * p.tokens + tok) * (p.H * p.G) + head] = make_float2(m, ok ? l : NAN);
-        } else {
-            leave(T(), [&](int h, int k) { return static_cast<T*>(p.out.data) + b * p.out.seq + (long long)h * p.out.head + (long long)k * p.out.token; });
         }
+    }
+    if constexpr (kShared) {
+        __syncwarp();
+        if (warp >= kRowWarps) cluster_sync();
+        cluster_sync();                                // nobody leaves while its sums are read
     }
     if (warp >= kRowWarps && !ok && lane == 0) atomicOr(p.status, kTimedOut);
     umma::fence_before_sync();
@@ -470,47 +563,37 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
     }
 }
 
-// The shares of a row's keys, in order; a thread has four numbers.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) join_kernel(const PromptParams p) {
-    pdl_begin();
-    const long long n_vec = (long long)p.B * p.tokens * (p.H * p.G);
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, vec = i / (D / 4);
-    const int d4 = (int)(i % (D / 4));
-    if (vec >= n_vec) return;
-    float top = kNoRef;
-    for (int s = 0; s < p.n_splits; ++s) top = fmaxf(top, p.ml_part[s * n_vec + vec].x);
-    float sum = 0.f;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < p.n_splits; ++s) {
-        const float2 ml = p.ml_part[s * n_vec + vec];
-        const float w = ml.y * ex2(ml.x - top);
-        const float4 o = *reinterpret_cast<const float4*>(p.o_part + (s * n_vec + vec) * D + 4 * d4);
-        sum += w;
-        v.x = fmaf(o.x, w, v.x), v.y = fmaf(o.y, w, v.y), v.z = fmaf(o.z, w, v.z), v.w = fmaf(o.w, w, v.w);
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int heads = p.H * p.G, head = (int)(vec % heads);
-    const long long tok = vec / heads % p.tokens, b = vec / heads / p.tokens;
-    T* dst = static_cast<T*>(p.out.data) + b * p.out.seq + head * p.out.head + tok * p.out.token + 4 * d4;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_as<T>(v.x * inv, v.y * inv), pack_as<T>(v.z * inv, v.w * inv));
-}
-
-template <typename T, int D>
-int launch(const PromptParams& p, int blocks, cudaStream_t st) {
+int launch(PromptParams p, int blocks, int most_splits, cudaStream_t st) {
     static std::atomic<unsigned long long> ready{0};             // a bit for each device
+    static int rooms[64][kMaxCluster + 1];                       // clusters of so many CTAs that a device holds at once
     int dev = 0;
     LEANKV_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64) return LEANKV_ELIMIT;
     if (((ready.load(std::memory_order_acquire) >> dev) & 1ull) == 0) {
-        LEANKV_CUDA_TRY(cudaFuncSetAttribute(prompt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(D)));
+        LEANKV_CUDA_TRY(cudaFuncSetAttribute(prompt_kernel<T, D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(D)));
+        LEANKV_CUDA_TRY(cudaFuncSetAttribute(prompt_kernel<T, D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(D)));
+        for (int i = 2; i <= kMaxCluster; ++i) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(1, 1, i);
+            cfg.blockDim = dim3(kThreads);
+            cfg.dynamicSmemBytes = smem_bytes(D);
+            cudaLaunchAttribute attr;
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = attr.val.clusterDim.y = 1, attr.val.clusterDim.z = i;
+            cfg.attrs = &attr, cfg.numAttrs = 1;
+            LEANKV_CUDA_TRY(cudaOccupancyMaxActiveClusters(&rooms[dev][i], prompt_kernel<T, D, true>, &cfg));
+        }
         ready.fetch_or(1ull << dev, std::memory_order_release);
     }
-    LEANKV_CUDA_TRY(launch_early(prompt_kernel<T, D>, dim3((unsigned)(p.H * p.B), (unsigned)blocks, (unsigned)p.n_splits), dim3(kThreads), smem_bytes(D), st, p));
-    if (p.n_splits > 1) {
-        const long long work = (long long)p.B * p.tokens * p.H * p.G * (D / 4);
-        LEANKV_CUDA_TRY(launch_early(join_kernel<T, D>, dim3((unsigned)((work + 255) / 256)), dim3(256), 0, st, p));
-    }
+    // as many CTAs share a block's keys as leave the launch in one wave
+    const long long units = (long long)p.H * p.B * blocks;
+    p.n_splits = 1;
+    for (int i = 2; i <= std::min(kMaxCluster, most_splits); ++i)
+        if (units <= rooms[dev][i]) p.n_splits = i;
+    const dim3 grid((unsigned)(p.H * p.B), (unsigned)blocks, (unsigned)p.n_splits);
+    if (p.n_splits == 1) LEANKV_CUDA_TRY(launch_early(prompt_kernel<T, D, false>, grid, dim3(kThreads), smem_bytes(D), st, p));
+    else LEANKV_CUDA_TRY(launch_cluster_kernel_ex(true, dim3(1, 1, p.n_splits), prompt_kernel<T, D, true>, grid, dim3(kThreads), smem_bytes(D), st, p));
     return LEANKV_OK;
 }
 
@@ -533,15 +616,10 @@ extern "C" int leankv_byte_prompt_attn(const leankv_byte_attn_t* a, void* stream
     p.indptr = a->kv_indptr, p.indices = a->kv_page_indices, p.last = a->kv_last_page_len;
     p.status = static_cast<int*>(a->workspace);
     const long long blocks = ((long long)p.tokens + bytes::kTiles * p.tile_tokens - 1) / (bytes::kTiles * p.tile_tokens);
-    const long long ctas = blocks * p.H * p.B;
     if (blocks > 65535 || (long long)p.H * p.B > 0x7fffffffll) return LEANKV_ELIMIT;
-    // fewer CTAs than SMs share the keys, four key tiles each at least; the partial sums of so many CTAs fit the workspace
-    const long long key_tiles = ((long long)a->max_pages_seq + bytes::kPagesTile - 1) / bytes::kPagesTile;
-    const long long room = std::min(sm_count(), bytes::kPromptCtas) / ctas;
-    p.n_splits = (int)std::max(1ll, std::min({room, key_tiles / 4, 16ll}));
-    p.ml_part = reinterpret_cast<float2*>(static_cast<uint8_t*>(a->workspace) + bytes::kPartialsAt);
-    p.o_part = reinterpret_cast<float*>(p.ml_part + (size_t)bytes::kPromptCtas * bytes::kPromptRows);
+    // CTAs that share the keys have four key tiles each at least
+    const int most_splits = (int)(std::min(((long long)a->max_pages_seq + bytes::kPagesTile - 1) / bytes::kPagesTile / 4, 64ll));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (a->pool.dim == 128) return a->dtype == LEANKV_BYTES_F16 ? bytes::launch<__half, 128>(p, (int)blocks, st) : bytes::launch<bf16, 128>(p, (int)blocks, st);
-    return a->dtype == LEANKV_BYTES_F16 ? bytes::launch<__half, 64>(p, (int)blocks, st) : bytes::launch<bf16, 64>(p, (int)blocks, st);
+    if (a->pool.dim == 128) return a->dtype == LEANKV_BYTES_F16 ? bytes::launch<__half, 128>(p, (int)blocks, most_splits, st) : bytes::launch<bf16, 128>(p, (int)blocks, most_splits, st);
+    return a->dtype == LEANKV_BYTES_F16 ? bytes::launch<__half, 64>(p, (int)blocks, most_splits, st) : bytes::launch<bf16, 64>(p, (int)blocks, most_splits, st);
 }

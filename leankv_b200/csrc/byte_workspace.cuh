@@ -14,12 +14,7 @@ constexpr size_t kPartialsAt = 4 * ((size_t)kStatusWords + kCounters);
 // Few query tokens: a partial result of up to 16 rows for each part of a triple.
 constexpr int kMaxParts = kCounters;
 __host__ __device__ constexpr size_t partial_floats(int dim, int rows) { return (size_t)rows * (dim + 2); }
-// Prompts: one of 256 rows for each CTA of a launch that splits its keys.
-constexpr int kPromptCtas = 160, kPromptRows = 256;
-
-constexpr size_t larger(size_t a, size_t b) { return a > b ? a : b; }
-constexpr size_t kWorkspaceBytes =
-    kPartialsAt + 4 * larger((size_t)kMaxParts * partial_floats(128, 16), (size_t)kPromptCtas * partial_floats(128, kPromptRows));
+constexpr size_t kWorkspaceBytes = kPartialsAt + 4 * (size_t)kMaxParts * partial_floats(128, 16);
 
 }  // namespace bytes
 }  // namespace leankv
