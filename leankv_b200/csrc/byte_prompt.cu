@@ -7,7 +7,7 @@
 //   warp 12       S_r = Q_r K^T and O_r += P_r V of both row tiles, one thread issues
 //   warps 0 - 7   a thread a row: scores from tensor memory, maximum, weights back over the scores as fp16
 // A row's 128 scores stay in registers, which the row warps take from the others (of the launch's 128 each: 184, converting warps 96, the last four 48).
-// The row tiles alternate: the products of one run under the exponentials of the other. Tensor memory: S of both (128 columns each), O of both (dim each).
+// The row tiles alternate: the products of one run under the exponentials of the other. Tensor memory: S of both (128 columns each), O of both (dim each), for dim 64 weights.
 //
 // Exactness. Keys enter as their codes (the scale, one number for 16 keys, is multiplied to the scores in fp32), queries in fp16 with a power of two taken out
 // of each row. Values enter as code * 2^(e - r), r the largest exponent among the CTA's pages: exact down to 2^-24, and a page whose numbers are 2^-25 of
@@ -17,7 +17,7 @@
 // Bound: a key tile is 4 x 512 tensor cycles (dim 128) and 2 x 1024 cycles of ex2; operand reads (192 KB) and the converted tiles (64 KB written) take the
 // same time of shared memory's 128 bytes a cycle. It takes some 3600: a row tile's rows have 128 scores for 2400 cycles and then nothing for 1250, until the last weights
 // are multiplied (400) and the next scores formed over them (580, and 270 on the way); two row tiles are what tensor memory holds, and what one leaves the other does not fill.
-// 4096 tokens, 8 kv heads of 4, bf16: 142 us, 970 TFLOP/s; 8192: 489, 1124; 512 behind 3584: 47.8; dim 64, 4096: 123.
+// 4096 tokens, 8 kv heads of 4, bf16: 139 us, 990 TFLOP/s; 8192: 481, 1143; 512 behind 3584: 46.8; dim 64, 4096: 117.
 //
 // Long caches behind few rows: a cluster's CTAs share the keys of a block of rows, each leaves its sums in its shared memory, and each joins a part of the rows from there
 // (through the workspace and a second kernel: 512 behind 3584 52.4 us).
@@ -61,7 +61,7 @@ struct PromptParams {
     int* status;
 };
 
-enum { kQFull, kKFull = kQFull + 2, kVFull = kKFull + 2, kKFree = kVFull + 2, kVFree = kKFree + 2, kSFull = kVFree + 2, kPHalf = kSFull + 2, kPFull = kPHalf + 2, kPvDone = kPFull + 2, kBars = kPvDone + 2 };
+enum { kQFull, kKFull = kQFull + 2, kVFull = kKFull + 2, kKFree = kVFull + 2, kVFree = kKFree + 2, kSFull = kVFree + 2, kPHalf = kSFull + 2, kPFull = kPHalf + 2, kSRead = kPFull + 2, kPvDone = kSRead + 2, kBars = kPvDone + 2 };
 
 // Codes of a word's bytes 0, 1 / 2, 3 times s: (1024 + byte) s - 1152 s in one rounding of an exact number.
 __device__ __forceinline__ uint32_t codes_times(uint32_t w, uint32_t sel, __half2 s, __half2 off) {
@@ -112,7 +112,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
     __syncthreads();
     umma::fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
-    const uint32_t tm_s = tmem, tm_o = tmem + 2 * kKeysTile;
+    // dim 64 leaves room for weights of their own: the next scores need not wait for the value product (4096 tokens 123 -> 117 us)
+    constexpr bool kApart = D == 64;
+    constexpr int kPColumns = kApart ? kKeysTile / 2 : kKeysTile;
+    const uint32_t tm_s = tmem, tm_o = tmem + kTiles * kKeysTile, tm_p = kApart ? tm_o + kTiles * D : tm_s;
 
     const int kvh = blockIdx.x % p.H, b = blockIdx.x / p.H, split = kShared ? blockIdx.z : 0;
     const int ip = p.indptr[b], pages = p.indptr[b + 1] - ip;
@@ -143,6 +146,25 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
                 }
                 __syncwarp();
             };
+            auto values = [&](int r, int j) {              // both parts of a row tile's weights
+                const uint64_t c = umma::desc_k(umma::smem_addr(s_v + (j & 1) * k_bytes(D)), kKeysTile / 8);
+#pragma unroll
+                for (int part = 0; part < 2; ++part) {
+                    ok = ok && all(wait1((part == 0 ? kPHalf : kPFull) + r, j));
+                    if (!ok) return;
+                    umma::fence_after_sync();
+                    if (umma::elect()) {
+#pragma unroll
+                        for (int ks = part * 6; ks < 6 + part * 2; ++ks)
+                            umma::mma_f16_ts(tm_o + r * D, tm_p + r * kPColumns + 8 * ks, c + (uint64_t)ks * (2 * umma::kLbo >> 4), umma::idesc_n(D), j > 0 || ks > 0);
+                        if (part == 1) {
+                            umma::commit(bar(kPvDone + r));
+                            if (r == kTiles - 1 && j + 2 < n) umma::commit(bar(kVFree + (j & 1)));
+                        }
+                    }
+                    __syncwarp();
+                }
+            };
             if (n > 0) ok = all(wait2(kKFull, 0));
             for (int r = 0; r < kTiles && ok && n > 0; ++r) {
                 ok = all(wait1(kQFull + r, 0));
@@ -150,36 +172,31 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
                 if (ok) scores(r, 0);
             }
             for (int j = 0; j < n && ok; ++j) {
-                ok = all(wait2(kVFull, j));
                 for (int r = 0; r < kTiles && ok; ++r) {
-                    const uint64_t c = umma::desc_k(umma::smem_addr(s_v + (j & 1) * k_bytes(D)), kKeysTile / 8);
-#pragma unroll
-                    for (int part = 0; part < 2; ++part) {
-                        ok = ok && all(wait1((part == 0 ? kPHalf : kPFull) + r, j));
-                        if (!ok) break;
-                        umma::fence_after_sync();
-                        if (umma::elect()) {
-#pragma unroll
-                            for (int ks = part * 6; ks < 6 + part * 2; ++ks)
-                                umma::mma_f16_ts(tm_o + r * D, tm_s + r * kKeysTile + 8 * ks, c + (uint64_t)ks * (2 * umma::kLbo >> 4), umma::idesc_n(D), j > 0 || ks > 0);
-                            if (part == 1) {
-                                umma::commit(bar(kPvDone + r));
-                                if (r == kTiles - 1 && j + 2 < n) umma::commit(bar(kVFree + (j & 1)));
-                            }
-                        }
-                        __syncwarp();
-                    }
-                    if (!ok) break;
-                    if (j + 1 < n) {                       // its scores go over these weights
-                        if (r == 0) ok = all(wait2(kKFull, j + 1));
-                        ok = ok && all(wait1(kPvDone + r, j));
-                        if (ok) {
+                    if constexpr (kApart) {                // as soon as the ones before have been read; then the other row tile's weights
+                        if (j + 1 < n) {
+                            if (r == 0) ok = all(wait2(kKFull, j + 1));
+                            ok = ok && all(wait1(kSRead + r, j));
                             umma::fence_after_sync();
-                            scores(r, j + 1);
+                            if (ok) scores(r, j + 1);
+                        }
+                        const int vr = 1 - r, vj = j - vr;
+                        if (vj < 0 || !ok) continue;
+                        if (vr == 0) ok = all(wait2(kVFull, vj));
+                        values(vr, vj);
+                    } else {
+                        if (r == 0) ok = all(wait2(kVFull, j));
+                        values(r, j);
+                        if (ok && j + 1 < n) {             // its scores go over these weights
+                            if (r == 0) ok = all(wait2(kKFull, j + 1));
+                            ok = ok && all(wait1(kPvDone + r, j));
+                            umma::fence_after_sync();
+                            if (ok) scores(r, j + 1);
                         }
                     }
                 }
             }
+            if (kApart && ok && n > 0) values(1, n - 1);
         }
     } else if (warp >= kRowWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
@@ -358,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
         float m = kNoRef, l = 0.f;
         const int lane0 = 32 * (warp & 3);
         const int qpos = start + (real ? tok : last_tok);       // rows that are none see what the last token sees; nothing of theirs is kept
-        const uint32_t tm = tm_s + tile * kKeysTile, to = tm_o + tile * D;
+        const uint32_t tm = tm_s + tile * kKeysTile, tp = tm_p + tile * kPColumns, to = tm_o + tile * D;
         for (int j = 0; j < n && ok; ++j) {
             ok = all(wait1(kSFull + tile, j));
             if (!ok) break;
@@ -377,6 +394,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
             umma::settled(s[1]);
             umma::settled(s[2]);
             umma::settled(s[3]);
+            if constexpr (kApart) {
+                umma::fence_before_sync();
+                umma::bar_arrive(bar(kSRead + tile));
+            }
             const int k1 = qpos - (t0 + j) * kKeysTile;                  // the row's last key of the tile
             const bool cut = __any_sync(0xffffffffu, k1 < kKeysTile - 1);
             if (cut) {
@@ -394,6 +415,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
                 a = largest3(__float_as_uint(a), v[6], v[7]), c = largest3(__float_as_uint(c), v[8], v[9]);
                 a = largest3(__float_as_uint(a), v[10], v[11]), c = largest3(__float_as_uint(c), v[12], v[13]);
                 best = fmaxf(best, largest3(__float_as_uint(a), __float_as_uint(c), __float_as_uint(fmaxf(__uint_as_float(v[14]), __uint_as_float(v[15])))) * ks[i]);
+            }
+            if constexpr (kApart) {                    // neither outputs nor weights are in use any more
+                if (j > 0) ok = all(wait1(kPvDone + tile, j - 1));
+                umma::fence_after_sync();
             }
             const bool raise = best > m + kReach;
             if (__any_sync(0xffffffffu, raise)) {
@@ -423,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
                         const __half2 h = __floats2half2_rn(w.x, w.y);
                         w16[x / 2] = *reinterpret_cast<const uint32_t*>(&h);
                     }
-                    umma::st16_async(w16, tm, lane0, 16 * c);
+                    umma::st16_async(w16, tp, lane0, 16 * c);
                     if (c == 2) {                      // the first 96 keys' product begins (64: 157 us where this takes 154)
                         umma::stored();
                         umma::fence_before_sync();
