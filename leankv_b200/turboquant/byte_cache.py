@@ -109,7 +109,7 @@ class ByteKVCache(PagedKVCache):
             # (arguments, what a call passes, its tensors)
             self._args.append(((append, byref(append), append.k, append.v), (attn, byref(attn), attn.q, attn.out), (select, byref(select), select.q)))
         self._device_index = self.kv_data.get_device()
-        self._lib = _native.byte_lib()
+        self._lib, self._table_lib = _native.byte_lib(), _native.lib()
         self._captured = False                # an attention call was: graphs may be replayed
         self._earlier_tables = []
         self._alloc_tables(0)
@@ -123,16 +123,21 @@ class ByteKVCache(PagedKVCache):
             for a in args:
                 a[0].kv_indptr, a[0].kv_page_indices = self._kv_indptr.data_ptr(), self._kv_page_indices.data_ptr()
             args[0][0].kv_last_page_len = args[1][0].kv_last_page_len = self._kv_last.data_ptr()
-        self._step_args = (self._seq_len_dev.data_ptr(), self._block_table.data_ptr(), self._pps_cap, self._free_stack.data_ptr(),
-                           self._free_top.data_ptr(), self._kv_indptr.data_ptr(), self._kv_page_indices.data_ptr(),
-                           self._kv_last.data_ptr(), self._start_dev.data_ptr(), self._status.data_ptr())
+        at = lambda t: ctypes.c_void_p(t.data_ptr())      # converted once, not at every call
+        self._step_args = (at(self._seq_len_dev), at(self._block_table), ctypes.c_int(self._pps_cap), at(self._free_stack), at(self._free_top),
+                           at(self._kv_indptr), at(self._kv_page_indices), at(self._kv_last), at(self._start_dev), at(self._status))
 
     def _table_step(self, t_new: int, batch: int):
         with _native.on_device(self._device):
-            rc = _native.lib().leankv_paged_table_step(t_new, batch, *self._step_args, _native.current_stream())
-        _native.check(rc, "leankv_paged_table_step")
-        # what a graph records has not been built yet
-        self._meta_batch = -1 if self._device.type == "cuda" and _capturing() else batch
+            self._step(t_new, batch, _native.current_stream())
+        if self._device.type == "cuda" and _capturing():
+            self._meta_batch = -1                         # what a graph records has not been built yet
+
+    def _step(self, t_new: int, batch: int, stream: int):
+        rc = self._table_lib.leankv_paged_table_step(t_new, batch, *self._step_args, stream)
+        if rc:
+            _native.check(rc, "leankv_paged_table_step")
+        self._meta_batch = batch
 
     def _device_meta(self, batch_size: int):
         """(kv_indptr, kv_page_indices, kv_last_page_len) int32 on the device, for all known sequences: the first ones' part is the same
@@ -186,10 +191,10 @@ class ByteKVCache(PagedKVCache):
             v = v.to(k.dtype)
         if t_new == 0:
             return
+        if _capturing():
+            raise RuntimeError("ByteKVCache: append goes by lengths that the host keeps, too, and cannot be captured")
         known = self._seq_lengths
         if layer_idx == 0:
-            if _capturing():
-                raise RuntimeError("ByteKVCache: append advances lengths that the host keeps, too, and cannot be captured")
             lengths = known[:batch] + [0] * (batch - len(known))
             if t_new == 1:
                 need = [n % PAGE for n in lengths].count(0)
@@ -200,20 +205,22 @@ class ByteKVCache(PagedKVCache):
                                    f"Increase max_pages or reduce batch/sequence length.")
             if len(known) < batch:
                 self._ensure_batch_size(batch)
-            self._table_step(t_new, batch)
-            self._seen_tokens += t_new
-            self._free_count -= need
-            known[:batch] = [n + t_new for n in lengths]
-            if batch < len(known):
-                self._table_step(0, len(known))
         elif len(known) < batch or min(known[:batch]) < t_new:
             raise RuntimeError("ByteKVCache: layer 0 has not appended these tokens yet")
-        if self._meta_batch < batch:
+        elif self._meta_batch < batch:
             self._device_meta(batch)
         args.dtype, args.batch, args.tokens = _TYPES[k.dtype], batch, t_new
         k, v = _point(kp, k), _point(vp, v)
         with _native.on_device(self._device):
-            rc = self._lib.leankv_byte_append(call, _native.current_stream())
+            stream = _native.current_stream()
+            if layer_idx == 0:
+                self._step(t_new, batch, stream)
+                self._seen_tokens += t_new
+                self._free_count -= need
+                known[:batch] = [n + t_new for n in lengths]
+                if batch < len(known):
+                    self._step(0, len(known), stream)
+            rc = self._lib.leankv_byte_append(call, stream)
         if rc:
             _native.check(rc, "leankv_byte_append", self._lib)
 

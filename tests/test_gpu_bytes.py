@@ -582,6 +582,22 @@ def test_a_replay_answers_for_the_lengths_that_the_sequences_have_by_then():
     close(one, p.plain.attend(0, new[0, :, None])[:, 0][None], BF16)
 
 
+def test_no_layer_appends_inside_a_capture():
+    cache = ByteKVCache(num_layers=2, num_kv_heads=1, num_q_heads=1, head_dim=64, max_pages=4, dtype=F16, device=DEV)
+    k = vectors(torch.Generator().manual_seed(4), 1, 1, 3, 64, F16).to(DEV)
+    for layer in range(2):
+        cache.append(layer, k, k)
+    before = cache.kv_data.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        doubled = k * 2
+        for layer in range(2):
+            with pytest.raises(RuntimeError, match="captured"):
+                cache.append(layer, doubled, doubled)
+    graph.replay()
+    assert torch.equal(cache.kv_data, before) and cache.get_seq_length() == 3
+
+
 def test_a_reset_is_not_captured():
     cache = ByteKVCache(num_layers=1, num_kv_heads=1, num_q_heads=1, max_pages=4, dtype=F16, device="cuda")
     k = vectors(torch.Generator().manual_seed(3), 1, 1, 20, 128, F16).to(DEV)
