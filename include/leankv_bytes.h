@@ -1,6 +1,6 @@
 /*
  * leankv_bytes — C ABI of the paged cache that holds keys and values in 8 bits, and of the attention over it
- * (libleankv_bytes.so, sm_100a). The reference project has no cache of this kind: its paged cache keeps fp16 pages for FlashInfer
+ * (libleankv_bytes.so, sm_100a). The reference project has no cache of this kind: its paged cache keeps fp16 pages
  * (leankv/turboquant/paged_cache.py) and its quantized one 3-bit codes (leankv/turboquant/cache.py). Conventions (device
  * pointers, ownership, streams, status codes, page table) are those of leankv_b200.h.
  *

@@ -99,9 +99,10 @@ class ByteKVCache(PagedKVCache):
         # 8 after 8000, 8 thousand, 26 / 27; 16 after 8000, 16 thousand, 36 / 27; 128 after none, 2 thousand, 9 / 13)
         self._prompt_work = 10_000
         # the calls' arguments, one set for each layer: a call fills in what changes
-        self._args = []
+        self._args, self._pools = [], []
         for i in range(num_layers):
             pool = _native.BytePool(head_dim, num_kv_heads, max_pages, self.kv_data[i].data_ptr(), self.bounds[i].data_ptr())
+            self._pools.append(byref(pool))
             append = _native.ByteAppend(pool=pool)
             attn = _native.ByteAttn(pool=pool, q_heads=num_q_heads, scale=1.0 / math.sqrt(head_dim), workspace=self._workspace.data_ptr(),
                                     workspace_bytes=size)
@@ -126,6 +127,12 @@ class ByteKVCache(PagedKVCache):
         at = lambda t: ctypes.c_void_p(t.data_ptr())      # converted once, not at every call
         self._step_args = (at(self._seq_len_dev), at(self._block_table), ctypes.c_int(self._pps_cap), at(self._free_stack), at(self._free_top),
                            at(self._kv_indptr), at(self._kv_page_indices), at(self._kv_last), at(self._start_dev), at(self._status))
+        # an empty table: the status word, the free stack and its height lie one behind the other; before them the flat arrays and the lengths, as long as there
+        # was never more than one sequence
+        self._lengths_too = self._batch_cap == 1
+        first = self._seq_len_dev if self._lengths_too else self._status
+        zeros = (self._free_stack.data_ptr() - first.data_ptr()) // 4
+        self._begin_args = (at(first), zeros, self.max_pages, zeros + -(-self.max_pages // 4) * 4)
 
     def _table_step(self, t_new: int, batch: int):
         with _native.on_device(self._device):
@@ -226,16 +233,20 @@ class ByteKVCache(PagedKVCache):
 
     def _gather_kv(self, layer_idx: int, batch_size: int):
         """Dense ``[B, Hkv, max_seq, D]`` K and V in the cache's type (zeros behind a sequence's last token)."""
-        pool, lib = self._layer(layer_idx)[0][0].pool, self._lib
-        max_seq = max(self._seq_lengths[:batch_size], default=0)
+        self._layer(layer_idx)
+        lengths = self._seq_lengths[:batch_size]
+        max_seq = max(lengths) if lengths else 0
         shape = (batch_size, self.num_kv_heads, max_seq, self.head_dim)
-        keys, values = (torch.empty(shape, dtype=self._dtype, device=self._device) for _ in range(2))
+        keys = torch.empty(shape, dtype=self._dtype, device=self._device)
+        values = torch.empty_like(keys)
         if batch_size and max_seq:
-            indptr, flat, last = self._device_meta(batch_size)
+            if self._meta_batch < batch_size:
+                self._device_meta(batch_size)
             with _native.on_device(self._device):
-                rc = lib.leankv_byte_unpack(byref(pool), _TYPES[self._dtype], keys.data_ptr(), values.data_ptr(), batch_size, max_seq,
-                                            indptr.data_ptr(), flat.data_ptr(), last.data_ptr(), _native.current_stream())
-            _native.check(rc, "leankv_byte_unpack", lib)
+                rc = self._lib.leankv_byte_unpack(self._pools[layer_idx], _TYPES[self._dtype], keys.data_ptr(), values.data_ptr(), batch_size, max_seq,
+                                                  *self._step_args[5:8], _native.current_stream())
+            if rc:
+                _native.check(rc, "leankv_byte_unpack", self._lib)
         return keys, values
 
     def unpack_sequence(self, layer_idx: int, batch_idx: int, which: int):
@@ -373,15 +384,10 @@ class ByteKVCache(PagedKVCache):
             return super().reset()
         if _capturing():
             raise RuntimeError("ByteKVCache: reset changes lengths that the host keeps, too, and cannot be captured")
-        # the status word, the free stack and its height lie one behind the other; before them the flat arrays and the lengths, as long as there was
-        # never more than one sequence
-        whole = self._batch_cap == 1
-        at = (self._seq_len_dev if whole else self._status).data_ptr()
-        zeros = (self._free_stack.data_ptr() - at) // 4
         with _native.on_device(self._device):
-            rc = _native.lib().leankv_paged_table_begin(at, zeros, self.max_pages, zeros + -(-self.max_pages // 4) * 4, _native.current_stream())
+            rc = self._table_lib.leankv_paged_table_begin(*self._begin_args, _native.current_stream())
         _native.check(rc, "leankv_paged_table_begin")
-        if not whole:
+        if not self._lengths_too:
             self._seq_len_dev.zero_()
             if self._captured and self._seq_lengths:
                 self._table_step(0, len(self._seq_lengths))
@@ -395,6 +401,11 @@ class ByteKVCache(PagedKVCache):
         raise RuntimeError("ByteKVCache keeps its sequences in their places: no beams, repeated or chosen rows")
 
     batch_repeat_interleave = batch_select_indices = reorder_cache = _one_row_each
+
+    def _not_copied(self, *args):
+        raise RuntimeError("ByteKVCache cannot be copied: its page table lies on the device")
+
+    __copy__ = __deepcopy__ = __reduce_ex__ = _not_copied
 
     # ── diagnostics ────────────────────────────────────────────────────
 

@@ -1,8 +1,10 @@
 """The 8-bit paged cache on the CPU: its format's definition, the C ABI's checks, and the arguments that Python refuses."""
 
+import copy
 import ctypes
 import math
 import os
+import pickle
 import re
 
 import pytest
@@ -81,6 +83,13 @@ def test_rows_that_would_have_to_move_are_refused():
     for call in (lambda: cache.reorder_cache(torch.tensor([0])), lambda: cache.batch_repeat_interleave(2), lambda: cache.batch_select_indices(torch.tensor([0]))):
         with pytest.raises(RuntimeError, match="places"):
             call()
+
+
+def test_a_cache_is_not_copied():
+    cache = _cpu_cache()
+    for copied in (copy.copy, copy.deepcopy, pickle.dumps):
+        with pytest.raises(RuntimeError, match="copied"):
+            copied(cache)
 
 
 def test_vectors_are_read_where_they_are_or_copied():
