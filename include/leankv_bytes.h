@@ -61,7 +61,7 @@ typedef struct {
 int leankv_byte_append(const leankv_byte_append_t* a /* host */, void* stream);
 
 /* The stored numbers of the first T positions of B sequences, as `dtype`: k_out, v_out [B][kv_heads][T][dim], zeros behind a sequence's
- * last token. A number beyond the type's range becomes its largest one. */
+ * last token; 16-byte aligned, fp32 32-byte. A number beyond the type's range becomes its largest one. */
 int leankv_byte_unpack(const leankv_byte_pool_t* pool /* host */, int dtype, void* k_out, void* v_out, int B, int T,
                        const int32_t* kv_indptr, const int32_t* kv_page_indices, const int32_t* kv_last_page_len, void* stream);
 

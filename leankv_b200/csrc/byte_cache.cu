@@ -165,8 +165,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, bf16) { return pack_
 template <typename T>
 __device__ __forceinline__ void store8(T* to, const float (&v)[8]) {
     if constexpr (std::is_same<T, float>::value) {
-        reinterpret_cast<float4*>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        // a whole 32-byte sector of a lane at once (as two halves: 16 x 2011 tokens 69 us, so 54)
+        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
     } else {
         *reinterpret_cast<uint4*>(to) = make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()), pack2(v[4], v[5], T()), pack2(v[6], v[7], T()));
     }
@@ -263,7 +263,8 @@ extern "C" int leankv_byte_unpack(const leankv_byte_pool_t* pool, int dtype, voi
     if (!bytes::good_pool(pool) || !bytes::good_type(dtype) || !k_out || !v_out || B <= 0 || T <= 0 || !kv_indptr || !kv_page_indices || !kv_last_page_len)
         return LEANKV_EINVAL;
     if (B > LEANKV_BYTES_MAX_BATCH) return LEANKV_ELIMIT;
-    if (!bytes::aligned_pool(pool) || !aligned16(k_out) || !aligned16(v_out)) return LEANKV_EALIGN;
+    const uintptr_t loose = dtype == LEANKV_BYTES_F32 ? 31u : 15u;
+    if (!bytes::aligned_pool(pool) || ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & loose) != 0) return LEANKV_EALIGN;
     bytes::UnpackParams p = {};
     p.chunks = static_cast<const uint8_t*>(pool->chunks);
     p.H = pool->kv_heads, p.n_pages = pool->n_pages, p.B = B, p.T = T;

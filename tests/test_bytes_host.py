@@ -208,6 +208,13 @@ def test_append_and_unpack_check_their_arguments():
         assert f(**kw) == code, kw
 
 
+def test_dense_reads_check_where_they_write():
+    lib = _native.byte_lib()
+    f = lambda dtype, k, v: lib.leankv_byte_unpack(ctypes.byref(_pool()), dtype, k, v, 1, 1, 64, 64, 64, None)
+    for dtype, good in ((_native.BYTES_F16, 16), (_native.BYTES_BF16, 16), (_native.BYTES_F32, 32)):
+        assert f(dtype, 64 + good // 2, 64) == f(dtype, 64, 64 + good // 2) == -2
+
+
 def test_attention_checks_its_arguments():
     _no_gpu()
     lib = _native.byte_lib()
