@@ -17,10 +17,10 @@
 // Bound: a key tile is 4 x 512 tensor cycles (dim 128) and 2 x 1024 cycles of ex2; operand reads (192 KB) and the converted tiles (64 KB written) take the
 // same time of shared memory's 128 bytes a cycle. It takes some 3600: a row tile's rows have 128 scores for 2400 cycles and then nothing for 1250, until the last weights
 // are multiplied (400) and the next scores formed over them (580, and 270 on the way); two row tiles are what tensor memory holds, and what one leaves the other does not fill.
-// 4096 tokens, 8 kv heads of 4, bf16: 139 us, 990 TFLOP/s; 8192: 481, 1143; 512 behind 3584: 46.8; dim 64, 4096: 117.
+// 4096 tokens, 8 kv heads of 4, bf16: 139 us, 990 TFLOP/s; 8192: 481, 1143; 512 behind 3584: 48; dim 64, 4096: 117.
 //
 // Long caches behind few rows: a cluster's CTAs share the keys of a block of rows, each leaves its sums in its shared memory, and each joins a part of the rows from there
-// (through the workspace and a second kernel: 512 behind 3584 52.4 us).
+// (through the workspace and a second kernel: 512 behind 3584 52.4 us). Where a cluster of eight leaves SMs free several clusters share them, and their sums meet in the workspace.
 
 #include <algorithm>
 #include <atomic>
@@ -57,7 +57,9 @@ struct PromptParams {
     const int32_t* indptr;
     const int32_t* indices;
     const int32_t* last;
-    int n_splits;                                     // CTAs of a cluster, which share a block's keys
+    int n_splits, ctas;                               // shares of a block's keys; CTAs of a cluster. More shares than that are joined in the workspace
+    float* partials;                                  // [block of a kv head][cluster][256 rows][dim + 2]
+    unsigned* counters;                               // [block of a kv head][CTA of a cluster], zero between launches
     int* status;
 };
 
@@ -88,6 +90,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
     __shared__ int s_top[kConvWarps];
     __shared__ __align__(16) float s_ks[kScaleSlots][kPagesTile];
     __shared__ __align__(8) float2 s_ml[kTiles * kRowsTile];          // reference and sum of a row
+    __shared__ int s_last;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     uint8_t* base = s_raw + ((1024u - (umma::smem_addr(s_raw) & 1023u)) & 1023u);
     uint8_t* s_q = base;                              // two row tiles
@@ -524,16 +527,21 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
             s_ml[tid] = make_float2(m, ok ? l : NAN);
             __syncwarp();
             cluster_sync();
-            // what each share counts (over the scales, which are behind us), then four numbers of a row at a time, eight such in flight
-            const int from = kTiles * kRowsTile * split / p.n_splits, rows = kTiles * kRowsTile * (split + 1) / p.n_splits - from;
-            const uint32_t at0 = umma::smem_addr(s_k), ml0 = umma::smem_addr(s_ml) + 8 * from;
+            // what each share counts, then four numbers of a row at a time, eight such in flight. Rows that are none are left out
+            const int rank = split % p.ctas, group = split / p.ctas, groups = p.n_splits / p.ctas;
+            const int in_first = min(p.tile_tokens, last_tok + 1 - tok0) * p.G, in_all = (last_tok + 1 - tok0) * p.G;
+            const int from = in_all * rank / p.ctas, rows = in_all * (rank + 1) / p.ctas - from;
+            auto row_of = [&](int i) { return from + i < in_first ? from + i : kRowsTile + from + i - in_first; };
+            const uint32_t at0 = umma::smem_addr(s_k), ml0 = umma::smem_addr(s_ml);
             float* factor_of = reinterpret_cast<float*>(s_q);         // [row][share]
+            const int unit = blockIdx.x + blockIdx.y * gridDim.x;
+            float* partial = p.partials + (size_t)(unit * groups + group) * partial_floats(D, kTiles * kRowsTile);
             if (tid < rows) {
                 float2 ml[kMaxCluster];
                 float best = kNoRef, sum = 0.f;
 #pragma unroll
                 for (int k = 0; k < kMaxCluster; ++k) {
-                    ml[k] = k < p.n_splits ? peer_f32x2(ml0 + 8 * tid, k) : make_float2(kNoRef, 0.f);
+                    ml[k] = k < p.ctas ? peer_f32x2(ml0 + 8 * row_of(tid), k) : make_float2(kNoRef, 0.f);
                     best = fmaxf(best, ml[k].x);
                 }
 #pragma unroll
@@ -544,21 +552,27 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
                 const float part = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
                 for (int k = 0; k < kMaxCluster; ++k)
-                    if (k < p.n_splits) factor_of[tid * kMaxCluster + k] = ml[k].y * part;
+                    if (k < p.ctas) factor_of[tid * kMaxCluster + k] = ml[k].y * part;
+                if (groups > 1) reinterpret_cast<float2*>(partial + kTiles * kRowsTile * D)[from + tid] = make_float2(best, sum);
             }
             asm volatile("bar.sync 2, %0;" ::"n"(32 * kRowWarps) : "memory");
             constexpr int kAtOnce = 8, kRowsOnce = 32 * kRowWarps / kFours;
             const int piece = tid % kFours;
+            auto store = [&](int i, float4 v) {
+                T* dst = target(row_of(i));
+                if (dst != nullptr) *reinterpret_cast<uint2*>(dst + 4 * piece) = make_uint2(pack_as<T>(v.x, v.y), pack_as<T>(v.z, v.w));
+            };
             for (int r0 = tid / kFours; r0 < rows; r0 += kAtOnce * kRowsOnce) {
                 float4 v[kAtOnce];
 #pragma unroll
                 for (int x = 0; x < kAtOnce; ++x) v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (int k = 0; k < p.n_splits; ++k) {
+                for (int k = 0; k < p.ctas; ++k) {
                     float4 y[kAtOnce];
 #pragma unroll
                     for (int x = 0; x < kAtOnce; ++x) {
-                        const int r = from + min(r0 + x * kRowsOnce, rows - 1);
-                        y[x] = peer_f32x4(at0 + 16 * (r * kFours + (piece ^ (r & (kFours - 1)))), k);
+                        const int r = row_of(r0 + x * kRowsOnce);
+                        y[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (r0 + x * kRowsOnce < rows) y[x] = peer_f32x4(at0 + 16 * (r * kFours + (piece ^ (r & (kFours - 1)))), k);
                     }
 #pragma unroll
                     for (int x = 0; x < kAtOnce; ++x) {
@@ -568,8 +582,36 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
                 }
 #pragma unroll
                 for (int x = 0; x < kAtOnce; ++x) {
-                    T* dst = r0 + x * kRowsOnce < rows ? target(from + r0 + x * kRowsOnce) : nullptr;
-                    if (dst != nullptr) *reinterpret_cast<uint2*>(dst + 4 * piece) = make_uint2(pack_as<T>(v[x].x, v[x].y), pack_as<T>(v[x].z, v[x].w));
+                    const int i = r0 + x * kRowsOnce;
+                    if (i >= rows) continue;
+                    if (groups == 1) store(i, v[x]);
+                    else reinterpret_cast<float4*>(partial)[(from + i) * kFours + piece] = v[x];
+                }
+            }
+            if (groups > 1) {
+                // the clusters' sums: of the CTAs that have the same rows, the last one to come adds them up, in order
+                asm volatile("bar.sync 2, %0;" ::"n"(32 * kRowWarps) : "memory");
+                if (tid == 0) {
+                    unsigned* counter = p.counters + unit * kMaxCluster + rank;
+                    s_last = arrive(counter) == (unsigned)groups - 1;
+                    if (s_last) *counter = 0;
+                }
+                asm volatile("bar.sync 2, %0;" ::"n"(32 * kRowWarps) : "memory");
+                const float* first = p.partials + (size_t)unit * groups * partial_floats(D, kTiles * kRowsTile);
+                for (int i = s_last ? tid / kFours : rows; i < rows; i += kRowsOnce) {
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    float best = kNoRef, sum = 0.f;
+                    for (int k = 0; k < groups; ++k) {
+                        const float* there = first + (size_t)k * partial_floats(D, kTiles * kRowsTile);
+                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(there + kTiles * kRowsTile * D) + from + i);
+                        const float4 y = __ldcg(reinterpret_cast<const float4*>(there) + (from + i) * kFours + piece);
+                        const float now = fmaxf(best, ml.x), keep = ex2(best - now), w = ml.y * ex2(ml.x - now);
+                        best = now;
+                        sum = fmaf(sum, keep, w);
+                        v.x = fmaf(v.x, keep, y.x * w), v.y = fmaf(v.y, keep, y.y * w), v.z = fmaf(v.z, keep, y.z * w), v.w = fmaf(v.w, keep, y.w * w);
+                    }
+                    const float part = sum == 0.f ? 0.f : 1.f / sum;
+                    store(i, make_float4(v.x * part, v.y * part, v.z * part, v.w * part));
                 }
             }
         }
@@ -611,14 +653,17 @@ int launch(PromptParams p, int blocks, int most_splits, cudaStream_t st) {
         }
         ready.fetch_or(1ull << dev, std::memory_order_release);
     }
-    // as many CTAs share a block's keys as leave the launch in one wave
+    // as many CTAs share a block's keys as leave the launch in one wave: a cluster, or several of eight (8 tokens behind 8000, 8 kv heads: one 39 us, two 28;
+    // clusters of 16 43)
     const long long units = (long long)p.H * p.B * blocks;
-    p.n_splits = 1;
+    p.ctas = 1;
     for (int i = 2; i <= std::min(kMaxCluster, most_splits); ++i)
-        if (units <= rooms[dev][i]) p.n_splits = i;
+        if (units <= rooms[dev][i]) p.ctas = i;
+    const long long groups = p.ctas < kMaxCluster ? 1 : std::max(1ll, std::min((long long)rooms[dev][kMaxCluster] / units, (long long)most_splits / kMaxCluster));
+    p.n_splits = (int)(p.ctas * groups);
     const dim3 grid((unsigned)(p.H * p.B), (unsigned)blocks, (unsigned)p.n_splits);
-    if (p.n_splits == 1) LEANKV_CUDA_TRY(launch_early(prompt_kernel<T, D, false>, grid, dim3(kThreads), smem_bytes(D), st, p));
-    else LEANKV_CUDA_TRY(launch_cluster_kernel_ex(true, dim3(1, 1, p.n_splits), prompt_kernel<T, D, true>, grid, dim3(kThreads), smem_bytes(D), st, p));
+    if (p.ctas == 1) LEANKV_CUDA_TRY(launch_early(prompt_kernel<T, D, false>, grid, dim3(kThreads), smem_bytes(D), st, p));
+    else LEANKV_CUDA_TRY(launch_cluster_kernel_ex(true, dim3(1, 1, p.ctas), prompt_kernel<T, D, true>, grid, dim3(kThreads), smem_bytes(D), st, p));
     return LEANKV_OK;
 }
 
@@ -640,6 +685,8 @@ extern "C" int leankv_byte_prompt_attn(const leankv_byte_attn_t* a, void* stream
     p.scale = a->scale * bytes::kLog2e;
     p.indptr = a->kv_indptr, p.indices = a->kv_page_indices, p.last = a->kv_last_page_len;
     p.status = static_cast<int*>(a->workspace);
+    p.counters = reinterpret_cast<unsigned*>(p.status + bytes::kStatusWords);
+    p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + bytes::kPartialsAt);
     const long long blocks = ((long long)p.tokens + bytes::kTiles * p.tile_tokens - 1) / (bytes::kTiles * p.tile_tokens);
     if (blocks > 65535 || (long long)p.H * p.B > 0x7fffffffll) return LEANKV_ELIMIT;
     // CTAs that share the keys have four key tiles each at least

@@ -95,8 +95,9 @@ class ByteKVCache(PagedKVCache):
         size = _native.byte_lib().leankv_byte_attn_workspace_bytes() if self._device.type == "cuda" else 0
         self._workspace = torch.zeros(size, dtype=torch.uint8, device=self._device)
         # pages read by 16 (token, query head) rows at a time from which a chunk goes to the prompt kernel. Up to there the kernel for few tokens
-        # is faster (us, 8 kv heads of 4, few tokens' / prompt kernel: 32 tokens after 1000, 4 thousand of these pages, 17 / 24; 128 after 1000, 18 thousand, 30 / 27;
-        # 8 after 8000, 8 thousand, 26 / 27; 16 after 8000, 16 thousand, 36 / 27; 128 after none, 2 thousand, 9 / 13)
+        # is faster (us, 8 kv heads of 4, few tokens' / prompt kernel: 32 tokens after 1000, 4 thousand of these pages, 17 / 22; 64 after 1000, 9 thousand, 20 / 25; 128 after
+        # 1000, 18 thousand, 30 / 25; 8 after 8000, 8 thousand, 26 / 28; 16 after 8000, 16 thousand, 36 / 29). Where nothing is cached before them it is up to 4 us slower
+        # (256 after none, 8 thousand, 16 / 12)
         self._prompt_work = 10_000
         # the calls' arguments, one set for each layer: a call fills in what changes
         self._args, self._pools = [], []

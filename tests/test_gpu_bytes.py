@@ -321,6 +321,22 @@ def test_prompt_attention_over_several_tiles_and_shares(dtype, dim, group, heads
     assert all(torch.equal(p.cache.prefill_attention(0, q), first) for _ in range(3))
 
 
+@pytest.mark.parametrize("dtype, dim, group, heads, past, tokens", [
+    (F16, 128, 4, 1, 8200, 20), (BF16, 64, 7, 2, 16390, 40), (F16, 128, 16, 2, 9000, 9), (BF16, 128, 3, 1, 12345, 1)])
+def test_prompt_attention_of_few_rows_behind_many_pages(dtype, dim, group, heads, past, tokens):
+    """Keys shared by several clusters, whose sums meet in the workspace: twice, the second time on what the first has left there."""
+    p = Pair(1, heads, group, dim, dtype, pages=(past + tokens) // 16 + 1, seed=past)
+    p.append(past)
+    p.append(tokens)
+    q = p.queries(tokens)
+    want = p.plain.attend(0, q[0])[None]
+    p.cache._prompt_work = 0
+    first = p.cache.prefill_attention(0, q.to(DEV))
+    again = p.cache.prefill_attention(0, q.to(DEV))
+    close(first, want, dtype, weights=True)
+    assert torch.equal(first, again) and p.cache.kernel_status() == 0
+
+
 @pytest.mark.parametrize("scale", [1e-30, 1e-6, 1.0])
 def test_prompt_attention_on_values_of_different_magnitudes(scale):
     """Value blocks whose scales differ by up to 2^20 under the largest one, which the weights do not prefer."""
