@@ -5,6 +5,7 @@
 //   warps 8 - 11  pages from memory into registers a whole key tile ahead; code + 128 behind the byte 0x64 is the fp16 number 1152 + code, one
 //                 fused multiply-add makes it exact (and scales values); 16-byte (8-byte) stores fill core matrices in order
 //   warp 12       S_r = Q_r K^T and O_r += P_r V of both row tiles, one thread issues
+//   warps 13 - 15 ask for pages into L2, then wait
 //   warps 0 - 7   a thread a row: scores from tensor memory, maximum, weights back over the scores as fp16
 // A row's 128 scores stay in registers, which the row warps take from the others (of the launch's 128 each: 184, converting warps 96, the last four 48).
 // The row tiles alternate: the products of one run under the exponentials of the other. Tensor memory: S of both (128 columns each), O of both (dim each), for dim 64 weights.
@@ -17,7 +18,7 @@
 // Bound: a key tile is 4 x 512 tensor cycles (dim 128) and 2 x 1024 cycles of ex2; operand reads (192 KB) and the converted tiles (64 KB written) take the
 // same time of shared memory's 128 bytes a cycle. It takes some 3600: a row tile's rows have 128 scores for 2400 cycles and then nothing for 1250, until the last weights
 // are multiplied (400) and the next scores formed over them (580, and 270 on the way); two row tiles are what tensor memory holds, and what one leaves the other does not fill.
-// 4096 tokens, 8 kv heads of 4, bf16: 139 us, 990 TFLOP/s; 8192: 481, 1143; 512 behind 3584: 48; dim 64, 4096: 117.
+// 4096 tokens, 8 kv heads of 4, bf16: 139 us, 990 TFLOP/s; 8192: 476, 1155; 512 behind 3584: 48; dim 64, 4096: 117.
 //
 // Long caches behind few rows: a cluster's CTAs share the keys of a block of rows, each leaves its sums in its shared memory, and each joins a part of the rows from there
 // (through the workspace and a second kernel: 512 behind 3584 52.4 us). Where a cluster of eight leaves SMs free several clusters share them, and their sums meet in the workspace.
@@ -57,6 +58,7 @@ struct PromptParams {
     const int32_t* indptr;
     const int32_t* indices;
     const int32_t* last;
+    int first_blocks;                                 // blocks of rows that start together
     int n_splits, ctas;                               // shares of a block's keys; CTAs of a cluster. More shares than that are joined in the workspace
     float* partials;                                  // [block of a kv head][cluster][256 rows][dim + 2]
     unsigned* counters;                               // [block of a kv head][CTA of a cluster], zero between launches
@@ -200,6 +202,15 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
                 }
             }
             if (kApart && ok && n > 0) values(1, n - 1);
+        } else if ((int)blockIdx.y < p.first_blocks) {
+            // ---- the CTAs that start together walk the same pages: each asks for a part of them into L2 (4096 tokens of six caches in turn 150 -> 145 us) ----
+            constexpr int kAskers = kThreads - 32 * (kMmaWarp + 1);
+            const int to = kShared ? min(page0 + n * kPagesTile, pages) : pages;
+            for (int i = page0 + blockIdx.y + p.first_blocks * (tid - 32 * (kMmaWarp + 1)); i < to; i += p.first_blocks * kAskers) {
+                const int id = p.indices[ip + i];
+                if ((unsigned)id < (unsigned)p.n_pages)
+                    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.chunks + ((size_t)id * p.H + kvh) * chunk_bytes(D)), "r"(chunk_bytes(D)) : "memory");
+            }
         }
     } else if (warp >= kRowWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
@@ -657,6 +668,7 @@ int launch(PromptParams p, int blocks, int most_splits, cudaStream_t st) {
     // clusters of 16 43)
     const long long units = (long long)p.H * p.B * blocks;
     p.ctas = 1;
+    p.first_blocks = (int)std::min((long long)blocks, std::max(1ll, sm_count() / ((long long)p.H * p.B)));
     for (int i = 2; i <= std::min(kMaxCluster, most_splits); ++i)
         if (units <= rooms[dev][i]) p.ctas = i;
     const long long groups = p.ctas < kMaxCluster ? 1 : std::max(1ll, std::min((long long)rooms[dev][kMaxCluster] / units, (long long)most_splits / kMaxCluster));
