@@ -673,6 +673,27 @@ def test_a_larger_batch_leaves_the_tables_of_an_earlier_graph_alive():
     assert want.shape == out.shape
 
 
+def test_two_caches_on_two_streams_at_once():
+    pairs = [Pair(2, 2, 4, 128, BF16, pages=400, seed=21), Pair(1, 4, 3, 64, F16, pages=600, seed=22)]
+    calls = []
+    for p in pairs:
+        p.append(2500)
+        q, q3 = p.queries().to(DEV), p.queries(70).to(DEV)
+        calls.append(lambda p=p, q=q, q3=q3: (p.cache.decode_attention(0, q), p.cache.prefill_attention(0, q3), p.cache.sparse_decode_attention(0, q, 20)))
+        p.cache._prompt_work = 0
+    want = [f() for f in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in pairs]
+    got = [[], []]
+    for _ in range(10):
+        for f, stream, to in zip(calls, streams, got):
+            with torch.cuda.stream(stream):
+                to.append(f())
+    torch.cuda.synchronize()
+    for outs, first, p in zip(got, want, pairs):
+        assert all(torch.equal(a, b) for out in outs for a, b in zip(out, first)) and p.cache.kernel_status() == 0
+
+
 def test_pages_beyond_four_gigabytes():
     """The free stack hands out the last pages first: offsets of 6 GB and of 3 GB into the pool."""
     p = Pair(2, 8, 2, 128, F16, pages=200_000)
