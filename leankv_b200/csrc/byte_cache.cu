@@ -9,6 +9,7 @@
 #include <type_traits>
 
 #include "byte_layout.cuh"
+#include "tile_softmax.cuh"
 
 namespace leankv {
 namespace bytes {
@@ -37,8 +38,9 @@ __device__ __forceinline__ uint32_t coarser(uint32_t w, float f) {
     return out;
 }
 
+// CTAs an SM: as many as the registers of a page's numbers leave (16 x 2011 tokens, bf16: 5 by the compiler's own choice 43.7 us, 6 41.0, 7 40.3, 8 with spills 43.9)
 template <typename T, int D>
-__global__ void __launch_bounds__(kWarps * 32) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kWarps * 32, sizeof(T) == 4 ? 4 : D == 128 ? 7 : 9) append_kernel(const AppendParams p) {
     using R = Rows<D>;
     __shared__ __align__(16) uint32_t s_words[kWarps][R::kWords];
     pdl_begin();
@@ -103,7 +105,10 @@ __global__ void __launch_bounds__(kWarps * 32) append_kernel(const AppendParams 
             for (int half = 0; half < 2; ++half) {
                 uint32_t c[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) c[k] = __float_as_uint(fmaf(row[i][j].get(4 * half + k), to_codes, 12583040.f));
+                for (int k = 0; k < 4; k += 2) {
+                    const Two v = fma2({row[i][j].get(4 * half + k), row[i][j].get(4 * half + k + 1)}, {to_codes, to_codes}, {12583040.f, 12583040.f});
+                    c[k] = __float_as_uint(v.x), c[k + 1] = __float_as_uint(v.y);
+                }
                 const uint32_t q = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
                 if (!old) w[i][j][half] = q;
                 else if (e != e_old) w[i][j][half] = coarser(w[i][j][half], power_of_two(max(e_old - e, -126)));
