@@ -24,6 +24,7 @@ capture. Appends and ``crop`` are not captured: the host keeps the lengths, too.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from ctypes import byref
 
@@ -50,6 +51,22 @@ def _point(v: _native.Vectors, t: torch.Tensor) -> torch.Tensor:
             return _point(v, t.clone(memory_format=torch.contiguous_format))
     v.data, v.seq, v.head, v.token = at, seq, head, token
     return t
+
+
+@functools.lru_cache(maxsize=4096)
+def _is_prompt(pairs: int, group: int, dim: int, tokens: int, pages: int) -> bool:
+    """Whether a chunk is taken by the prompt kernel, by what either kernel is expected to take (us). The one for few tokens reads the pages
+    once for 16 (token, query head) rows: 6 and one for each 550 of them (head size 64: 5, 1000). The prompt kernel goes through tiles of 8 pages, 2 (1.6) each
+    behind 8 (6.5), shared by as many CTAs as the device's 148 SMs hold; joining them is another 7 (5). Measured, few tokens' / prompt kernel, 8 kv heads of 4, head size 128: 64 tokens
+    after 1000 20 / 24, 128 30 / 25; 8 after 8000 26 / 28, 16 35 / 29, 4 of four sequences 35 / 44, 16 83 / 44; 128 after none 9 / 10, 256 16 / 12."""
+    few = 6 + pairs * -(-tokens * group // 16) * pages / 550 if dim == 128 else 5 + pairs * -(-tokens * group // 16) * pages / 1000
+    units, tiles = pairs * -(-tokens // (2 * (128 // group))), -(-pages // 8)
+    shares = max(1, min(148 // units, tiles // 4))
+    if shares > 8:
+        shares -= shares % 8
+    steps = -(-tiles // shares) * -(-units // 148)
+    prompt = 8 + 2 * steps + 7 * (shares > 1) if dim == 128 else 6.5 + 1.6 * steps + 5 * (shares > 1)
+    return few > prompt
 
 
 def _capturing() -> bool:
@@ -94,11 +111,8 @@ class ByteKVCache(PagedKVCache):
         # not on first use: a call that is being captured would record the clearing instead of doing it
         size = _native.byte_lib().leankv_byte_attn_workspace_bytes() if self._device.type == "cuda" else 0
         self._workspace = torch.zeros(size, dtype=torch.uint8, device=self._device)
-        # pages read by 16 (token, query head) rows at a time from which a chunk goes to the prompt kernel. Up to there the kernel for few tokens
-        # is faster (us, 8 kv heads of 4, few tokens' / prompt kernel: 32 tokens after 1000, 4 thousand of these pages, 17 / 22; 64 after 1000, 9 thousand, 20 / 25; 128 after
-        # 1000, 18 thousand, 30 / 25; 8 after 8000, 8 thousand, 26 / 28; 16 after 8000, 16 thousand, 36 / 29). Where nothing is cached before them it is up to 4 us slower
-        # (256 after none, 8 thousand, 16 / 12)
-        self._prompt_work = 10_000
+        # None: by the rule above; else the pages read by 16 (token, query head) rows at a time from which a chunk goes to the prompt kernel
+        self._prompt_work = None
         # the calls' arguments, one set for each layer: a call fills in what changes
         self._args, self._pools = [], []
         for i in range(num_layers):
@@ -337,9 +351,14 @@ class ByteKVCache(PagedKVCache):
             raise RuntimeError("prefill_attention: the chunk has not been appended to this sequence")
         out = torch.empty(batch, t_new, self.num_q_heads, self.head_dim, dtype=q.dtype, device=q.device).transpose(1, 2)
         if t_new:
-            tiles = -(-t_new * (self.num_q_heads // self.num_kv_heads) // 16)
+            group = self.num_q_heads // self.num_kv_heads
             pages = self._most_pages(batch)
-            prompt = batch * self.num_kv_heads * tiles * pages > self._prompt_work and q.dtype != torch.float32
+            if q.dtype == torch.float32:
+                prompt = False
+            elif self._prompt_work is None:
+                prompt = _is_prompt(batch * self.num_kv_heads, group, self.head_dim, t_new, pages)
+            else:
+                prompt = batch * self.num_kv_heads * -(-t_new * group // 16) * pages > self._prompt_work
             self._attend(layer_idx, q, out, t_new, pages, prompt=prompt)
         return out if out.dtype == query.dtype else out.to(query.dtype)
 

@@ -12,7 +12,7 @@ import torch
 
 from leankv_b200 import _native, combined
 from leankv_b200.turboquant import hf_attention
-from leankv_b200.turboquant.byte_cache import ByteKVCache, _point
+from leankv_b200.turboquant.byte_cache import ByteKVCache, _is_prompt, _point
 from leankv_b200.turboquant.paged_cache import PagedKVCache
 from oracle import bytes as obytes
 
@@ -83,6 +83,14 @@ def test_rows_that_would_have_to_move_are_refused():
     for call in (lambda: cache.reorder_cache(torch.tensor([0])), lambda: cache.batch_repeat_interleave(2), lambda: cache.batch_select_indices(torch.tensor([0]))):
         with pytest.raises(RuntimeError, match="places"):
             call()
+
+
+def test_a_chunk_goes_to_the_kernel_that_takes_less():
+    for pairs, group, dim, tokens, past, prompt in (
+            (8, 4, 128, 64, 1000, False), (8, 4, 128, 128, 1000, True), (8, 4, 128, 8, 8000, False), (8, 4, 128, 16, 8000, True), (32, 4, 128, 4, 8000, False),
+            (32, 4, 128, 16, 8000, True), (8, 4, 128, 64, 0, False), (8, 4, 128, 256, 0, True), (4, 3, 64, 128, 1000, False), (4, 3, 64, 64, 8000, True),
+            (8, 1, 128, 1, 0, False), (1024 * 8, 16, 128, 4000, 100000, True)):
+        assert _is_prompt(pairs, group, dim, tokens, -(-(past + tokens) // 16)) == prompt
 
 
 def test_a_cache_is_not_copied():
