@@ -143,10 +143,11 @@ __global__ void __launch_bounds__(kScoreThreads) score_kernel(const SelectParams
     }
 }
 
-// fp32 numbers as whole numbers in the same order; NaN (without a sign) above infinity.
+// fp32 numbers as whole numbers in the same order; every NaN is the one number above infinity. (A product with NaN is 0x7fffffff whatever NaN came in:
+// in the numbers' own order that is the last of 32 bits, and a range of keys that began there would end at zero.)
 __device__ __forceinline__ uint32_t ordered(float v) {
     const uint32_t x = __float_as_uint(v);
-    return x ^ ((x >> 31) ? 0xffffffffu : 0x80000000u);
+    return isnan(v) ? 0xff800001u : x ^ ((x >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
 template <int kThreads>
@@ -242,7 +243,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) 
             room -= s_above;
             low += (uint32_t)s_at << shift;
             if (shift == 0 || s_in == room) break;
-            high = low + ((1u << shift) - 1u);
+            high = low + min(high - low, (1u << shift) - 1u);
         }
         border = low;
         // a bin that is chosen whole: everything from its lower end on
@@ -291,6 +292,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) 
             const int n_in = base + (int)(r & 0xffffu) + __popc(in[i] & lanes), n_at = base_at + (int)(r >> 16) + __popc(at[i] & lanes);
             if (!is_in && n_at >= room) continue;
             const int j = slab * kSlab + i * kThreads + tid, to = n_in + min(n_at, room);
+            if (to >= p.n_blocks) continue;        // never: the list is another pair's from there on
             blocks[to] = j;
             block_pages[to] = p.indices[ip + j];
         }

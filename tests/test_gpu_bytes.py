@@ -468,6 +468,29 @@ def test_equal_scores_go_to_the_earlier_block():
     assert p.check_sparse(6, 0, 1)[0, 1].tolist() == [0, 1, 2, 3, 4, 43]
 
 
+@pytest.mark.parametrize("bad, blocks", [(30, 32), (29, 32), (28, 32), (100, 32), (509, 32), (40, 4), (300, 301)])
+def test_more_blocks_without_a_number_than_there_is_room_for(bad, blocks):
+    """One sequence of three has ``bad`` key blocks that are no numbers: the first of them are chosen, and the lists of the others are what they are without it."""
+    p = Pair(3, 2, 2, 64, BF16, pages=1600, seed=bad)
+    k, v = (vectors(p.gen, 3, 2, 16 * 512, 64, BF16) for _ in range(2))
+    at = 16 * (1 + torch.randperm(509, generator=p.gen)[:bad])
+    k[1, 1, at, 3] = torch.tensor([math.inf, -math.inf, math.nan], dtype=BF16)[torch.arange(bad) % 3]
+    p.cache.append(0, k.to(DEV), v.to(DEV))
+    p.plain.append(k, v)
+    q = p.queries()
+    got, chosen = p.cache.sparse_decode_attention(0, q.to(DEV), blocks, return_blocks=True)
+    for b in range(3):
+        want = p.plain.choose(b, q[b], blocks, 1, 2)
+        assert torch.equal(chosen[b].cpu(), want), b
+        out = p.plain.attend(b, q[b, :, None], want)[:, 0]
+        if b == 1:
+            assert bool(got[b, 2:].isnan().all())
+            close(got[b, :2], out[:2], BF16)
+        else:
+            close(got[b], out, BF16)
+    assert p.cache.kernel_status() == 0
+
+
 @pytest.mark.parametrize("tokens, blocks", [(70000, 300), (16 * 4097, 33), (270000, 17)])
 def test_choice_among_many_blocks(tokens, blocks):
     """More blocks than a small CTA, and than any CTA, keeps in registers; scores against the definition, vectorised."""
