@@ -67,7 +67,7 @@ int leankv_byte_unpack(const leankv_byte_pool_t* pool /* host */, int dtype, voi
 
 /* Attention of the last `tokens` tokens of each of `batch` sequences over the cache, causal among themselves: q_heads / kv_heads (up to
  * LEANKV_BYTES_MAX_GROUP) query heads share a kv head; q and out of `dtype`. Softmax statistics and sums are fp32. A sequence
- * without tokens, and a query before the first token, gets zeros.
+ * without tokens (kv_indptr[b + 1] <= kv_indptr[b]), and a query before the first token, gets zeros.
  * max_pages_seq, total_pages: upper bounds of any sequence's pages and of all sequences' together, for the launch's shape.
  * block_pages = NULL: every page. Else (tokens = 1) the pages of sequence b and kv head h are block_pages[(b * kv_heads + h) * n_blocks ..], as
  * many as there are blocks or n_blocks, the last of them the sequence's last page (leankv_byte_select writes such lists).

@@ -17,8 +17,8 @@ heads a kv head, keys, values and queries in fp16, bf16 or fp32, tensors of any 
     out = cache.sparse_decode_attention(layer, q, blocks=128)   # the same, 128 blocks per kv head
 
 A cache is used by one stream at a time: its pages, its page table and the workspace of its attention are one set. Attention may be captured into
-a CUDA graph; a replay answers for the lengths that the sequences have by then, as long as there are no more sequences than at the
-capture. Appends and ``crop`` are not captured: the host keeps the lengths, too.
+a CUDA graph; a replay answers for the lengths that the sequences have by then, however many sequences there are.
+Appends and ``crop`` are not captured: the host keeps the lengths, too.
 """
 
 from __future__ import annotations
@@ -131,23 +131,48 @@ class ByteKVCache(PagedKVCache):
         self._alloc_tables(0)
 
     def _alloc_tables(self, batch_cap: int):
-        if getattr(self, "_kv_indptr", None) is not None:
-            # a graph that was captured before may still read these
-            self._earlier_tables.append((self._kv_indptr, self._kv_page_indices, self._kv_last))
-        super()._alloc_tables(batch_cap)
-        for args in self._args:
-            for a in args:
-                a[0].kv_indptr, a[0].kv_page_indices = self._kv_indptr.data_ptr(), self._kv_page_indices.data_ptr()
-            args[0][0].kv_last_page_len = args[1][0].kv_last_page_len = self._kv_last.data_ptr()
+        """Room for the pages of ``batch_cap`` sequences. Only the block table ever moves: lengths and flat arrays, which the kernels of a captured call
+        read, have their place for as many sequences as a call may have (16 KB)."""
+        dev, i32 = self._device, torch.int32
+        table = getattr(self, "_block_table", None)
+        self._batch_cap = max(batch_cap, 1)
+        self._pps_cap = self.max_pages                       # a single sequence may take the whole pool
+        if table is None:
+            most = _native.BYTES_MAX_BATCH
+            # one allocation, each array from a 16-byte boundary on; zeros as far as the free stack
+            sizes = [most, most + 1, most, most, self.max_pages, 1, self.max_pages, 1]
+            padded = [-(-n // 4) * 4 for n in sizes]
+            store = torch.empty(sum(padded), dtype=i32, device=dev)
+            (self._seq_len_dev, self._kv_indptr, self._kv_last, self._start_dev, self._kv_page_indices, self._status, self._free_stack,
+             self._free_top) = (v[:n] for v, n in zip(store.split(padded), sizes))
+            self._begin_args = (ctypes.c_void_p(store.data_ptr()), sum(padded[:6]), self.max_pages, sum(padded[:7]))
+            self._begin(store)
+            self._block_table = torch.zeros(self._batch_cap, self._pps_cap, dtype=i32, device=dev)
+            for args in self._args:
+                for a in args:
+                    a[0].kv_indptr, a[0].kv_page_indices = self._kv_indptr.data_ptr(), self._kv_page_indices.data_ptr()
+                args[0][0].kv_last_page_len = args[1][0].kv_last_page_len = self._kv_last.data_ptr()
+        else:
+            self._earlier_tables.append(table)               # a graph that was captured before may still read it
+            self._block_table = torch.zeros(self._batch_cap, self._pps_cap, dtype=i32, device=dev)
+            self._block_table[:len(table)] = table
         at = lambda t: ctypes.c_void_p(t.data_ptr())      # converted once, not at every call
         self._step_args = (at(self._seq_len_dev), at(self._block_table), ctypes.c_int(self._pps_cap), at(self._free_stack), at(self._free_top),
                            at(self._kv_indptr), at(self._kv_page_indices), at(self._kv_last), at(self._start_dev), at(self._status))
-        # an empty table: the status word, the free stack and its height lie one behind the other; before them the flat arrays and the lengths, as long as there
-        # was never more than one sequence
-        self._lengths_too = self._batch_cap == 1
-        first = self._seq_len_dev if self._lengths_too else self._status
-        zeros = (self._free_stack.data_ptr() - first.data_ptr()) // 4
-        self._begin_args = (at(first), zeros, self.max_pages, zeros + -(-self.max_pages // 4) * 4)
+        self._meta_batch = -1                                # sequences that the flat arrays were built for
+
+    def _begin(self, store=None):
+        """No sequences: every page is free, lengths and flat arrays are zeros, so that a sequence behind the last one of a table has no pages (or
+        fewer, where ``kv_indptr`` falls back to zero: none as well)."""
+        if self._device.type != "cuda":
+            store[:self._begin_args[1]].zero_()
+            torch.arange(self.max_pages, out=self._free_stack)
+            self._free_top.fill_(self.max_pages)
+            return
+        with _native.on_device(self._device):
+            rc = self._table_lib.leankv_paged_table_begin(*self._begin_args, _native.current_stream())
+        if rc:
+            _native.check(rc, "leankv_paged_table_begin")
 
     def _table_step(self, t_new: int, batch: int):
         with _native.on_device(self._device):
@@ -404,13 +429,7 @@ class ByteKVCache(PagedKVCache):
             return super().reset()
         if _capturing():
             raise RuntimeError("ByteKVCache: reset changes lengths that the host keeps, too, and cannot be captured")
-        with _native.on_device(self._device):
-            rc = self._table_lib.leankv_paged_table_begin(*self._begin_args, _native.current_stream())
-        _native.check(rc, "leankv_paged_table_begin")
-        if not self._lengths_too:
-            self._seq_len_dev.zero_()
-            if self._captured and self._seq_lengths:
-                self._table_step(0, len(self._seq_lengths))
+        self._begin()
         self._seq_lengths = []
         self._batch_size = 0
         self._seen_tokens = 0

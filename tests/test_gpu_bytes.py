@@ -696,6 +696,52 @@ def test_a_larger_batch_leaves_the_tables_of_an_earlier_graph_alive():
     assert want.shape == out.shape
 
 
+def test_a_graph_from_before_the_table_grew_answers_for_what_the_sequences_hold():
+    """Captured for two sequences, replayed with five: pages that are new by then, pages that were given back, and a table of one sequence again."""
+    p = Pair(5, 2, 3, 64, BF16, pages=300)
+    p.append(40, batch=2)
+    q, q3 = p.queries()[:2].to(DEV), p.queries(3)[:2].to(DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dense = p.cache.decode_attention(0, q)
+        few, chosen = p.cache.sparse_decode_attention(0, q, 4, return_blocks=True)
+        prompt = p.cache.prefill_attention(0, q3)
+
+    def check():
+        graph.replay()
+        torch.cuda.synchronize()
+        for b in range(2):
+            if p.plain.n[b] == 0:
+                assert not bool(dense[b].any()) and not bool(few[b].any()) and not bool(prompt[b].any()) and bool((chosen[b] == -1).all())
+                continue
+            close(dense[b], p.plain.attend(b, q[b, :, None].cpu())[:, 0], BF16)
+            close(prompt[b], p.plain.attend(b, q3[b].cpu()), BF16)
+            want = p.plain.choose(b, q[b].cpu(), 4, 1, 2)
+            assert torch.equal(chosen[b].cpu(), want)
+            close(few[b], p.plain.attend(b, q[b, :, None].cpu(), want)[:, 0], BF16)
+        assert p.cache.kernel_status() == 0 and p.cache.page_table_status() == 0
+
+    check()
+    p.append(33)                                       # five sequences: another block table
+    held = [torch.full((1 << 18,), 7, dtype=torch.int32, device=DEV) for _ in range(8)]
+    check()
+    p.append(100, batch=1)
+    check()
+    p.append(5, batch=3)
+    check()
+    p.cache.crop(70)
+    p.plain.crop(70)
+    check()
+    p.cache.reset()
+    p.plain = obytes.Cache(5, 2, 64)
+    check()
+    p.append(50, batch=1)                              # the second sequence holds nothing
+    check()
+    p.append(9, batch=2)
+    check()
+    del held
+
+
 def test_two_caches_on_two_streams_at_once():
     pairs = [Pair(2, 2, 4, 128, BF16, pages=400, seed=21), Pair(1, 4, 3, 64, F16, pages=600, seed=22)]
     calls = []
