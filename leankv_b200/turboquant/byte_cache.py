@@ -94,6 +94,8 @@ class ByteKVCache(PagedKVCache):
         self.bits = bits
         self._dtype = dtype
         self._device = torch.device(device) if device is not None else torch.device("cuda")
+        if self._device.type == "cuda" and _capturing():
+            raise RuntimeError("ByteKVCache: a cache cannot be made inside a capture: its page table would be cleared by every replay")
         if self._device.type == "cuda" and self._device.index is None:
             self._device = torch.device("cuda", torch.cuda.current_device())       # whichever device is current in later calls
         self._seen_tokens = 0
@@ -126,8 +128,6 @@ class ByteKVCache(PagedKVCache):
             self._args.append(((append, byref(append), append.k, append.v), (attn, byref(attn), attn.q, attn.out), (select, byref(select), select.q)))
         self._device_index = self.kv_data.get_device()
         self._lib, self._table_lib = _native.byte_lib(), _native.lib()
-        self._captured = False                # an attention call was: graphs may be replayed
-        self._earlier_tables = []
         self._alloc_tables(0)
 
     def _alloc_tables(self, batch_cap: int):
@@ -147,19 +147,18 @@ class ByteKVCache(PagedKVCache):
              self._free_top) = (v[:n] for v, n in zip(store.split(padded), sizes))
             self._begin_args = (ctypes.c_void_p(store.data_ptr()), sum(padded[:6]), self.max_pages, sum(padded[:7]))
             self._begin(store)
+            self._meta_batch = 0                             # sequences that the flat arrays were built for; -1: they are not the table's
             self._block_table = torch.zeros(self._batch_cap, self._pps_cap, dtype=i32, device=dev)
             for args in self._args:
                 for a in args:
                     a[0].kv_indptr, a[0].kv_page_indices = self._kv_indptr.data_ptr(), self._kv_page_indices.data_ptr()
                 args[0][0].kv_last_page_len = args[1][0].kv_last_page_len = self._kv_last.data_ptr()
         else:
-            self._earlier_tables.append(table)               # a graph that was captured before may still read it
             self._block_table = torch.zeros(self._batch_cap, self._pps_cap, dtype=i32, device=dev)
             self._block_table[:len(table)] = table
         at = lambda t: ctypes.c_void_p(t.data_ptr())      # converted once, not at every call
         self._step_args = (at(self._seq_len_dev), at(self._block_table), ctypes.c_int(self._pps_cap), at(self._free_stack), at(self._free_top),
                            at(self._kv_indptr), at(self._kv_page_indices), at(self._kv_last), at(self._start_dev), at(self._status))
-        self._meta_batch = -1                                # sequences that the flat arrays were built for
 
     def _begin(self, store=None):
         """No sequences: every page is free, lengths and flat arrays are zeros, so that a sequence behind the last one of a table has no pages (or
@@ -177,8 +176,6 @@ class ByteKVCache(PagedKVCache):
     def _table_step(self, t_new: int, batch: int):
         with _native.on_device(self._device):
             self._step(t_new, batch, _native.current_stream())
-        if self._device.type == "cuda" and _capturing():
-            self._meta_batch = -1                         # what a graph records has not been built yet
 
     def _step(self, t_new: int, batch: int, stream: int):
         rc = self._table_lib.leankv_paged_table_step(t_new, batch, *self._step_args, stream)
@@ -188,10 +185,14 @@ class ByteKVCache(PagedKVCache):
 
     def _device_meta(self, batch_size: int):
         """(kv_indptr, kv_page_indices, kv_last_page_len) int32 on the device, for all known sequences: the first ones' part is the same
-        for any smaller batch."""
+        for any smaller batch. A capture finds them as they are, with no pages for sequences that nobody knows yet: it neither takes
+        memory for the table, which would be the graph's, nor records steps, which later replays would take on a table that has moved on."""
         if self._meta_batch < batch_size:
-            self._ensure_batch_size(batch_size)
-            self._table_step(0, len(self._seq_lengths))
+            if self._device.type != "cuda" or not _capturing():
+                self._ensure_batch_size(batch_size)
+                self._table_step(0, len(self._seq_lengths))
+            elif self._meta_batch < 0:
+                raise RuntimeError("ByteKVCache: the page table has changed: call the attention once before it is captured")
         return self._kv_indptr, self._kv_page_indices, self._kv_last
 
     # ── arguments ──────────────────────────────────────────────────────
@@ -221,7 +222,6 @@ class ByteKVCache(PagedKVCache):
     def _most_pages(self, batch: int) -> int:
         """Of any of the first sequences; of any there may be where a graph is captured, whose replays meet longer ones."""
         if _capturing():
-            self._captured = True
             return self.max_pages
         return -(-max(self._seq_lengths[:batch]) // PAGE)
 
@@ -324,7 +324,7 @@ class ByteKVCache(PagedKVCache):
 
     def _answer(self, q: torch.Tensor) -> torch.Tensor:
         """Room for a one-token answer."""
-        if len(self._seq_lengths) < q.shape[0]:
+        if len(self._seq_lengths) < q.shape[0] and not _capturing():
             self._ensure_batch_size(q.shape[0])
         return torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=q.dtype, device=q.device)
 
@@ -410,18 +410,18 @@ class ByteKVCache(PagedKVCache):
         if not batch or max(self._seq_lengths) <= max_length:
             return
         with _native.on_device(self._device):
-            rc = _native.lib().leankv_paged_table_crop(max_length, batch, self._seq_len_dev.data_ptr(), self._block_table.data_ptr(),
-                                                       self._pps_cap, self._free_stack.data_ptr(), self._free_top.data_ptr(),
-                                                       self.max_pages, self._status.data_ptr(), _native.current_stream())
-        _native.check(rc, "leankv_paged_table_crop")
+            stream = _native.current_stream()
+            rc = self._table_lib.leankv_paged_table_crop(max_length, batch, self._seq_len_dev.data_ptr(), self._block_table.data_ptr(),
+                                                         self._pps_cap, self._free_stack.data_ptr(), self._free_top.data_ptr(),
+                                                         self.max_pages, self._status.data_ptr(), stream)
+            if rc:
+                _native.check(rc, "leankv_paged_table_crop")
+            self._step(0, batch, stream)      # a replay reads the flat arrays without a call of this class in between
         kept = -(-max_length // PAGE)
         for b, n in enumerate(self._seq_lengths):
             if n > max_length:
                 self._free_count += -(-n // PAGE) - kept
                 self._seq_lengths[b] = max_length
-        self._meta_batch = -1
-        if self._captured:                    # a replay reads the flat arrays without a call of this class in between
-            self._table_step(0, batch)
 
     def reset(self):
         """Forget every sequence. Pages need no clearing: only positions that have been written are read."""
@@ -434,7 +434,7 @@ class ByteKVCache(PagedKVCache):
         self._batch_size = 0
         self._seen_tokens = 0
         self._free_count = self.max_pages
-        self._meta_batch = -1
+        self._meta_batch = 0
 
     def _one_row_each(self, *args):
         raise RuntimeError("ByteKVCache keeps its sequences in their places: no beams, repeated or chosen rows")

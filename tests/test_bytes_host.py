@@ -11,7 +11,7 @@ import pytest
 import torch
 
 from leankv_b200 import _native, combined
-from leankv_b200.turboquant import hf_attention
+from leankv_b200.turboquant import byte_cache, hf_attention
 from leankv_b200.turboquant.byte_cache import ByteKVCache, _is_prompt, _point
 from leankv_b200.turboquant.paged_cache import PagedKVCache
 from oracle import bytes as obytes
@@ -98,6 +98,13 @@ def test_a_cache_is_not_copied():
     for copied in (copy.copy, copy.deepcopy, pickle.dumps):
         with pytest.raises(RuntimeError, match="copied"):
             copied(cache)
+
+
+def test_a_cache_is_not_made_inside_a_capture(monkeypatch):
+    monkeypatch.setattr(byte_cache, "_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="inside a capture"):
+        _cpu_cache(device="cuda:0")
+    assert _cpu_cache().get_seq_length() == 0
 
 
 def test_vectors_are_read_where_they_are_or_copied():

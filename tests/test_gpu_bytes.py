@@ -696,6 +696,84 @@ def test_a_larger_batch_leaves_the_tables_of_an_earlier_graph_alive():
     assert want.shape == out.shape
 
 
+@pytest.mark.parametrize("known", [0, 1, 2])
+def test_attention_captured_ahead_of_the_sequences_answers_once_they_are_there(known):
+    """A capture for more sequences than have been appended leaves the cache as it was; the table is taken by the appends behind it."""
+    p = Pair(4, 2, 2, 64, F16, pages=200)
+    if known:
+        p.append(21, batch=known)
+    q = p.queries().to(DEV)
+    table, lengths = p.cache._block_table, list(p.cache._seq_lengths)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dense = p.cache.decode_attention(0, q)
+        few, chosen = p.cache.sparse_decode_attention(0, q, 4, return_blocks=True)
+    assert p.cache._block_table is table and p.cache._seq_lengths == lengths
+
+    def check():
+        graph.replay()
+        torch.cuda.synchronize()
+        for b in range(4):
+            close(dense[b], p.plain.attend(b, q[b, :, None].cpu())[:, 0], F16)
+            if p.plain.n[b]:
+                want = p.plain.choose(b, q[b].cpu(), 4, 1, 2)
+                assert torch.equal(chosen[b].cpu(), want)
+                close(few[b], p.plain.attend(b, q[b, :, None].cpu(), want)[:, 0], F16)
+        assert p.cache.kernel_status() == 0 and p.cache.page_table_status() == 0
+
+    check()
+    for tokens, batch in ((20, 2), (1, 2), (90, 4), (1, 3)):
+        p.append(tokens, batch=batch)
+        check()
+        p.check_pages()
+    p.check_decode()
+
+
+def test_attention_captured_behind_a_crop_or_a_reset_replays_on_a_larger_table():
+    """What these leave is in place before the capture: nothing that a replay would repeat on a table that has moved on."""
+    p = Pair(4, 1, 2, 64, F16, pages=200)
+    p.append(70, batch=2)
+    p.cache.crop(50)
+    p.plain.crop(50)
+    q = p.queries().to(DEV)
+    cropped, empty = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(cropped):
+        first = p.cache.decode_attention(0, q[:2])
+    cropped.replay()
+    close(first, torch.stack([p.plain.attend(b, q[b, :, None].cpu())[:, 0] for b in range(2)]), F16)
+    p.cache.reset()
+    p.plain = obytes.Cache(4, 1, 64)
+    with torch.cuda.graph(empty):
+        second = p.cache.decode_attention(0, q)
+    for tokens, batch in ((30, 1), (40, 4), (9, 2)):
+        p.append(tokens, batch=batch)
+        cropped.replay()
+        empty.replay()
+        torch.cuda.synchronize()
+        want = torch.stack([p.plain.attend(b, q[b, :, None].cpu())[:, 0] for b in range(4)])
+        close(first, want[:2], F16)
+        close(second, want, F16)
+        p.check_decode()                               # a replay has changed nothing that an eager call reads
+        p.check_pages()
+
+
+def test_a_table_that_does_not_fit_its_flat_arrays_is_not_captured():
+    p = Pair(2, 1, 2, 64, F16)
+    p.append(30)
+    p.cache._free_sequence_pages(1)
+    q = p.queries().to(DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        doubled = q * 2
+        with pytest.raises(RuntimeError, match="before it is captured"):
+            p.cache.decode_attention(0, q)
+    graph.replay()
+    assert torch.equal(doubled, q * 2)
+    out = p.cache.decode_attention(0, q)
+    close(out[0], p.plain.attend(0, q[0, :, None].cpu())[:, 0], F16)
+    assert not bool(out[1].any())
+
+
 def test_a_graph_from_before_the_table_grew_answers_for_what_the_sequences_hold():
     """Captured for two sequences, replayed with five: pages that are new by then, pages that were given back, and a table of one sequence again."""
     p = Pair(5, 2, 3, 64, BF16, pages=300)
