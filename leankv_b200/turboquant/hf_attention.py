@@ -110,7 +110,8 @@ def enable_paged_attention(model, cache, fused_prefill: bool = False, sparse_blo
         if not hasattr(cache, "sparse_decode_attention"):
             raise RuntimeError("sparse_blocks needs a cache that selects blocks: ByteKVCache")
         cache.check_blocks(sparse_blocks)
-        cache.sparse_blocks = sparse_blocks
+    if hasattr(cache, "sparse_decode_attention"):
+        cache.sparse_blocks = sparse_blocks        # None too: what an earlier call asked for does not stay
     register()
     for attn in _attention_modules(model):
         attn._leankv_paged_cache = cache

@@ -180,6 +180,29 @@ def test_decode_steps_are_routed_to_the_chosen_blocks():
     assert asked == [(3, (2, 6, 64), 5), (3, (2, 6, 64), None)]
 
 
+def test_every_call_of_the_plug_in_sets_what_decode_steps_read():
+    """Dense attention behind chosen blocks, on the same model or another, and a refused call that changes nothing."""
+    from types import SimpleNamespace
+
+    def model():
+        return SimpleNamespace(model=SimpleNamespace(layers=[SimpleNamespace(self_attn=SimpleNamespace())]), config=SimpleNamespace(_attn_implementation="sdpa"))
+
+    cache, first = _cpu_cache(), model()
+    hf_attention.enable_paged_attention(first, cache, sparse_blocks=64)
+    assert cache.sparse_blocks == 64
+    hf_attention.enable_paged_attention(first, cache)
+    assert cache.sparse_blocks is None
+    hf_attention.enable_paged_attention(first, cache, sparse_blocks=8)
+    with pytest.raises(RuntimeError, match="sparse"):
+        hf_attention.enable_paged_attention(first, cache, sparse_blocks=1)
+    assert cache.sparse_blocks == 8
+    hf_attention.enable_paged_attention(model(), cache, fused_prefill=True)
+    assert cache.sparse_blocks is None and cache.fused_prefill
+    other = PagedKVCache(num_layers=1, num_kv_heads=1, num_q_heads=4, max_pages=2, device="cpu")
+    hf_attention.enable_paged_attention(model(), other)
+    assert not hasattr(other, "sparse_blocks")
+
+
 # ── the C ABI: refused before any launch ─────────────────────────────────────────────────────────────────────
 
 def _no_gpu():
