@@ -422,6 +422,7 @@ class ByteKVCache(PagedKVCache):
             if n > max_length:
                 self._free_count += -(-n // PAGE) - kept
                 self._seq_lengths[b] = max_length
+        self._seen_tokens = min(self._seen_tokens, max_length)
 
     def reset(self):
         """Forget every sequence. Pages need no clearing: only positions that have been written are read."""

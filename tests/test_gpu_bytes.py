@@ -217,6 +217,16 @@ def test_crop_gives_pages_back_and_the_next_tokens_join_what_is_left():
     assert sorted(free + held) == list(range(24)) and int(p.cache._free_top) == len(free)
 
 
+def test_crop_takes_back_what_was_seen():
+    p = Pair(2, 1, 1, 64, F16)
+    p.append(50)
+    for keep, seen in ((60, 50), (41, 41), (-3, 38), (0, 0)):
+        p.cache.crop(keep)
+        assert p.cache.seen_tokens == p.cache.get_seq_length() == seen
+    p.append(7, batch=1)
+    assert p.cache.seen_tokens == p.cache.get_seq_length() == 7
+
+
 def test_a_full_pool_is_refused_and_leaves_the_cache_as_it_was():
     p = Pair(2, 1, 1, 64, F16, pages=6)
     p.append(40)
