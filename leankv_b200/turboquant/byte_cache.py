@@ -234,8 +234,8 @@ class ByteKVCache(PagedKVCache):
         batch, t_new = k.shape[0], k.shape[2]
         v = self._typed(value_states, "value_states", self.num_kv_heads, batch, t_new)
         (args, call, kp, vp), _, _ = self._layer(layer_idx)
-        if k.dtype != v.dtype:
-            v = v.to(k.dtype)
+        if k.dtype != v.dtype:                # a type that holds the numbers of both: a cast of one to the other's would round it, or lose its range
+            k, v = k.float(), v.float()
         if t_new == 0:
             return
         if _capturing():

@@ -440,6 +440,18 @@ def test_other_strides_other_types_and_views():
     close(mixed, torch.stack([p.plain.attend(b, q[b, 7, :, None])[:, 0] for b in range(2)]), F32)
 
 
+@pytest.mark.parametrize("k_type, v_type", [(F16, BF16), (BF16, F16), (F16, F32), (F32, BF16)])
+def test_keys_and_values_of_different_types_keep_their_numbers(k_type, v_type):
+    """Values of 1e6 beside keys in fp16, and keys of eleven bits beside values in bf16."""
+    p = Pair(2, 2, 2, 64, BF16)
+    for tokens in (19, 1):
+        k, v = vectors(p.gen, 2, 2, tokens, 64, k_type), (vectors(p.gen, 2, 2, tokens, 64, F32) * (1.0 if v_type == F16 else 1e5)).to(v_type)
+        p.cache.append(0, k.to(DEV), v.to(DEV))
+        p.plain.append(k, v)
+    p.check_pages()
+    p.check_decode()
+
+
 # ── blocks by score ──────────────────────────────────────────────────────────────────────────────────────────
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
