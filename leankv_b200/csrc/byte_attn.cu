@@ -41,7 +41,7 @@ constexpr int kWavePages = 96;                     // of a CTA where there is mo
 // A row's reference lies kLift below the largest score seen when it last moved, and moves when a score exceeds it by more than kReach: weights are at most
 // 2^15 in fp16, and one of 2^-24 of the largest is still a normal number there. Moving costs the rescaling of all sums.
 constexpr float kLift = 10.f, kReach = 15.f;
-constexpr float kNoRef = -1.0e30f;                 // a maximum before any score: finite, so that masked scores give weight 0
+constexpr float kNoRef = -3.402823466e38f;         // a maximum before any score: below all of them, and finite, so that masked scores give weight 0
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kJoin = 32;                          // parts of a triple that are joined at a time
 __host__ __device__ constexpr int stages(int dim) { return dim == 128 ? 3 : 6; }

@@ -41,7 +41,7 @@ constexpr int kKeysTile = 128, kPagesTile = kKeysTile / kPage;
 constexpr int kRowWarps = 8, kConvWarps = 4, kMmaWarp = kRowWarps + kConvWarps;
 constexpr int kThreads = 512;                         // four warpgroups: registers change hands by warpgroup
 constexpr int kPagesWarp = kPagesTile / kConvWarps;
-constexpr float kNoRef = -1.0e30f;
+constexpr float kNoRef = -3.402823466e38f;            // a maximum before any score: below all of them, and finite, so that masked scores give weight 0
 constexpr float kLift = 7.f, kReach = 15.f;           // the reference of a row is its maximum - kLift when it moves, and moves beyond kReach above it
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kScaleSlots = 4;

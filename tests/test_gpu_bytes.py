@@ -401,6 +401,27 @@ def test_weights_far_apart_and_rows_that_grow():
     assert bool(((got.cpu().double() - want).abs()[0] <= 1e-4 * (w @ size)).all())
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("dim, past", [(64, 0), (128, 700)])
+def test_scores_far_below_zero_are_scores(dtype, dim, past):
+    """Products of -1e36: every one is finite in 32 bits, and what is seen is never a row without tokens. The keys' sizes are powers of two, so that a row's largest
+    score stands alone by 1e35 and the answer is one token's value."""
+    p = Pair(1, 1, 2, dim, dtype, pages=60)
+    k = -torch.exp2(60.0 + (torch.arange(past + 20) * 7 % 5)).to(dtype)[None, None, :, None].expand(1, 1, -1, dim).contiguous()
+    k[0, 0, 1:] *= 2                                   # the first token is the largest score of every row
+    v = vectors(p.gen, 1, 1, past + 20, dim, dtype)
+    p.cache.append(0, k.to(DEV), v.to(DEV))
+    p.plain.append(k, v)
+    q = torch.full((1, 2, 20, dim), 2.0 ** 56).to(dtype)
+    p.cache._prompt_work = 1 << 60
+    want = p.plain.attend(0, q[0])[None]
+    assert bool((want.norm(dim=-1) > 0).all())
+    close(p.cache.decode_attention(0, q[:, :, -1].to(DEV)), want[:, :, -1], dtype)
+    for work in (0, 1 << 60):
+        p.cache._prompt_work = work
+        close(p.cache.prefill_attention(0, q.to(DEV)), want, dtype, weights=work == 0)
+
+
 def test_queries_of_any_scale():
     for dtype, scale in ((BF16, 1e-30), (BF16, 1e4), (F32, 1e-35), (F32, 1e-3), (F16, 1e-4)):
         p = Pair(1, 2, 3, 64, dtype)
