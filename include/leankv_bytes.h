@@ -67,7 +67,8 @@ int leankv_byte_unpack(const leankv_byte_pool_t* pool /* host */, int dtype, voi
 
 /* Attention of the last `tokens` tokens of each of `batch` sequences over the cache, causal among themselves: q_heads / kv_heads (up to
  * LEANKV_BYTES_MAX_GROUP) query heads share a kv head; q and out of `dtype`. Softmax statistics and sums are fp32. A sequence
- * without tokens (kv_indptr[b + 1] <= kv_indptr[b]), and a query before the first token, gets zeros.
+ * without tokens (kv_indptr[b + 1] <= kv_indptr[b]), and a query before the first token, gets zeros. A weight is rounded by 2^-35 of the
+ * row's largest weight, or by 2^-21 of itself where that is more.
  * max_pages_seq, total_pages: upper bounds of any sequence's pages and of all sequences' together, for the launch's shape.
  * block_pages = NULL: every page. Else (tokens = 1) the pages of sequence b and kv head h are block_pages[(b * kv_heads + h) * n_blocks ..], as
  * many as there are blocks or n_blocks, the last of them the sequence's last page (leankv_byte_select writes such lists).
@@ -91,7 +92,8 @@ typedef struct {
 size_t leankv_byte_attn_workspace_bytes(void);       /* the same for all shapes */
 int leankv_byte_attn(const leankv_byte_attn_t* a /* host */, void* stream);
 /* The same for longer chunks of prompts, on tcgen05 (256 (token, head) rows against 128 keys at a time); q and out fp16 or bf16 (fp32:
- * LEANKV_EUNSUPPORTED), scale > 0, block_pages NULL. Weights enter the value product as fp16. */
+ * LEANKV_EUNSUPPORTED), scale > 0, block_pages NULL. Each term of a row's output (weight times value) is rounded by 2^-11 of itself at most, where
+ * leankv_byte_attn keeps 21 bits, or by 2^-24 of the row's largest term; values that a row does not see have no part in it. */
 int leankv_byte_prompt_attn(const leankv_byte_attn_t* a /* host */, void* stream);
 
 /* The blocks that one query token of each sequence reads, for each kv head: all of them where there are no more than n_blocks; else the

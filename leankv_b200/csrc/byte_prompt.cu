@@ -5,20 +5,25 @@
 //   warps 8 - 11  pages from memory into registers a whole key tile ahead; code + 128 behind the byte 0x64 is the fp16 number 1152 + code, one
 //                 fused multiply-add makes it exact (and scales values); 16-byte (8-byte) stores fill core matrices in order
 //   warp 12       S_r = Q_r K^T and O_r += P_r V of both row tiles, one thread issues
-//   warps 13 - 15 ask for pages into L2, then wait
+//   warp 13       the scales of a key tile: the keys' for the rows, the values' exponents for rows and converting warps
+//   warps 14, 15  ask for pages into L2, then wait
 //   warps 0 - 7   a thread a row: scores from tensor memory, maximum, weights back over the scores as fp16
-// A row's 128 scores stay in registers, which the row warps take from the others (of the launch's 128 each: 184, converting warps 96, the last four 48).
+// A row's 128 scores stay in registers, which the row warps take from the others (of the launch's 128 each: 192, converting warps 88, the last four 40).
 // The row tiles alternate: the products of one run under the exponentials of the other. Tensor memory: S of both (128 columns each), O of both (dim each), for dim 64 weights.
 //
 // Exactness. Keys enter as their codes (the scale, one number for 16 keys, is multiplied to the scores in fp32), queries in fp16 with a power of two taken out
-// of each row. Values enter as code * 2^(e - r), r the largest exponent among the CTA's pages: exact down to 2^-24, and a page whose numbers are 2^-25 of
-// the largest page's is lost against it. Weights are fp16 (2^-11), the reference of a row kLift below its maximum so that 2^-21 of the
-// largest weight still has all its places; their sum is fp32 before that rounding.
+// of each row. Values enter as code * 2^(e - t), t the largest exponent of the key tile's pages, exactly; the tile's t goes into the weights, which are
+// 2^(score - m + t - r) against a row's own references: m for its sum, r for the exponents of the values that count for it. So no row depends on values that it
+// does not see, and a row of small ones is as good as any. (One exponent for all pages of the CTA, which was simpler, turned rows of values 2^-25 below a later token's into zeros.) Where the
+// pages of a tile are more than kFlat exponents apart, their codes enter as they are and each page's e goes into its weights; such a tile, or one whose t is far from
+// the row's r, has its exponentials for sums and outputs apart. Weights are fp16 (2^-11), with references such that 2^-21 of a row's largest term still
+// has all its places (2^-13 under a tile whose exponents are kFlat apart); their sum is fp32 before that rounding.
 //
 // Bound: a key tile is 4 x 512 tensor cycles (dim 128) and 2 x 1024 cycles of ex2; operand reads (192 KB) and the converted tiles (64 KB written) take the
 // same time of shared memory's 128 bytes a cycle. It takes some 3600: a row tile's rows have 128 scores for 2400 cycles and then nothing for 1250, until the last weights
 // are multiplied (400) and the next scores formed over them (580, and 270 on the way); two row tiles are what tensor memory holds, and what one leaves the other does not fill.
-// 4096 tokens, 8 kv heads of 4, bf16: 139 us, 990 TFLOP/s; 8192: 476, 1155; 512 behind 3584: 48; dim 64, 4096: 117.
+// 4096 tokens, 8 kv heads of 4, bf16: 144 us, 955 TFLOP/s; 8192, fp16: 482, 1140; 512 behind 3584: 46; dim 64, 4096: 117. (With one exponent a CTA 140, 479, 48, 118: a warp for the
+// scales gives the converting warps back the registers that the rows' second reference takes.)
 //
 // Long caches behind few rows: a cluster's CTAs share the keys of a block of rows, each leaves its sums in its shared memory, and each joins a part of the rows from there
 // (through the workspace and a second kernel: 512 behind 3584 52.4 us). Where a cluster of eight leaves SMs free several clusters share them, and their sums meet in the workspace.
@@ -38,13 +43,16 @@ namespace {
 
 constexpr int kRowsTile = 128, kTiles = 2;
 constexpr int kKeysTile = 128, kPagesTile = kKeysTile / kPage;
-constexpr int kRowWarps = 8, kConvWarps = 4, kMmaWarp = kRowWarps + kConvWarps;
+constexpr int kRowWarps = 8, kConvWarps = 4, kMmaWarp = kRowWarps + kConvWarps, kScaleWarp = kMmaWarp + 1;
 constexpr int kThreads = 512;                         // four warpgroups: registers change hands by warpgroup
 constexpr int kPagesWarp = kPagesTile / kConvWarps;
 constexpr float kNoRef = -3.402823466e38f;            // a maximum before any score: below all of them, and finite, so that masked scores give weight 0
 constexpr float kLift = 7.f, kReach = 15.f;           // the reference of a row is its maximum - kLift when it moves, and moves beyond kReach above it
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kScaleSlots = 4;
+constexpr int kFlat = 8;                              // value scales of a key tile share an exponent if theirs are no further apart: each step costs a row's weights a bit of fp16's range
+constexpr int kPaged = 1024;                          // on top of a tile's exponent: its pages keep their own
+constexpr float kFar = 60.f, kExact = 4194304.f;      // a tile's exponent against the row's, and a row's reference, up to which one exponential serves outputs and sum
 
 __host__ __device__ constexpr uint32_t q_bytes(int dim) { return kRowsTile * dim * 2; }
 __host__ __device__ constexpr uint32_t k_bytes(int dim) { return kKeysTile * dim * 2; }
@@ -89,8 +97,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
     extern __shared__ __align__(16) uint8_t s_raw[];
     __shared__ __align__(8) uint64_t s_bar[kBars];
     __shared__ uint32_t s_tmem;
-    __shared__ int s_top[kConvWarps];
     __shared__ __align__(16) float s_ks[kScaleSlots][kPagesTile];
+    __shared__ float s_ve[kScaleSlots][kPagesTile];                   // the values' exponent of each page
+    __shared__ __half2 s_times[kScaleSlots][kPagesTile];              // what a page's value codes are multiplied with
+    __shared__ float s_tile[kScaleSlots];                             // the largest of a key tile, kPaged more where its pages keep their own
     __shared__ __align__(8) float2 s_ml[kTiles * kRowsTile];          // reference and sum of a row
     __shared__ int s_last;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -105,7 +115,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
 
     if (tid == 0) {
         for (int b = 0; b < kBars; ++b) {
-            const int count = b >= kKFull && b < kKFree ? 32 * kConvWarps : b < kKFull || (b >= kPHalf && b < kPvDone) ? kRowsTile : 1;
+            const int count = b >= kKFull && b < kVFull ? 32 * (kConvWarps + 1) : b >= kVFull && b < kKFree ? 32 * kConvWarps : b < kKFull || (b >= kPHalf && b < kPvDone) ? kRowsTile : 1;
             umma::bar_init_n(bar(b), count);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -137,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
     const bool real = warp < kRowWarps && row < p.tile_tokens * p.G && tok < p.tokens;
     const int head = kvh * p.G + row % p.G;
     if (warp >= kMmaWarp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == kMmaWarp) {
             // ---- products ----
             auto scores = [&](int r, int j) {
@@ -202,25 +212,53 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
                 }
             }
             if (kApart && ok && n > 0) values(1, n - 1);
+        } else if (warp == kScaleWarp) {
+            // ---- scales: lane i < 2 kPagesTile has the values' (the second eight the keys') of page i % kPagesTile of a key tile ----
+            auto scale_of = [&](int j) -> uint32_t {       // as bits; 0: no such page
+                const int i = page0 + j * kPagesTile + lane % kPagesTile;
+                const int id = lane >= 2 * kPagesTile || j >= n || i >= pages ? -1 : p.indices[ip + i];
+                return (unsigned)id >= (unsigned)p.n_pages ? 0u
+                     : __ldg(reinterpret_cast<const uint32_t*>(p.chunks + ((size_t)id * p.H + kvh) * chunk_bytes(D) + 2 * half_bytes(D)) + (lane < kPagesTile ? 1 : 0));
+            };
+            uint32_t scale = scale_of(0);
+            for (int j = 0; j < n && ok; ++j) {
+                if (j >= 2) ok = all(wait2(kKFree, j - 2));
+                if (!ok) break;
+                const uint32_t next = scale_of(j + 1);
+                // the values' exponents, of pages that are there and hold numbers
+                const bool counts = lane < kPagesTile && scale - 1u < 0x7f7fffffu;
+                const int e = (int)(scale >> 23) - 127, slot = j & (kScaleSlots - 1);
+                const int top = __reduce_max_sync(0xffffffffu, counts ? e : -127);
+                const bool flat = top - __reduce_min_sync(0xffffffffu, counts ? e : top) <= kFlat;
+                const uint32_t key_scale = __shfl_down_sync(0xffffffffu, scale, kPagesTile);
+                if (lane < kPagesTile) {
+                    s_ks[slot][lane] = __uint_as_float(scale > 0x7f800000u ? scale : key_scale);
+                    s_ve[slot][lane] = counts ? (float)(flat ? top : e) : -1000.f;
+                    // 2^(e - top) in fp16, 1 where the pages keep their own; 0 for a scale that is no number (its codes are zeros)
+                    s_times[slot][lane] = __half2half2(__ushort_as_half((unsigned short)(!counts ? 0 : flat ? (e - top + 15) << 10 : 0x3c00)));
+                    if (lane == 0) s_tile[slot] = (float)(flat ? top : top + kPaged);
+                }
+                umma::bar_arrive(bar(kKFull + (j & 1)));
+                scale = next;
+            }
         } else if ((int)blockIdx.y < p.first_blocks) {
             // ---- the CTAs that start together walk the same pages: each asks for a part of them into L2 (4096 tokens of six caches in turn 150 -> 145 us) ----
-            constexpr int kAskers = kThreads - 32 * (kMmaWarp + 1);
+            constexpr int kAskers = kThreads - 32 * (kScaleWarp + 1);
             const int to = kShared ? min(page0 + n * kPagesTile, pages) : pages;
-            for (int i = page0 + blockIdx.y + p.first_blocks * (tid - 32 * (kMmaWarp + 1)); i < to; i += p.first_blocks * kAskers) {
+            for (int i = page0 + blockIdx.y + p.first_blocks * (tid - 32 * (kScaleWarp + 1)); i < to; i += p.first_blocks * kAskers) {
                 const int id = p.indices[ip + i];
                 if ((unsigned)id < (unsigned)p.n_pages)
                     asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.chunks + ((size_t)id * p.H + kvh) * chunk_bytes(D)), "r"(chunk_bytes(D)) : "memory");
             }
         }
     } else if (warp >= kRowWarps) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         // ---- codes to operands: a warp has pages kPagesWarp w .. of every key tile ----
         const int first = (warp - kRowWarps) * kPagesWarp;
         // values: lanes of half a warp have eight channels of the same tokens' half, so that their stores fill a core matrix
         const int g = lane >> 1 & 7, t = 2 * (lane >> 4) + (lane & 1);
         constexpr int kLoads = D / 32;                // 16-byte pieces of a lane, of keys and of values
         uint4 kr[kPagesWarp][kLoads], vr[kPagesWarp][kLoads];
-        float2 sc[kPagesWarp];
         auto page_of = [&](int j) -> int {            // lane i < kPagesWarp: page id of key tile j, or -1
             const int i = page0 + j * kPagesTile + first + lane;
             if (lane >= kPagesWarp || j >= n || i >= pages) return -1;
@@ -241,7 +279,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
 #pragma unroll
             for (int x = 0; x < kLoads; ++x)
                 kr[i][x] = chunk == nullptr ? none : __ldg(reinterpret_cast<const uint4*>(chunk + (x >> 1) * 1024 + token_at(8 * (x & 1) + (lane & 7)) * 64 + (lane >> 3) * 16));
-            sc[i] = chunk == nullptr ? make_float2(0.f, 0.f) : __ldg(reinterpret_cast<const float2*>(chunk + 2 * half_bytes(D)));
         };
         auto load_values = [&](const uint8_t* chunk, int i) {
 #pragma unroll
@@ -249,31 +286,19 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
                 vr[i][x] = chunk == nullptr ? none : __ldg(reinterpret_cast<const uint4*>(chunk + half_bytes(D)) + x * 32 + 4 * g + t);
         };
         int ids = page_of(0), ids_next = page_of(1);
-        // the values' scales of the CTA's pages: a thread's first two are asked for now
-        const int to = min(page0 + n * kPagesTile, pages);
-        auto page_id = [&](int i) { return i < to ? p.indices[ip + i] : -1; };
-        auto value_scale = [&](int id) {
-            return (unsigned)id >= (unsigned)p.n_pages ? 0u : __ldg(reinterpret_cast<const uint32_t*>(p.chunks + ((size_t)id * p.H + kvh) * chunk_bytes(D) + 2 * half_bytes(D) + 4));
-        };
-        constexpr int kConvThreads = 32 * kConvWarps;
-        const int own = page0 + tid - 32 * kRowWarps;
-        const int id0 = page_id(own), id1 = page_id(own + kConvThreads);
 #pragma unroll
         for (int i = 0; i < kPagesWarp; ++i) {
             const uint8_t* chunk = chunk_of(ids, i);
             load_keys(chunk, i);
             load_values(chunk, i);
         }
-        const uint32_t scale0 = value_scale(id0), scale1 = value_scale(id1);
         const __half2 one = __half2half2(__ushort_as_half(0x3c00)), minus = __half2half2(__ushort_as_half(0xe480));      // 1, -1152
-        int top = 1;                                  // biased exponent
         for (int j = 0; j < n && ok; ++j) {
             if (j >= 2) ok = all(wait2(kKFree, j - 2));
             if (!ok) break;
             ids = ids_next;
             ids_next = page_of(j + 2);
             uint8_t* k_to = s_k + (j & 1) * k_bytes(D);
-            float vs[kPagesWarp];
 #pragma unroll
             for (int i = 0; i < kPagesWarp; ++i) {
 #pragma unroll
@@ -287,38 +312,16 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
                             make_uint4(codes_times(a, 0x4140, one, minus), codes_times(a, 0x4342, one, minus), codes_times(c, 0x4140, one, minus), codes_times(c, 0x4342, one, minus));
                     }
                 }
-                vs[i] = sc[i].y;
-                if (lane == 0) s_ks[j & (kScaleSlots - 1)][first + i] = isnan(sc[i].y) ? sc[i].y : sc[i].x;
                 load_keys(chunk_of(ids, i), i);
             }
             umma::fence_operands();
             umma::bar_arrive(bar(kKFull + (j & 1)));
-            if (j == 0) {
-                // ---- the largest exponent of the values that this CTA will see ----
-                int e = 1;
-                auto look = [&](uint32_t s) {
-                    if (s < 0x7f800000u) e = max(e, (int)(s >> 23));
-                };
-                look(scale0);
-                look(scale1);
-#pragma unroll 4
-                for (int i = own + 2 * kConvThreads; i < to; i += kConvThreads) look(value_scale(page_id(i)));
-                e = __reduce_max_sync(0xffffffffu, e);
-                if (lane == 0) s_top[warp - kRowWarps] = e;
-                asm volatile("bar.sync 1, %0;" ::"n"(32 * kConvWarps) : "memory");
-#pragma unroll
-                for (int w = 0; w < kConvWarps; ++w) top = max(top, s_top[w]);
-            }
-            if (j >= 2) ok = all(wait2(kVFree, j - 2));
+            ok = all(wait2(kKFull, j) && (j < 2 || wait2(kVFree, j - 2)));             // the first for the scales
             if (!ok) break;
             uint8_t* v_to = s_v + (j & 1) * k_bytes(D);
 #pragma unroll
             for (int i = 0; i < kPagesWarp; ++i) {
-                // 2^(e - r) in fp16: 0 below 2^-24, and for a scale that is no number (its codes are zeros)
-                const int e = (int)(__float_as_uint(vs[i]) >> 23) - top;
-                const uint32_t bits = e > 0 || e < -24 ? 0u : e >= -14 ? (uint32_t)(e + 15) << 10 : 1u << (e + 24);
-                const __half2 s = __half2half2(__ushort_as_half((unsigned short)bits));
-                const __half2 off = __hmul2(s, minus);
+                const __half2 s = s_times[j & (kScaleSlots - 1)][first + i], off = __hmul2(s, minus);
 #pragma unroll
                 for (int x = 0; x < kLoads; ++x) {
                     const uint32_t w[4] = {vr[i][x].x, vr[i][x].y, vr[i][x].z, vr[i][x].w};
@@ -333,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
             umma::bar_arrive(bar(kVFull + (j & 1)));
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
         // ---- queries: a thread a row, fp16 with the row's power of two taken out ----
         uint8_t* q_to = s_q + tile * q_bytes(D);
         // a warp's 32 rows come by whole vectors and turn to a row a thread through where they will lie (a thread that asks for its own row's pieces: 32 rows in one load)
@@ -386,7 +389,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
         umma::bar_arrive(bar(kQFull + tile));
 
         // ---- rows ----
-        float m = kNoRef, l = 0.f;
+        // O = sum 2^(score - m - r) value, l = sum 2^(score - m). m and r are whole numbers, so that the tile's t - r is exact beside a score - m
+        float m = kNoRef, r = 0.f, l = 0.f;
+        bool large = false;                            // some row's m is beyond kExact
         const int lane0 = 32 * (warp & 3);
         const int qpos = start + (real ? tok : last_tok);       // rows that are none see what the last token sees; nothing of theirs is kept
         const uint32_t tm = tm_s + tile * kKeysTile, tp = tm_p + tile * kPColumns, to = tm_o + tile * D;
@@ -434,13 +439,52 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
                 if (j > 0) ok = all(wait1(kPvDone + tile, j - 1));
                 umma::fence_after_sync();
             }
-            const bool raise = best > m + kReach;
-            if (__any_sync(0xffffffffu, raise)) {
-                // nothing is being added to these outputs: the scores were asked for behind the last value product
-                const float now = raise ? best - kLift : m, f = ex2(m - now);
-                m = now;
-                l *= f;
-                if (j > 0) scale_outputs(to, lane0, D, f);
+            // one exponential a weight, 2^(score - m + t - r); the tile's sum of them, times 2^(r - t), is its part of l
+            const float of_tile = s_tile[j & (kScaleSlots - 1)];
+            float less = (of_tile - r) - m, back_to_l = ex2(r - of_tile);
+            if (__builtin_expect(__any_sync(0xffffffffu, best - m > kReach - fmaxf(of_tile - r, 0.f) || fabsf(of_tile - r) > kFar || large), 0)) {
+                const float* ve = s_ve[j & (kScaleSlots - 1)];
+                const bool paged = of_tile > 0.5f * kPaged;
+                float e = of_tile;
+                if (__builtin_expect(paged, 0)) {      // the exponent of the pages that count the most for this row
+                    float most = kNoRef;
+#pragma unroll
+                    for (int i = 0; i < kPagesTile; ++i) {
+                        float top = -INFINITY;
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) top = fmaxf(top, __uint_as_float(s[i >> 1][16 * (i & 1) + x]));
+                        most = fmaxf(most, (__fmul_rn(top, ks[i]) - best) + ve[i]);      // -inf for a page that the row does not see
+                    }
+                    e = ceilf(most);
+                }
+                const bool raise = best - m > kReach - fmaxf(e - r, 0.f);
+                if (__any_sync(0xffffffffu, raise)) {
+                    // nothing is being added to these outputs: the scores were asked for behind the last value product
+                    const float now = raise ? fmaxf(m, floorf(best) - kLift) : m, up = now - m;
+                    const float r_now = raise ? fmaxf(r - up, floorf(best - now) + e - kLift) : r, f = ex2((r - r_now) - up);
+                    l *= ex2(-up);
+                    m = now;
+                    r = r_now;
+                    if (j > 0) scale_outputs(to, lane0, D, f);
+                    large = __any_sync(0xffffffffu, m != kNoRef && fabsf(m) > kExact);
+                    less = (of_tile - r) - m;
+                    back_to_l = ex2(r - of_tile);
+                }
+                if (__builtin_expect(paged || large || __any_sync(0xffffffffu, fabsf(of_tile - r) > kFar), 0)) {
+                    // sums here, and scores that have their page's exponent less r already. Products rounded as the maximum's was: what a fused one has more of a score
+                    // beyond kExact may be many powers of two
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) {
+                            const float at = __uint_as_float(s[c][x]), w = __fmul_rn(at, ks[2 * c + (x >> 4)]) - m;
+                            if (at != -INFINITY) l += ex2(w);
+                            s[c][x] = __float_as_uint(w + (ve[2 * c + (x >> 4)] - r));
+                        }
+#pragma unroll
+                    for (int i = 0; i < kPagesTile; ++i) ks[i] = 1.f;
+                    less = back_to_l = 0.f;
+                }
             }
             Two sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
             // the masked form apart from the other: one loop for both spends two instructions a weight on masks that are not there
@@ -451,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
 #pragma unroll
                     for (int x = 0; x < 32; x += 2) {
                         const float k = ks[2 * c + (x >> 4)];
-                        Two w = fma2({__uint_as_float(s[c][x]), __uint_as_float(s[c][x + 1])}, {k, k}, {-m, -m});
+                        Two w = fma2({__uint_as_float(s[c][x]), __uint_as_float(s[c][x + 1])}, {k, k}, {less, less});
                         w.x = ex2(w.x);
                         w.y = ex2(w.y);
                         if constexpr (decltype(masked)::value) {         // a scale that is no number does not reach a row that does not see its block
@@ -472,22 +516,19 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
             };
             if (cut) weights(std::true_type());
             else weights(std::false_type());
-            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+            l = fmaf((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y), back_to_l, l);
             umma::stored();
             if (j + 1 < n) ok = all(wait2(kKFull, j + 1));
             umma::fence_before_sync();
             umma::bar_arrive(bar(kPFull + tile));
         }
-        if (ok && n > 0) ok = all(wait1(kPvDone + tile, n - 1) && wait2(kVFull, n - 1));       // the second for the values' largest exponent
+        if (ok && n > 0) ok = all(wait1(kPvDone + tile, n - 1));
         umma::fence_after_sync();
         if (!ok && lane == 0) atomicOr(p.status, kTimedOut);
 
         // ---- out ----
         const float inv = !ok ? NAN : l == 0.f ? 0.f : 1.f / l;
-        int top = 1;
-#pragma unroll
-        for (int w = 0; w < kConvWarps; ++w) top = n > 0 ? max(top, s_top[w]) : 1;
-        const float back = __uint_as_float((uint32_t)top << 23);
+        const float back = r < -126.f ? ex2(r + 64.f) * 5.421010862427522e-20f : ex2(r);       // 2^r, 2^-64 of it apart where r is below fp32's exponents
         const int reciprocal = (65535 + p.G) / p.G;   // i / G is i * reciprocal >> 16 for i below 128
         auto target = [&](int r) -> T* {              // where row r of the CTA's 256 goes, or null
             const int in_tile = r & (kRowsTile - 1), in_tok = in_tile * reciprocal >> 16, r_tok = tok0 + (r / kRowsTile) * p.tile_tokens + in_tok;

@@ -359,6 +359,54 @@ def test_prompt_attention_on_values_of_different_magnitudes(scale):
     p.check_prompt(200)
 
 
+@pytest.mark.parametrize("kind, dtype, dim, group, heads, past, tokens", [
+    ("later", BF16, 128, 4, 1, 0, 300), ("later", F16, 64, 4, 2, 0, 200), ("later", BF16, 64, 3, 1, 37, 700), ("mixed", BF16, 64, 2, 1, 90, 150),
+    ("mixed", BF16, 128, 4, 1, 0, 600), ("mixed", BF16, 128, 16, 1, 2000, 40), ("mixed", BF16, 128, 4, 1, 8200, 20), ("outweighed", BF16, 64, 7, 1, 500, 130),
+    ("outweighed", BF16, 128, 4, 1, 0, 700), ("zeros", BF16, 128, 4, 1, 0, 500), ("zeros", F16, 64, 2, 1, 3000, 30), ("far", BF16, 128, 2, 1, 0, 400),
+    ("far", BF16, 64, 2, 1, 1100, 30), ("far, near", BF16, 128, 2, 1, 0, 400), ("far, near", BF16, 64, 2, 1, 1100, 30), ("cliff", BF16, 64, 4, 1, 0, 400),
+    ("cliff", BF16, 128, 2, 1, 1000, 50)])
+def test_a_prompt_row_goes_by_the_values_that_it_sees(kind, dtype, dim, group, heads, past, tokens):
+    """Values of any spread: a row of small ones ahead of a later token's large ones; large ones whose weights leave the small ones what counts; blocks
+    of zeros that take weight. A term is 2^-11 off for its weight's rounding, whatever its value, or 2^-24 of the row's largest term: the bound that ``close`` has."""
+    n = past + tokens
+    p = Pair(1, heads, group, dim, dtype, pages=n // 16 + 2, seed=n + dim)
+    k, v = (vectors(p.gen, 1, heads, n, dim, F32, large=False) for _ in range(2))
+    q = p.queries(tokens)
+    block = torch.arange(n) // 16
+    if kind == "later":
+        small, large = (2.0 ** -10, 2.0 ** 13) if dtype == F16 else (2.0 ** -20, 2.0 ** 40)
+        v *= torch.where((block % 7 == 6) | (torch.arange(n) == n - 1), large, small)[:, None]
+    elif kind == "mixed":
+        sizes = torch.tensor([-60.0, -30.0, -9.0, 0.0, 0.0, 13.0, 40.0])
+        v *= torch.exp2(sizes[torch.randint(0, 7, (n // 16 + 1,), generator=p.gen)])[block][:, None]
+    elif kind == "outweighed":                         # every third block: values of 2^40 under scores some 28 (40 powers of two) lower
+        k[..., 0] = torch.where(block % 3 == 1, -28.0, 0.0)
+        q[..., 0] = dim ** 0.5
+        v *= torch.where(block % 3 == 1, 2.0 ** 40, 1.0)[:, None]
+    elif kind == "cliff":                              # beyond the first key tile scores 710 lower, 2^-1024, of values 2^60 apart
+        k[..., 0] = torch.where(torch.arange(n) < 128, 0.0, -710.0)
+        q[..., 0] = dim ** 0.5
+        v *= torch.exp2(30.0 - 60 * (block % 2))[:, None]
+    elif kind == "zeros":
+        v *= (block % 40 >= 20).float()[:, None]
+    else:                                              # products of -1e36: the first token is all that counts
+        k = -torch.exp2(60.0 + (torch.arange(n) * 7 % 5))[None, None, :, None].expand(1, 1, -1, dim).contiguous()
+        k[0, 0, 1:] *= 2
+        q = torch.full((1, 2, tokens, dim), 2.0 ** 56).to(dtype)
+        v *= (torch.where(block == 0, 1.0, torch.exp2(30.0 - 60 * (block % 2))) if kind == "far" else torch.exp2(2.0 * (block % 4)))[:, None]
+    k, v = k.to(dtype), v.to(dtype)
+    p.cache.append(0, k.to(DEV), v.to(DEV))
+    p.plain.append(k, v)
+    want = p.plain.attend(0, q[0])[None]
+    p.cache._prompt_work = 0
+    got = p.cache.prefill_attention(0, q.to(DEV))
+    close(got, want, dtype, weights=True)
+    assert torch.equal(p.cache.prefill_attention(0, q.to(DEV)), got) and p.cache.kernel_status() == 0
+    if kind in ("later", "zeros"):
+        p.cache._prompt_work = 1 << 60
+        close(p.cache.prefill_attention(0, q.to(DEV)), want, dtype)
+
+
 def test_prompt_attention_of_rows_whose_reference_moves():
     """Scores that rise from key tile to key tile, beyond what weights in fp16 reach."""
     p = Pair(1, 1, 4, 64, BF16, pages=80)
