@@ -320,9 +320,10 @@ __global__ void __launch_bounds__(kThreads, 4) attn_kernel(const AttnParams p) {
         for (int n8 = 0; n8 < kTiles; ++n8) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {          // token g + 8 (e >> 1), row 2t + (e & 1)
-                sc[n8][e] *= ks * factor[n8][e & 1];
+                // rounded by itself: fused with the weight's subtraction, its last places would be powers of two of a large score
+                sc[n8][e] = __fmul_rn(sc[n8][e], ks * factor[n8][e & 1]);
                 if (cut && (bad || first + g + 8 * (e >> 1) > limit[n8][e & 1])) sc[n8][e] = -INFINITY;
-                raise |= sc[n8][e] > m[n8][e & 1] + kReach;
+                raise |= sc[n8][e] > __fadd_rd(m[n8][e & 1], kReach);          // to nearest, m + 15 is m + 16 for numbers around 2^28, a weight beyond fp16
             }
         }
         if (__any_sync(0xffffffffu, raise)) {
@@ -333,9 +334,10 @@ __global__ void __launch_bounds__(kThreads, 4) attn_kernel(const AttnParams p) {
                     float best = fmaxf(sc[n8][e], sc[n8][e + 2]);
 #pragma unroll
                     for (int x = 4; x < 32; x *= 2) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, x));
-                    if (best - kLift > m[n8][e]) {
-                        const float down = ex2(m[n8][e] - (best - kLift));
-                        m[n8][e] = best - kLift;
+                    const float now = __fadd_ru(best, -kLift);
+                    if (now > m[n8][e]) {
+                        const float down = ex2(m[n8][e] - now);
+                        m[n8][e] = now;
                         l[n8][e] *= down;
 #pragma unroll
                         for (int k = 0; k < kSteps; ++k) {

@@ -470,6 +470,35 @@ def test_scores_far_below_zero_are_scores(dtype, dim, past):
         close(p.cache.prefill_attention(0, q.to(DEV)), want, dtype, weights=work == 0)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("power", [16, 20, 23, 25, 27, 28, 29, 30, 31, 34, 45, 60])
+def test_scores_of_any_size_choose_a_token(dtype, power):
+    """Scores of 2^power: a product's rounding, 2^-24 of it, is many powers of two. Keys are random signs times a size each, queries some of the keys, so that a row's first
+    two scores are further apart than any rounding and the answer is the first one's value."""
+    p = Pair(1, 1, 4, 64, dtype, pages=60)
+    n = 600
+    k = torch.sign(torch.randn(1, 1, n, 64, generator=p.gen)) * (0.3 + 0.7 * torch.rand(1, 1, n, 1, generator=p.gen)) * 2.0 ** (power // 2)
+    v = vectors(p.gen, 1, 1, n, 64, dtype, large=False)
+    p.cache.append(0, k.to(dtype).to(DEV), v.to(DEV))
+    p.plain.append(k.to(dtype), v)
+    held = p.plain.values(0, 0)[0]
+    at = torch.randint(0, n - 40, (1, 4, 40), generator=p.gen)
+    q = (held[at] / 2.0 ** (power // 2) * 2.0 ** (power - power // 2) / 8).to(dtype)        # rows that ask for one of the tokens
+    scores = torch.einsum("hqd,kd->hqk", q[0].double(), held) / 8
+    top = scores.topk(2, -1).values
+    clear = (top[..., 0] - top[..., 1]) > 2.0 ** -18 * top[..., 0].abs() + 64               # far beyond what 32 bits round
+    assert float(clear.double().mean()) > 0.9
+    want = p.plain.attend(0, q[0])[None]
+    p.cache._prompt_work = 1 << 60
+    last = p.cache.decode_attention(0, q[:, :, -1].to(DEV))
+    close(last[:, clear[:, -1]], want[:, :, -1][:, clear[:, -1]], dtype)
+    for work in (0, 1 << 60):
+        p.cache._prompt_work = work
+        got = p.cache.prefill_attention(0, q.to(DEV))
+        close(got[:, clear], want[:, clear], dtype, weights=work == 0)
+    assert p.cache.kernel_status() == 0
+
+
 def test_queries_of_any_scale():
     for dtype, scale in ((BF16, 1e-30), (BF16, 1e4), (F32, 1e-35), (F32, 1e-3), (F16, 1e-4)):
         p = Pair(1, 2, 3, 64, dtype)
