@@ -143,11 +143,10 @@ __global__ void __launch_bounds__(kScoreThreads) score_kernel(const SelectParams
     }
 }
 
-// fp32 numbers as whole numbers in the same order; every NaN is the one number above infinity. (A product with NaN is 0x7fffffff whatever NaN came in:
-// in the numbers' own order that is the last of 32 bits, and a range of keys that began there would end at zero.)
+// fp32 numbers as whole numbers in the same order; a product with NaN, which is 0x7fffffff, is the largest of 32 bits.
 __device__ __forceinline__ uint32_t ordered(float v) {
     const uint32_t x = __float_as_uint(v);
-    return isnan(v) ? 0xff800001u : x ^ ((x >> 31) ? 0xffffffffu : 0x80000000u);
+    return x ^ ((x >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
 template <int kThreads>
@@ -243,7 +242,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) 
             room -= s_above;
             low += (uint32_t)s_at << shift;
             if (shift == 0 || s_in == room) break;
-            high = low + min(high - low, (1u << shift) - 1u);
+            high = low + min(high - low, (1u << shift) - 1u);          // not beyond the range before: with NaN in it that would end at zero
         }
         border = low;
         // a bin that is chosen whole: everything from its lower end on
@@ -265,7 +264,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) 
             if (lane == 0) s_rank[i * kWarps + warp] = (uint32_t)__popc(in[i]) | (uint32_t)__popc(at[i]) << 16;
         }
         __syncthreads();
-        // kPer * kWarps sums: two of a thread at most; counts of a slab stay below 2^16
+        // kPer * kWarps sums, one of a thread at most; counts of a slab stay below 2^16
         constexpr int kSums = kPer * kWarps;
         static_assert(kSums <= kThreads, "one sum of a thread");
         uint32_t mine = tid < kSums ? s_rank[tid] : 0u, incl = mine;
@@ -292,7 +291,6 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) 
             const int n_in = base + (int)(r & 0xffffu) + __popc(in[i] & lanes), n_at = base_at + (int)(r >> 16) + __popc(at[i] & lanes);
             if (!is_in && n_at >= room) continue;
             const int j = slab * kSlab + i * kThreads + tid, to = n_in + min(n_at, room);
-            if (to >= p.n_blocks) continue;        // never: the list is another pair's from there on
             blocks[to] = j;
             block_pages[to] = p.indices[ip + j];
         }
