@@ -148,13 +148,13 @@ class ByteKVCache(PagedKVCache):
             self._begin_args = (ctypes.c_void_p(store.data_ptr()), sum(padded[:6]), self.max_pages, sum(padded[:7]))
             self._begin(store)
             self._meta_batch = 0                             # sequences that the flat arrays were built for; -1: they are not the table's
-            self._block_table = torch.zeros(self._batch_cap, self._pps_cap, dtype=i32, device=dev)
             for args in self._args:
                 for a in args:
                     a[0].kv_indptr, a[0].kv_page_indices = self._kv_indptr.data_ptr(), self._kv_page_indices.data_ptr()
                 args[0][0].kv_last_page_len = args[1][0].kv_last_page_len = self._kv_last.data_ptr()
-        else:
-            self._block_table = torch.zeros(self._batch_cap, self._pps_cap, dtype=i32, device=dev)
+        # only places of pages that a sequence holds are read
+        self._block_table = torch.empty(self._batch_cap, self._pps_cap, dtype=i32, device=dev)
+        if table is not None:
             self._block_table[:len(table)] = table
         at = lambda t: ctypes.c_void_p(t.data_ptr())      # converted once, not at every call
         self._step_args = (at(self._seq_len_dev), at(self._block_table), ctypes.c_int(self._pps_cap), at(self._free_stack), at(self._free_top),
@@ -389,7 +389,7 @@ class ByteKVCache(PagedKVCache):
 
     def kernel_status(self) -> int:
         """Status word of the attention's bounded waits and page checks (0 = clean, bit 0: a wait ran out, bit 1: a page id outside
-        the pool)."""
+        the pool, bit 2: a table with more pages than the pool)."""
         val = ctypes.c_int(0)
         if self._workspace.is_cuda:
             with _native.on_device(self._device):
@@ -401,7 +401,8 @@ class ByteKVCache(PagedKVCache):
 
     def crop(self, max_length: int):
         """Cut every sequence back to at most ``max_length`` tokens (below zero: that many tokens fewer than the longest has), as after
-        drafted tokens that were not accepted. The scale of a block that keeps some tokens stays as it is."""
+        drafted tokens that were not accepted. The scale of a block that keeps some tokens stays as it is, a block that holds no number
+        included."""
         if self._device.type == "cuda" and _capturing():
             raise RuntimeError("ByteKVCache: crop changes lengths that the host keeps, too, and cannot be captured")
         if max_length < 0:
