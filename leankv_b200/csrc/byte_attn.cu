@@ -12,8 +12,9 @@
 // fp16 parts, so that nothing on the way is rounded to fewer than 21 bits: with one part the weight of a token that
 // dominates a row would be 2^-12 off, and the products have room for it (the kernel is bound by memory).
 //
-// Bound: a chunk's 2 * 16 * dim + 16 bytes come once from memory. They come by one bulk copy into a ring of a warp's own (4 to 8 chunks ahead), 190 KB in
-// flight on an SM; the tensor cores and some 300 issue slots a page and warp run under that.
+// Bound: a chunk's 2 * 16 * dim + 16 bytes come once from memory. They come by one bulk copy into a ring of a warp's own (3 chunks ahead, 6 for head size 64), 190 KB in
+// flight on an SM; the tensor cores and some 300 issue slots a page and warp run under that. With two groups of eight rows at head size 128 four CTAs an SM take spills of 128 to 160 bytes a
+// thread (fp32 queries 432): 16 x 4096 tokens, 16 heads a kv head 51 us, three CTAs without them 57.
 //
 // Split. A cluster of CTAs has one (sequence, kv head, row tile) triple or, where there are fewer triples than the device has room for clusters, an equal part of
 // its pages; the CTAs share those pages and add their sums up through distributed shared memory, each a slice of the rows. Parts of one triple meet in the workspace:

@@ -38,7 +38,8 @@ __device__ __forceinline__ uint32_t coarser(uint32_t w, float f) {
     return out;
 }
 
-// CTAs an SM: as many as the registers of a page's numbers leave (16 x 2011 tokens, bf16: 5 by the compiler's own choice 43.7 us, 6 41.0, 7 40.3)
+// CTAs an SM. Seven leave the 16-bit types 72 registers at head size 128, for which 32 bytes of a thread are spilled (16 x 2011 tokens, bf16: 5, the compiler's own choice, 43.7 us, 6
+// 41.0, 7 40.3)
 template <typename T, int D>
 __global__ void __launch_bounds__(kWarps * 32, sizeof(T) == 4 ? 4 : D == 128 ? 7 : 9) append_kernel(const AppendParams p) {
     using R = Rows<D>;
