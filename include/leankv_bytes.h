@@ -93,7 +93,8 @@ size_t leankv_byte_attn_workspace_bytes(void);       /* the same for all shapes 
 int leankv_byte_attn(const leankv_byte_attn_t* a /* host */, void* stream);
 /* The same for longer chunks of prompts, on tcgen05 (256 (token, head) rows against 128 keys at a time); q and out fp16 or bf16 (fp32:
  * LEANKV_EUNSUPPORTED), scale > 0, block_pages NULL. Each term of a row's output (weight times value) is rounded by 2^-11 of itself at most, where
- * leankv_byte_attn keeps 21 bits, or by 2^-24 of the row's largest term; values that a row does not see have no part in it. */
+ * leankv_byte_attn keeps 21 bits, or by 2^-24 of its largest weight times the largest number of that token's block where that is more; blocks that a
+ * row does not see have no part in it. */
 int leankv_byte_prompt_attn(const leankv_byte_attn_t* a /* host */, void* stream);
 
 /* The blocks that one query token of each sequence reads, for each kv head: all of them where there are no more than n_blocks; else the

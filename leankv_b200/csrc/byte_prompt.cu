@@ -16,13 +16,14 @@
 // 2^(score - m + t - r) against a row's own references: m for its sum, r for the exponents of the values that count for it. So no row depends on values that it
 // does not see, and a row of small ones is as good as any. (One exponent for all pages of the CTA, which was simpler, turned rows of values 2^-25 below a later token's into zeros.) Where the
 // pages of a tile are more than kFlat exponents apart, their codes enter as they are and each page's e goes into its weights; such a tile, or one whose t is far from
-// the row's r, has its exponentials for sums and outputs apart. Weights are fp16 (2^-11), with references such that 2^-21 of a row's largest term still
-// has all its places (2^-13 under a tile whose exponents are kFlat apart); their sum is fp32 before that rounding.
+// the row's r, has its exponentials for sums and outputs apart. There a token counts for r only if one of its codes is not zero (a block's scale may be another token's, one
+// that the row does not see), and r comes down to where the outputs are when the weights of a later tile would be far below them. Weights are fp16 (2^-11), with references such that 2^-21 of a row's largest term still
+// has all its places (2^-13 under a tile whose exponents are kFlat apart; a row's largest term is its largest weight times that block's scale); their sum is fp32 before that rounding.
 //
 // Bound: a key tile is 4 x 512 tensor cycles (dim 128) and 2 x 1024 cycles of ex2; operand reads (192 KB) and the converted tiles (64 KB written) take the
 // same time of shared memory's 128 bytes a cycle. It takes some 3600: a row tile's rows have 128 scores for 2400 cycles and then nothing for 1250, until the last weights
 // are multiplied (400) and the next scores formed over them (580, and 270 on the way); two row tiles are what tensor memory holds, and what one leaves the other does not fill.
-// 4096 tokens, 8 kv heads of 4, bf16: 144 us, 955 TFLOP/s; 8192, fp16: 482, 1140; 512 behind 3584: 46; dim 64, 4096: 117. (With one exponent a CTA 140, 479, 48, 118: a warp for the
+// 4096 tokens, 8 kv heads of 4, bf16: 145 us, 948 TFLOP/s; 8192, fp16: 490, 1120; 512 behind 3584: 46; dim 64, 4096: 117. (With one exponent a CTA 140, 479, 48, 118: a warp for the
 // scales gives the converting warps back the registers that the rows' second reference takes.)
 //
 // Long caches behind few rows: a cluster's CTAs share the keys of a block of rows, each leaves its sums in its shared memory, and each joins a part of the rows from there
@@ -52,7 +53,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kScaleSlots = 4;
 constexpr int kFlat = 8;                              // value scales of a key tile share an exponent if theirs are no further apart: each step costs a row's weights a bit of fp16's range
 constexpr int kPaged = 1024;                          // on top of a tile's exponent: its pages keep their own
+constexpr float kLeap = 24.f;                         // a tile's exponent less a row's r, beyond which r moves for tokens only that hold more than zeros
 constexpr float kFar = 60.f, kExact = 4194304.f;      // a tile's exponent against the row's, and a row's reference, up to which one exponential serves outputs and sum
+constexpr float kLeast = -1000.f;                     // of r: weights of 2^-1000 and less are none in any type
 
 __host__ __device__ constexpr uint32_t q_bytes(int dim) { return kRowsTile * dim * 2; }
 __host__ __device__ constexpr uint32_t k_bytes(int dim) { return kKeysTile * dim * 2; }
@@ -391,6 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
         // ---- rows ----
         // O = sum 2^(score - m - r) value, l = sum 2^(score - m). m and r are whole numbers, so that the tile's t - r is exact beside a score - m
         float m = kNoRef, r = 0.f, l = 0.f;
+        float lowest = -kFlat;                         // a tile's exponent less r, below which r is looked at again
         bool large = false;                            // some row's m is beyond kExact
         const int lane0 = 32 * (warp & 3);
         const int qpos = start + (real ? tok : last_tok);       // rows that are none see what the last token sees; nothing of theirs is kept
@@ -442,26 +446,71 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
             // one exponential a weight, 2^(score - m + t - r); the tile's sum of them, times 2^(r - t), is its part of l
             const float of_tile = s_tile[j & (kScaleSlots - 1)];
             float less = (of_tile - r) - m, back_to_l = ex2(r - of_tile);
-            if (__builtin_expect(__any_sync(0xffffffffu, best - m > kReach - fmaxf(of_tile - r, 0.f) || fabsf(of_tile - r) > kFar || large), 0)) {
+            if (__builtin_expect(__any_sync(0xffffffffu, best - m > kReach - fmaxf(of_tile - r, 0.f) || of_tile - r > kFar || of_tile - r < lowest || large), 0)) {
                 const float* ve = s_ve[j & (kScaleSlots - 1)];
-                const bool paged = of_tile > 0.5f * kPaged;
+                // where the exponents would move r far, only tokens with a code that is not zero count
+                const bool paged = of_tile > 0.5f * kPaged, sparse = paged || __any_sync(0xffffffffu, of_tile - r > kLeap);
                 float e = of_tile;
-                if (__builtin_expect(paged, 0)) {      // the exponent of the pages that count the most for this row
+                uint32_t eight = 0;
+                auto filled_of = [&](int c) {          // tokens 32 c .. as bits
+                    uint32_t bits = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) bits |= __shfl_sync(0xffffffffu, eight, 4 * c + i) << 8 * i;
+                    return bits;
+                };
+                if (__builtin_expect(sparse, 0)) {
+                    if (!all(wait2(kVFull, j))) l = NAN;       // (the converting warps report it)
+                    const uint8_t* from = s_v + (j & 1) * k_bytes(D) + (lane & 15) * umma::kLbo + (lane >> 4) * (D / 16) * (kKeysTile / 8) * umma::kLbo;
+                    uint4 any = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+                    for (int i = 0; i < D / 2; ++i) {              // eight tokens of a channel
+                        const uint4 w = *reinterpret_cast<const uint4*>(from + (i >> 3) * (kKeysTile / 8) * umma::kLbo + ((i + lane) & 7) * 16);
+                        any.x |= w.x, any.y |= w.y, any.z |= w.z, any.w |= w.w;
+                    }
+                    const uint32_t words[4] = {any.x, any.y, any.z, any.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) eight |= (min(words[i] & 0x7fffu, 1u) | min(words[i] >> 16 & 0x7fffu, 1u) << 1) << 2 * i;
+                    eight |= __shfl_xor_sync(0xffffffffu, eight, 16);
                     float most = kNoRef;
 #pragma unroll
-                    for (int i = 0; i < kPagesTile; ++i) {
-                        float top = -INFINITY;
+                    for (int c = 0; c < 4; ++c) {
+                        const uint32_t filled = filled_of(c);
 #pragma unroll
-                        for (int x = 0; x < 16; ++x) top = fmaxf(top, __uint_as_float(s[i >> 1][16 * (i & 1) + x]));
-                        most = fmaxf(most, (__fmul_rn(top, ks[i]) - best) + ve[i]);      // -inf for a page that the row does not see
+                        for (int half = 0; half < 2; ++half) {
+                            float top = -INFINITY;
+#pragma unroll
+                            for (int x = 16 * half; x < 16 * half + 16; ++x) {
+                                const uint32_t keep = (uint32_t)((int)(filled << (31 - x)) >> 31);
+                                top = fmaxf(top, __uint_as_float((s[c][x] & keep) | (0xff800000u & ~keep)));
+                            }
+                            most = fmaxf(most, (__fmul_rn(top, ks[2 * c + half]) - best) + ve[2 * c + half]);      // -inf for a page that the row does not see
+                        }
                     }
                     e = ceilf(most);
                 }
-                const bool raise = best - m > kReach - fmaxf(e - r, 0.f);
-                if (__any_sync(0xffffffffu, raise)) {
+                const bool raise = best - m > kReach - fmaxf(e - r, 0.f), sink = !raise && j > 0 && e > kNoRef && e - r < lowest && best > kNoRef;
+                const float now = raise ? fmaxf(m, floorf(best) - kLift) : m, up = now - m, fit = floorf(best - now) + e - kLift;
+                float r_now = raise ? fmaxf(fmaxf(r - up, fit), kLeast) : r;
+                if (raise) lowest = -kFlat;
+                if (__any_sync(0xffffffffu, sink)) {
+                    // weights far down: r may come from tokens that turned out to add little. Not below where the outputs are
+                    uint32_t top = 0;
+#pragma unroll 1
+                    for (int c0 = 0; c0 < D; c0 += 16) {
+                        uint32_t o[16];
+                        umma::ld16(o, to, lane0, c0);
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) top = max(top, o[x] & 0x7fffffffu);
+                    }
+                    const float there = top == 0 ? kNoRef : r + (float)((int)(top >> 23) - 127) - kLift;
+                    if (sink) {
+                        r_now = fminf(r, fmaxf(fmaxf(fit, there), kLeast));
+                        if (there >= fit) lowest = -kFar;          // r is where the outputs are
+                    }
+                }
+                if (__any_sync(0xffffffffu, raise || r_now != r)) {
                     // nothing is being added to these outputs: the scores were asked for behind the last value product
-                    const float now = raise ? fmaxf(m, floorf(best) - kLift) : m, up = now - m;
-                    const float r_now = raise ? fmaxf(r - up, floorf(best - now) + e - kLift) : r, f = ex2((r - r_now) - up);
+                    const float f = ex2((r - r_now) - up);
                     l *= ex2(-up);
                     m = now;
                     r = r_now;
@@ -470,17 +519,29 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const PromptParams 
                     less = (of_tile - r) - m;
                     back_to_l = ex2(r - of_tile);
                 }
-                if (__builtin_expect(paged || large || __any_sync(0xffffffffu, fabsf(of_tile - r) > kFar), 0)) {
+                if (__builtin_expect(sparse || large || __any_sync(0xffffffffu, fabsf(of_tile - r) > kFar), 0)) {
                     // sums here, and scores that have their page's exponent less r already. Products rounded as the maximum's was: what a fused one has more of a score
                     // beyond kExact may be many powers of two
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                    for (int c = 0; c < 4; ++c) {
 #pragma unroll
                         for (int x = 0; x < 32; ++x) {
                             const float at = __uint_as_float(s[c][x]), w = __fmul_rn(at, ks[2 * c + (x >> 4)]) - m;
                             if (at != -INFINITY) l += ex2(w);
                             s[c][x] = __float_as_uint(w + (ve[2 * c + (x >> 4)] - r));
                         }
+                    }
+                    if (sparse) {                      // weights of what is zero are of no use, and may be beyond fp16
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const uint32_t filled = filled_of(c);
+#pragma unroll
+                            for (int x = 0; x < 32; ++x) {
+                                const uint32_t keep = (uint32_t)((int)(filled << (31 - x)) >> 31);
+                                s[c][x] = (s[c][x] & keep) | (0xff800000u & ~keep);
+                            }
+                        }
+                    }
 #pragma unroll
                     for (int i = 0; i < kPagesTile; ++i) ks[i] = 1.f;
                     less = back_to_l = 0.f;

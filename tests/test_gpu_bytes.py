@@ -364,10 +364,13 @@ def test_prompt_attention_on_values_of_different_magnitudes(scale):
     ("mixed", BF16, 128, 4, 1, 0, 600), ("mixed", BF16, 128, 16, 1, 2000, 40), ("mixed", BF16, 128, 4, 1, 8200, 20), ("outweighed", BF16, 64, 7, 1, 500, 130),
     ("outweighed", BF16, 128, 4, 1, 0, 700), ("zeros", BF16, 128, 4, 1, 0, 500), ("zeros", F16, 64, 2, 1, 3000, 30), ("far", BF16, 128, 2, 1, 0, 400),
     ("far", BF16, 64, 2, 1, 1100, 30), ("far, near", BF16, 128, 2, 1, 0, 400), ("far, near", BF16, 64, 2, 1, 1100, 30), ("cliff", BF16, 64, 4, 1, 0, 400),
-    ("cliff", BF16, 128, 2, 1, 1000, 50)])
+    ("cliff", BF16, 128, 2, 1, 1000, 50), ("own block", BF16, 64, 2, 1, 0, 270), ("own block", BF16, 128, 4, 1, 600, 30), ("own block", BF16, 64, 2, 1, 1390, 30),
+    ("rare", BF16, 128, 4, 1, 0, 500), ("rare", BF16, 64, 3, 1, 1700, 40), ("first", BF16, 128, 2, 1, 0, 420), ("first", BF16, 64, 4, 1, 1500, 30),
+    ("creeping", BF16, 128, 2, 1, 0, 800), ("creeping", BF16, 64, 2, 1, 2000, 20), ("silent", BF16, 128, 2, 1, 0, 500), ("silent", BF16, 64, 2, 1, 1500, 30)])
 def test_a_prompt_row_goes_by_the_values_that_it_sees(kind, dtype, dim, group, heads, past, tokens):
     """Values of any spread: a row of small ones ahead of a later token's large ones; large ones whose weights leave the small ones what counts; blocks
-    of zeros that take weight. A term is 2^-11 off for its weight's rounding, whatever its value, or 2^-24 of the row's largest term: the bound that ``close`` has."""
+    of zeros that take weight. A term is 2^-11 off for its weight's rounding, whatever its value, or 2^-24 of what the row's largest weight could bring in its block's
+    scale: the bound that ``close`` has."""
     n = past + tokens
     p = Pair(1, heads, group, dim, dtype, pages=n // 16 + 2, seed=n + dim)
     k, v = (vectors(p.gen, 1, heads, n, dim, F32, large=False) for _ in range(2))
@@ -387,6 +390,21 @@ def test_a_prompt_row_goes_by_the_values_that_it_sees(kind, dtype, dim, group, h
         k[..., 0] = torch.where(torch.arange(n) < 128, 0.0, -710.0)
         q[..., 0] = dim ** 0.5
         v *= torch.exp2(30.0 - 60 * (block % 2))[:, None]
+    elif kind == "own block":                          # the last token's block holds nothing else: its tokens before it are zeros by its scale
+        v[..., n - 1, :] *= 2.0 ** 40
+    elif kind in ("rare", "first", "creeping"):
+        # tokens of large values under weights of 2^-100 and less, whose blocks hold nothing else: now and then; in the first key tile; behind it ever larger ones, and
+        # ordinary values at the end
+        at = torch.arange(n)
+        loud = {"rare": at % 53 == 31, "first": (at < 128) & (at % 16 == 5), "creeping": (at % 16 == 3) & (at >= 128) & (at < n - 200)}[kind]
+        power = (at // 128 * 10).clamp(max=60).float() if kind == "creeping" else torch.full((n,), 40.0)
+        k[..., 0] = torch.where(loud, -70.0 - power / 2, 0.0)
+        q[..., 0] = dim ** 0.5
+        v *= torch.where(loud, torch.exp2(power + 8), 1.0)[:, None]
+    elif kind == "silent":                             # what takes nearly all weight has values of zero; what is left holds some 2^-12 of it
+        k[..., 0] = torch.where(torch.arange(n) < 140, 8.0, 0.0)
+        q[..., 0] = dim ** 0.5
+        v[..., :140, :] = 0
     elif kind == "zeros":
         v *= (block % 40 >= 20).float()[:, None]
     else:                                              # products of -1e36: the first token is all that counts
