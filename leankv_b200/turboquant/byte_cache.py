@@ -156,6 +156,8 @@ class ByteKVCache(PagedKVCache):
         self._block_table = torch.empty(self._batch_cap, self._pps_cap, dtype=i32, device=dev)
         if table is not None:
             self._block_table[:len(table)] = table
+            if table.is_cuda:                                # it may be of another stream than the copy's
+                table.record_stream(torch.cuda.current_stream(dev))
         at = lambda t: ctypes.c_void_p(t.data_ptr())      # converted once, not at every call
         self._step_args = (at(self._seq_len_dev), at(self._block_table), ctypes.c_int(self._pps_cap), at(self._free_stack), at(self._free_top),
                            at(self._kv_indptr), at(self._kv_page_indices), at(self._kv_last), at(self._start_dev), at(self._status))

@@ -958,6 +958,27 @@ def test_a_graph_from_before_the_table_grew_answers_for_what_the_sequences_hold(
     del held
 
 
+def test_a_table_that_grows_on_another_stream_is_copied_before_its_memory_is_used_again():
+    """The cache was made on the default stream, which goes on taking memory while the growth waits on a busy one."""
+    p = Pair(3, 1, 2, 64, F16, pages=4096)
+    p.append(200, batch=1)
+    k, v = (vectors(p.gen, 3, 1, 20, 64, F16) for _ in range(2))
+    on = k.to(DEV), v.to(DEV)
+    torch.cuda.synchronize()
+    held = len(p.cache._block_table)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)                  # some 10 ms
+        p.cache.append(0, *on)
+    p.plain.append(k, v)
+    for _ in range(4):                                 # of the old table's size
+        torch.full((held, 4096), 77, dtype=torch.int32, device=DEV)
+    torch.cuda.synchronize()
+    assert len(p.cache._block_table) == 3
+    p.check_pages()
+    p.check_decode()
+
+
 def test_two_caches_on_two_streams_at_once():
     pairs = [Pair(2, 2, 4, 128, BF16, pages=400, seed=21), Pair(1, 4, 3, 64, F16, pages=600, seed=22)]
     calls = []
